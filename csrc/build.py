@@ -55,6 +55,11 @@ def _write_stamp(target: str, digest: str):
         f.write(digest + "\n")
 
 
+#: no packed fp32 arithmetic (v_pk_add / mul / fma_f32): -O3 forms it from ordinary float code, and
+#: some of its forms have given wrong results without an error.  (hipcc's host pass does not
+#: know the feature and says so: harmless.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 #: per-source code-generation flags.  score_bf16.hip: MFMA accumulators in VGPRs (the
 #: default form kept them in AGPRs, and every 32 x 32 block's filter first copied its 16
 #: scores out with v_accvgpr_read: 16 of the ~30 vector instructions per 4 MFMAs)
@@ -91,7 +96,7 @@ def build_kernels(force: bool = False, verbose: bool = True, variant: str = None
     hdrs = sorted(glob.glob(os.path.join(kdir, "*.h")))
     target = os.path.join(out, "libfps_kernels.so")
     flags = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result",
-             "-I", kdir] + [f"-D{d}" for d in defines]
+             "-I", kdir] + NO_PACKED_FP32 + [f"-D{d}" for d in defines]
 
     def obj(src):
         extra = PER_FILE_FLAGS.get(os.path.basename(src), [])
