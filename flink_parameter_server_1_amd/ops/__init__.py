@@ -1454,3 +1454,6 @@ def mf_sq_err(U, I, uid, iid, r) -> torch.Tensor:
                 "mf_sq_err")
         return out
     return torch.tensor([R.mf_sq_err(U, I, uid, iid, r)], dtype=torch.float64)
+
+
+from .mx import MX_FORMATS, MXTable, mx_gather_rows, mx_set_rows  # noqa: E402,F401  (uses the helpers above)

@@ -1,0 +1,203 @@
+"""Microscaled tables: rows in 4 or 8 bits per value, written by index, read back and scored.
+
+A row is cut into blocks of 32 consecutive values; a block is 32 elements and one shared
+power of two (an E8M0 byte ``s``, value ``2^(s - 127)``, 255 = NaN):
+
+* ``fp4``: E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives): 4.25 bits a value,
+  7.5x smaller than the fp32 table it is written from;
+* ``fp8``: E4M3 elements (up to 448): 8.25 bits a value.
+
+The shared exponent is the largest magnitude's less the element format's largest
+(``floor(log2 max|x|) - 2`` or ``- 8``), elements are rounded to nearest even and saturated.
+A block that holds an infinity or a NaN reads back as NaN.  Every read of an element is
+exact in fp32 (and in bf16), so the only rounding is the write's: half an element step,
+``eps / 2`` of the element type relative to a value that does not saturate.
+
+Dispatch is by the table's device as for every op: the gfx950 kernels on a GPU, the plain
+PyTorch twin (``ops.reference``) on the CPU.  Nothing here is differentiated: tables are
+written from rows that the update kernels already produced.
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional
+
+import torch
+
+from . import _native as N
+from . import reference as R
+
+MX_BLOCK = 32
+#: bits per element of a table format
+MX_FORMATS = {"fp4": 4, "fp8": 8}
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _device_of(t: torch.Tensor):
+    """Context that makes ``t``'s GPU the current one (kernels launch on the current device)."""
+    if t.is_cuda and t.device.index != torch.cuda.current_device():
+        return torch.cuda.device(t.device)
+    return contextlib.nullcontext()
+
+
+def _same_device(what: str, *ts) -> None:
+    for t in ts[1:]:
+        if t is not None and t.device != ts[0].device:
+            raise ValueError(f"{what}: operands on {ts[0].device} and {t.device}")
+
+
+class MXTable:
+    """``rows x dim`` values in a microscaled format.
+
+    ``data`` uint8 ``[rows, dim_padded * bits / 8]`` (two fp4 elements per byte, the even
+    one in the low nibble), ``scale`` uint8 ``[rows, dim_padded / 32]``; ``dim_padded`` is
+    ``dim`` rounded up to 32, the elements behind ``dim`` are zero.
+    """
+
+    def __init__(self, rows: int, dim: int, fmt: str = "fp4", device="cpu"):
+        """A table of zero rows."""
+        bits, nblk = self._layout(rows, dim, fmt)
+        self._set(torch.zeros((rows, nblk * MX_BLOCK * bits // 8), dtype=torch.uint8, device=device),
+                  torch.zeros((rows, nblk), dtype=torch.uint8, device=device), dim, fmt)
+
+    @staticmethod
+    def _layout(rows: int, dim: int, fmt: str):
+        if fmt not in MX_FORMATS:
+            raise ValueError(f"MXTable: format must be one of {tuple(MX_FORMATS)}, not {fmt!r}")
+        if dim < 1 or rows < 0:
+            raise ValueError(f"MXTable: {rows} rows of {dim} values")
+        return MX_FORMATS[fmt], (dim + MX_BLOCK - 1) // MX_BLOCK
+
+    def _set(self, data, scale, dim, fmt):
+        self.data, self.scale, self.dim, self.fmt = data, scale, int(dim), fmt
+        self.bits = MX_FORMATS[fmt]
+        #: per-slot claim of an indexed write (-1 between writes), allocated by the first one
+        self._owner: Optional[torch.Tensor] = None
+
+    @classmethod
+    def wrap(cls, data: torch.Tensor, scale: torch.Tensor, dim: int, fmt: str = "fp4") -> "MXTable":
+        """A table over existing (contiguous) buffers, not copied.  The elements behind
+        ``dim`` must be zero codes."""
+        rows = data.shape[0] if data.dim() == 2 else -1
+        bits, nblk = cls._layout(max(rows, 0), dim, fmt)
+        if data.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise ValueError("MXTable.wrap: data and scale are uint8")
+        if rows < 0 or tuple(data.shape) != (rows, nblk * MX_BLOCK * bits // 8) or tuple(scale.shape) != (rows, nblk):
+            raise ValueError(f"MXTable.wrap: data {tuple(data.shape)}, scale {tuple(scale.shape)} do not hold {fmt} rows "
+                             f"of {dim} values")
+        if not (data.is_contiguous() and scale.is_contiguous()):
+            raise ValueError("MXTable.wrap: data and scale must be contiguous")
+        if data.data_ptr() % 16:
+            raise ValueError("MXTable.wrap: data must start on 16 bytes")
+        _same_device("MXTable.wrap", data, scale)
+        t = cls.__new__(cls)
+        t._set(data, scale, dim, fmt)
+        return t
+
+    @classmethod
+    def from_rows(cls, rows: torch.Tensor, fmt: str = "fp4") -> "MXTable":
+        """The table of the float rows ``rows [n, dim]`` (one launch on the GPU)."""
+        if rows.dim() != 2:
+            raise ValueError(f"MXTable.from_rows: expected [n, dim] rows, got {tuple(rows.shape)}")
+        n, dim = rows.shape
+        bits, nblk = cls._layout(n, dim, fmt)
+        t = cls.__new__(cls)
+        t._set(torch.empty((n, nblk * MX_BLOCK * bits // 8), dtype=torch.uint8, device=rows.device),
+               torch.empty((n, nblk), dtype=torch.uint8, device=rows.device), dim, fmt)
+        return mx_set_rows(t, None, rows)
+
+    @property
+    def rows(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + self.scale.numel()
+
+    def values(self, dtype=torch.float32) -> torch.Tensor:
+        """All rows as floats."""
+        return mx_gather_rows(self, None, out_dtype=dtype)
+
+
+def _index(what: str, table: MXTable, idx: torch.Tensor) -> torch.Tensor:
+    from . import DEBUG, check_index
+
+    if idx.dtype not in (torch.int32, torch.int64) or idx.dim() != 1 or not idx.is_contiguous():
+        raise ValueError(f"{what}: idx must be a contiguous 1-d int32 or int64 tensor")
+    _same_device(what, table.data, idx)
+    if DEBUG:
+        check_index(idx, table.rows, what, allow_negative=True)
+    return idx
+
+
+def mx_set_rows(table: MXTable, idx: Optional[torch.Tensor], rows: torch.Tensor) -> MXTable:
+    """Write ``table[idx[r]] = quantised(rows[r])`` in place; ``idx=None``: row ``r`` to slot ``r``.
+
+    ``rows [n, dim]`` fp32 / bf16 / fp16, contiguous.  An index outside ``[0, table.rows)`` is a
+    padding slot and skipped (as ``idx < 0`` of ``apply_rows``; ``FPS_DEBUG=1`` raises for one past
+    the table); where an index repeats, the last of its rows is stored whole.  Slots that no row
+    names stay as they were.  Calls on one table from several streams must not name the same slot.
+    The first indexed write of a table (of more than one row) allocates 4 bytes per slot, waits
+    for its stream once and cannot be captured into a graph; later ones can."""
+    if rows.dim() != 2 or rows.shape[1] != table.dim or rows.dtype not in _TYPE:
+        raise ValueError(f"mx_set_rows: rows must be fp32 / bf16 / fp16 [n, {table.dim}], got {rows.dtype} "
+                         f"{tuple(rows.shape)}")
+    if not rows.is_contiguous():
+        raise ValueError("mx_set_rows: rows must be contiguous")
+    _same_device("mx_set_rows", table.data, rows)
+    n = rows.shape[0]
+    if idx is None:
+        if n > table.rows:
+            raise ValueError(f"mx_set_rows: {n} rows into a table of {table.rows}")
+    else:
+        idx = _index("mx_set_rows", table, idx)
+        if idx.numel() != n:
+            raise ValueError(f"mx_set_rows: {idx.numel()} indices for {n} rows")
+    if not rows.is_cuda:
+        R.mx_set_rows(table.data, table.scale, table.bits, idx, rows)
+        return table
+    with _device_of(rows):
+        if idx is not None and n > 1 and table._owner is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("mx_set_rows: a table's first indexed write allocates its claims: run it once "
+                                   "before capturing")
+            table._owner = torch.full((table.rows,), -1, dtype=torch.int32, device=table.device)
+            torch.cuda.current_stream().synchronize()  # once: writes from any stream find it filled
+        N.check(N.require().fps_mx_set_rows(rows.data_ptr(), _TYPE[rows.dtype], N.ptr(idx),
+                                            int(idx is not None and idx.dtype == torch.int64), n, table.dim, table.rows,
+                                            table.data.data_ptr(), table.scale.data_ptr(), table.bits,
+                                            N.ptr(table._owner) if idx is not None else None,
+                                            N.stream_ptr(rows.device)), "mx_set_rows")
+    return table
+
+
+def mx_gather_rows(table: MXTable, idx: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                   out_dtype=torch.float32) -> torch.Tensor:
+    """Read rows back: ``out[r] = values of table[idx[r]]`` (``idx=None``: all rows), fp32 /
+    bf16 / fp16.  An index outside ``[0, table.rows)`` gives a zero row (as ``gather_rows``'
+    padding slots)."""
+    if idx is not None:
+        idx = _index("mx_gather_rows", table, idx)
+    n = table.rows if idx is None else idx.numel()
+    if out is None:
+        if out_dtype not in _TYPE:
+            raise ValueError(f"mx_gather_rows: out_dtype must be fp32, bf16 or fp16, not {out_dtype}")
+        out = torch.empty((n, table.dim), dtype=out_dtype, device=table.device)
+    else:
+        if tuple(out.shape) != (n, table.dim) or out.dtype not in _TYPE or not out.is_contiguous():
+            raise ValueError(f"mx_gather_rows: out must be contiguous fp32 / bf16 / fp16 [{n}, {table.dim}], got "
+                             f"{out.dtype} {tuple(out.shape)}")
+        _same_device("mx_gather_rows", table.data, out)
+    if not out.is_cuda:
+        out.copy_(R.mx_gather_rows(table.data, table.scale, table.bits, table.dim, idx))
+        return out
+    with _device_of(out):
+        N.check(N.require().fps_mx_gather_rows(table.data.data_ptr(), table.scale.data_ptr(), table.rows, table.dim,
+                                               table.bits, N.ptr(idx),
+                                               int(idx is not None and idx.dtype == torch.int64), n, out.data_ptr(),
+                                               _TYPE[out.dtype], N.stream_ptr(out.device)), "mx_gather_rows")
+    return out

@@ -557,3 +557,75 @@ def sgns_standard_batched(rows_in, rows_out, pos_c, pos_o, pos_neg, k, lr, d_in,
     d_out.index_add_(0, x.reshape(-1), (g.unsqueeze(2) * h.unsqueeze(1)).reshape(-1, h.shape[1]).to(d_out.dtype))
     d_in.index_add_(0, c, torch.einsum("pj,pjd->pd", g, X).to(d_in.dtype))
     return float(loss)
+
+
+# ---- microscaled tables (ops.mx) ----------------------------------------------------------
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e as fp32 for whole e in [-127, 127], exactly."""
+    return ((e.long() + 1023) << 52).view(torch.float64).float()
+
+
+def mx_encode(x: torch.Tensor, bits: int):
+    """``(data, scale)`` of float rows ``x [n, dim]``."""
+    n, dim = x.shape
+    nblk = (dim + 31) // 32
+    v = torch.zeros((n, nblk * 32), dtype=torch.float32, device=x.device)
+    v[:, :dim] = x.float()
+    v = v.view(n, nblk, 32)
+    field = v.abs().amax(2).view(torch.int32) >> 23  # NaN and infinity: 255
+    ok = torch.isfinite(v).all(2)
+    scale = torch.where(ok, (field - (2 if bits == 4 else 8)).clamp_min(0), torch.full_like(field, 255))
+    y = torch.where(ok[:, :, None], v * _pow2(127 - scale.clamp_max(254))[:, :, None], torch.zeros_like(v))
+    if bits == 8:
+        code = y.clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
+        return code.view(n, nblk * 32), scale.to(torch.uint8)
+    grid = torch.tensor(_E2M1, device=x.device)
+    mid = (grid[1:] + grid[:-1]) / 2
+    a = y.abs()
+    below, above = torch.bucketize(a, mid), torch.bucketize(a, mid, right=True)  # differ on a midpoint
+    code = torch.where(below % 2 == 0, below, above) + 8 * (torch.signbit(y) & ok[:, :, None]).long()
+    code = code.view(n, nblk * 16, 2)
+    return (code[:, :, 0] + 16 * code[:, :, 1]).to(torch.uint8), scale.to(torch.uint8)
+
+
+def mx_decode(data: torch.Tensor, scale: torch.Tensor, bits: int, dim: int) -> torch.Tensor:
+    """fp32 values of packed rows."""
+    n, nblk = scale.shape
+    if bits == 8:
+        v = data.view(torch.float8_e4m3fn).float()
+    else:
+        lut = torch.tensor(_E2M1 + tuple(-e for e in _E2M1), device=data.device)
+        b = data.long()
+        v = torch.stack([lut[b & 15], lut[b >> 4]], 2)
+    s = scale.long()
+    f = torch.where(s == 255, torch.full(s.shape, float("nan"), device=s.device), _pow2(s.clamp_max(254) - 127))
+    return (v.reshape(n, nblk, 32) * f[:, :, None]).reshape(n, nblk * 32)[:, :dim]
+
+
+def mx_set_rows(data, scale, bits: int, idx, rows) -> None:
+    q, s = mx_encode(rows, bits)
+    n, T = rows.shape[0], data.shape[0]
+    if idx is None:
+        data[:n], scale[:n] = q, s
+        return
+    i = idx.long()
+    live = (i >= 0) & (i < T)
+    pos = torch.arange(n, device=i.device)
+    owner = torch.full((T,), -1, dtype=torch.long, device=i.device)
+    owner.scatter_reduce_(0, i[live], pos[live], "amax")
+    win = pos[live][owner[i[live]] == pos[live]]  # the last row of every named slot
+    data[i[win]], scale[i[win]] = q[win], s[win]
+
+
+def mx_gather_rows(data, scale, bits: int, dim: int, idx) -> torch.Tensor:
+    if idx is None:
+        return mx_decode(data, scale, bits, dim)
+    i = idx.long()
+    live = (i >= 0) & (i < data.shape[0])
+    out = torch.zeros((i.numel(), dim), dtype=torch.float32, device=data.device)
+    out[live] = mx_decode(data[i[live]], scale[i[live]], bits, dim)
+    return out
