@@ -1456,4 +1456,4 @@ def mf_sq_err(U, I, uid, iid, r) -> torch.Tensor:
     return torch.tensor([R.mf_sq_err(U, I, uid, iid, r)], dtype=torch.float64)
 
 
-from .mx import MX_FORMATS, MXTable, mx_gather_rows, mx_set_rows  # noqa: E402,F401  (uses the helpers above)
+from .mx import MX_FORMATS, MXTable, mx_gather_rows, mx_score, mx_set_rows  # noqa: E402,F401  (uses the helpers above)

@@ -106,6 +106,7 @@ _SIGNATURES = {
                                c_vp, c_int],
     "fps_mx_set_rows": [c_vp, c_int, c_vp, c_int, c_i64, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_vp],
     "fps_mx_gather_rows": [c_vp, c_vp, c_i64, c_int, c_int, c_vp, c_int, c_i64, c_vp, c_int, c_vp],
+    "fps_mx_score": [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_i64, c_int, c_vp, c_int, c_i64, c_vp],
     "fps_sgns_rows": [c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp],
 }
 #: optional symbols (added by later kernel files); bound when present

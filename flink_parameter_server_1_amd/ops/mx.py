@@ -201,3 +201,49 @@ def mx_gather_rows(table: MXTable, idx: Optional[torch.Tensor] = None, out: Opti
                                                int(idx is not None and idx.dtype == torch.int64), n, out.data_ptr(),
                                                _TYPE[out.dtype], N.stream_ptr(out.device)), "mx_gather_rows")
     return out
+
+
+def mx_score(Q, X: MXTable, out: Optional[torch.Tensor] = None, out_dtype=torch.float32) -> torch.Tensor:
+    """Scores ``out[b, i] = <Q[b], X[i]>`` of every query with every row of a microscaled table
+    (K8's product, ``score_gemm``, against 4 or 8 bits).
+
+    ``Q``: bf16 queries ``[B, dim]`` (contiguous), or an fp4 ``MXTable`` against an fp4 ``X`` (both
+    sides in 4 bits).  ``out``: fp32 / bf16 / fp16 ``[B, rows]``, its rows may be strided (a column
+    slice of a wider score matrix).  Sums are held in fp32 and rounded once.  A NaN in a query row or
+    a NaN block in a table row makes its scores NaN."""
+    mx = isinstance(Q, MXTable)
+    if not isinstance(X, MXTable):
+        raise ValueError("mx_score: X must be an MXTable")
+    if mx:
+        if Q.fmt != "fp4" or X.fmt != "fp4":
+            raise ValueError(f"mx_score: {Q.fmt} queries against an {X.fmt} table: microscaled queries are fp4 against "
+                             "fp4 (pass bf16 queries otherwise)")
+        B, dim = Q.rows, Q.dim
+    else:
+        if Q.dim() != 2 or Q.dtype != torch.bfloat16 or not Q.is_contiguous():
+            raise ValueError(f"mx_score: queries must be contiguous bf16 [B, dim] or an fp4 MXTable, got {Q.dtype} "
+                             f"{tuple(Q.shape)}")
+        B, dim = Q.shape
+    if dim != X.dim:
+        raise ValueError(f"mx_score: queries of {dim} values, table rows of {X.dim}")
+    if out is None:
+        if out_dtype not in _TYPE:
+            raise ValueError(f"mx_score: out_dtype must be fp32, bf16 or fp16, not {out_dtype}")
+        out = torch.empty((B, X.rows), dtype=out_dtype, device=X.device)
+    elif tuple(out.shape) != (B, X.rows) or out.dtype not in _TYPE:
+        raise ValueError(f"mx_score: out must be fp32 / bf16 / fp16 [{B}, {X.rows}], got {out.dtype} {tuple(out.shape)}")
+    elif out.numel() and (out.stride(1) != 1 and X.rows > 1 or B > 1 and out.stride(0) < X.rows):
+        raise ValueError(f"mx_score: out's rows must be contiguous and apart, got strides {out.stride()}")
+    _same_device("mx_score", X.data, Q.data if mx else Q, out)
+    if out.numel() == 0:
+        return out
+    if not out.is_cuda:
+        q = R.mx_decode(Q.data, Q.scale, Q.bits, dim) if mx else Q.float()
+        out.copy_(q @ R.mx_decode(X.data, X.scale, X.bits, dim).t())
+        return out
+    ld = out.stride(0) if B > 1 else X.rows
+    with _device_of(out):
+        N.check(N.require().fps_mx_score(Q.data.data_ptr() if mx else Q.data_ptr(), Q.scale.data_ptr() if mx else None,
+                                         X.data.data_ptr(), X.scale.data_ptr(), X.bits, B, X.rows, dim,
+                                         out.data_ptr(), _TYPE[out.dtype], ld, N.stream_ptr(out.device)), "mx_score")
+    return out

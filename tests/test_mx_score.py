@@ -1,0 +1,161 @@
+"""Scores against microscaled tables (``ops.mx_score``) vs the inner products in 64 bits.
+
+Tolerance, derived before the first run: the operands are exact (bf16 or the table's own
+values; fp4 queries are the values they stand for), every product is exact in fp32, and the sum of
+D products in fp32 in any order is off by at most (D - 1) 2^-24 of the sum of magnitudes to first
+order; the matrix unit's own additions are allowed twice that (it may cut where a sum rounds).
+Rounding the result to 16 bits adds half a step (``eps / 2`` of the type), or half the smallest
+subnormal.
+"""
+import pytest
+import torch
+
+from flink_parameter_server_1_amd import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+FORMS = [("bf16", "fp4"), ("bf16", "fp8"), ("fp4", "fp4")]
+
+
+def make(n, dim, seed, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(n, dim, generator=g) * torch.exp(spread * torch.randn(n, 1, generator=g))
+
+
+def operands(B, N, dim, form, dev, seed=0, spread=1.0):
+    q, x = make(B, dim, seed, 0.3), make(N, dim, seed + 1, spread)
+    X = ops.MXTable.from_rows(x.to(dev), form[1])
+    Q = q.to(dev).bfloat16() if form[0] == "bf16" else ops.MXTable.from_rows(q.to(dev), "fp4")
+    return Q, X
+
+
+def floats(t):
+    return (t.values() if isinstance(t, ops.MXTable) else t).cpu().double()
+
+
+def check(S, Q, X):
+    q, x = floats(Q), floats(X)
+    want, mag = q @ x.t(), q.abs() @ x.abs().t()
+    S = S.cpu()
+    bound = 2 * q.shape[1] * 2.0**-24 * mag
+    info = torch.finfo(S.dtype)
+    if S.dtype != torch.float32:
+        bound = bound * (1 + info.eps) + want.abs() * (info.eps / 2)
+    bound = bound + info.tiny * info.eps / 2
+    off = (S.double() - want).abs()
+    finite = want.abs() < info.max
+    assert bool((off <= bound)[finite].all()), float((off / bound)[finite].max())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("B,N,dim", [(1, 1, 1), (1, 300, 64), (2, 257, 33), (5, 1000, 64), (33, 511, 300),
+                                     (31, 64, 1000), (64, 129, 96), (129, 700, 64), (130, 1030, 224), (3, 77, 4096),
+                                     (40, 513, 2080), (200, 255, 1056)])
+def test_against_64_bits(dev, form, B, N, dim):
+    Q, X = operands(B, N, dim, form, dev, seed=B + N + dim)
+    check(ops.mx_score(Q, X), Q, X)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [64, 75])
+def test_output_types_and_strided_rows(dev, form, dtype, N):
+    Q, X = operands(35, N, 64, form, dev, seed=5, spread=0.5)
+    check(ops.mx_score(Q, X, out_dtype=dtype), Q, X)
+    for width, first in ((N + 40, 0), (N + 41, 3)):  # column slices: even and odd strides and starts
+        big = torch.full((35, width), 9.0, dtype=dtype, device=dev)
+        view = big[:, first:first + N]
+        assert ops.mx_score(Q, X, out=view) is view
+        check(view, Q, X)
+        rest = torch.cat([big[:, :first], big[:, first + N:]], 1)
+        assert bool((rest == 9).all())  # nothing behind the scores is touched
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+def test_wide_scales(dev, form):
+    """Blocks 2^-40 .. 2^40 apart: the power of two of every block is its own."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(300, 320, generator=g)
+    e = torch.randint(-40, 41, (300, 10), generator=g)
+    x = x * torch.repeat_interleave(torch.exp2(e.float()), 32, 1)
+    q = torch.randn(9, 320, generator=g) * torch.repeat_interleave(torch.exp2(torch.randint(-30, 31, (9, 10), generator=g).float()), 32, 1)
+    X = ops.MXTable.from_rows(x.to(dev), form[1])
+    Q = q.to(dev).bfloat16() if form[0] == "bf16" else ops.MXTable.from_rows(q.to(dev))
+    check(ops.mx_score(Q, X), Q, X)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 300, 1024])
+def test_nan_rows_stay_in_their_rows(dev, form, dim):
+    q, x = make(40, dim, 1, 0.3), make(500, dim, 2)
+    x[17, dim - 1] = float("nan")
+    x[401, 3] = float("inf")
+    q[5, 2] = float("nan")
+    X = ops.MXTable.from_rows(x.to(dev), form[1])
+    Q = q.to(dev).bfloat16() if form[0] == "bf16" else ops.MXTable.from_rows(q.to(dev))
+    S = ops.mx_score(Q, X).cpu()
+    want = torch.zeros(40, 500, dtype=torch.bool)
+    want[5] = True
+    want[:, [17, 401]] = True
+    assert torch.equal(S.isnan(), want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_zero_rows_and_empty_operands(dev):
+    X = ops.MXTable(70, 64, "fp4", device=dev)
+    assert not ops.mx_score(torch.randn(3, 64, device=dev).bfloat16(), X).any()
+    assert ops.mx_score(torch.empty(0, 64, device=dev).bfloat16(), X).shape == (0, 70)
+    assert ops.mx_score(torch.randn(3, 64, device=dev).bfloat16(), ops.MXTable(0, 64, device=dev)).shape == (3, 0)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals(dev):
+    X = ops.MXTable(7, 64, "fp4", device=dev)
+    X8 = ops.MXTable(7, 64, "fp8", device=dev)
+    q = torch.zeros(2, 64, device=dev).bfloat16()
+    bad = [lambda: ops.mx_score(q.float(), X), lambda: ops.mx_score(q[:, :32].contiguous(), X),
+           lambda: ops.mx_score(q[0], X), lambda: ops.mx_score(torch.zeros(64, 2, device=dev).bfloat16().t(), X),
+           lambda: ops.mx_score(X, X8), lambda: ops.mx_score(X8, X8), lambda: ops.mx_score(X8, X),
+           lambda: ops.mx_score(q, X.values()), lambda: ops.mx_score(q, X, out_dtype=torch.float64),
+           lambda: ops.mx_score(q, X, out=torch.zeros(2, 8, device=dev)),
+           lambda: ops.mx_score(q, X, out=torch.zeros(7, 2, device=dev).t()),
+           lambda: ops.mx_score(q, X, out=torch.zeros(1, 7, device=dev).expand(2, 7))]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A score matrix of more than 2^32 bytes and 2^31 entries, a table of more than 2^31 bytes."""
+    N = 33_600_000  # 64 * N > 2^31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    X = ops.MXTable(N, 128, "fp4", device="cuda")
+    last = torch.randn(1000, 128, generator=g, device="cuda")
+    ops.mx_set_rows(X, torch.arange(N - 1000, N, device="cuda"), last)
+    q = torch.randn(65, 128, generator=g, device="cuda").bfloat16()
+    S = ops.mx_score(q, X, out_dtype=torch.bfloat16)
+    tail = ops.MXTable.from_rows(last, "fp4")
+    assert torch.equal(S[:, -1000:], ops.mx_score(q, tail, out_dtype=torch.bfloat16))
+    assert not S[64, :-1000].any()
+    back = ops.mx_gather_rows(X, torch.tensor([N - 1, 5, N - 1000], device="cuda"))
+    assert torch.equal(back[0], tail.values()[999]) and torch.equal(back[2], tail.values()[0]) and not back[1].any()
+
+
+@pytest.mark.gpu
+def test_replayed_scores_equal_eager_ones():
+    Q, X = operands(40, 3000, 64, ("bf16", "fp4"), "cuda", seed=9)
+    want = ops.mx_score(Q, X)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.mx_score(Q, X)
+    for k in range(3):
+        q = make(40, 64, 100 + k, 0.3).bfloat16()
+        Q.copy_(q)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.mx_score(Q, X))
+    assert want.shape == out.shape
