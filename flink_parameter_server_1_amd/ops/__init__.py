@@ -1457,3 +1457,4 @@ def mf_sq_err(U, I, uid, iid, r) -> torch.Tensor:
 
 
 from .mx import MX_FORMATS, MXTable, mx_gather_rows, mx_score, mx_set_rows  # noqa: E402,F401  (uses the helpers above)
+from .sample import sample_scores  # noqa: E402,F401

@@ -107,12 +107,15 @@ _SIGNATURES = {
     "fps_mx_set_rows": [c_vp, c_int, c_vp, c_int, c_i64, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_vp],
     "fps_mx_gather_rows": [c_vp, c_vp, c_i64, c_int, c_int, c_vp, c_int, c_i64, c_vp, c_int, c_vp],
     "fps_mx_score": [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_i64, c_int, c_vp, c_int, c_i64, c_vp],
+    "fps_sample_scores_ws_bytes": [c_i64, c_i64],
+    "fps_sample_scores": [c_vp, c_int, c_int, c_i64, c_i64, c_vp, c_vp, c_double, c_vp, c_i64, c_vp, c_double, c_vp,
+                          c_double, c_vp, c_vp, c_vp, c_vp],
     "fps_sgns_rows": [c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp],
 }
 #: optional symbols (added by later kernel files); bound when present
 OPTIONAL = {}
 #: launchers / sizers returning int64 (the rest return an int status)
-RESTYPE_I64 = {"fps_tile_partition_ws_ints", "fps_dedup_flags_ws_ints"}
+RESTYPE_I64 = {"fps_tile_partition_ws_ints", "fps_dedup_flags_ws_ints", "fps_sample_scores_ws_bytes"}
 
 
 def register(name, argtypes):

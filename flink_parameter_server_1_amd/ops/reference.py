@@ -629,3 +629,35 @@ def mx_gather_rows(data, scale, bits: int, dim: int, idx) -> torch.Tensor:
     out = torch.zeros((i.numel(), dim), dtype=torch.float32, device=data.device)
     out[live] = mx_decode(data[i[live]], scale[i[live]], bits, dim)
     return out
+
+
+def sample_scores(S, u, temperature, top_k, top_p, min_p):
+    """``(index int32[B], prob fp32[B])`` by sorting, in 64 bits."""
+    B, n = S.shape
+
+    def col(v):
+        v = v if torch.is_tensor(v) else torch.full((B,), float(v), dtype=torch.float64, device=S.device)
+        return v.double().view(B, 1)
+
+    T, k, p, q = col(temperature), col(top_k), col(top_p), col(min_p).clamp_max(1.0)
+    greedy = ~(T > 0)
+    s = S.float()
+    s = torch.where(torch.isnan(s), torch.full_like(s, float("-inf")), s + 0.0)
+    ss, order = torch.sort(s, dim=1, descending=True, stable=True)
+    best = ss[:, :1]
+    z = torch.where(ss == best, torch.zeros_like(ss, dtype=torch.float64),
+                    (ss.double() - best.double()) / torch.where(greedy, torch.ones_like(T), T))
+    w = torch.where(ss == float("-inf"), torch.zeros_like(z), torch.exp(z))
+    rank = torch.arange(n, device=S.device).view(1, n)
+    w = w * (((rank < k) | ~(k > 0)) & ((rank < 1) | ~greedy))
+    cum = w.cumsum(1)
+    w = w * ((cum - w < p * cum[:, -1:]) | ~(p < 1) | (rank < 1)) * ((w >= q) | ~(q > 0))
+    w = torch.zeros_like(w).scatter_(1, order, w)
+    cum = w.cumsum(1)
+    total = cum[:, -1:]
+    pos = torch.arange(n, device=S.device).view(1, n).expand(B, n)
+    first = torch.where((cum > u.double().view(B, 1) * total) & (w > 0), pos, torch.full_like(pos, n)).amin(1)
+    last = torch.where(w > 0, pos, torch.full_like(pos, -1)).amax(1)
+    idx = torch.where(first < n, first, last)
+    prob = w.gather(1, idx.clamp_min(0).view(B, 1)) / total
+    return idx.to(torch.int32), torch.where(idx >= 0, prob.view(B), torch.zeros_like(prob.view(B))).float()
