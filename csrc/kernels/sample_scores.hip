@@ -7,18 +7,20 @@
 //   min-p  of those, the ones with w_i >= min_p    (the best one has w = 1)
 //   answer the first index i with sum_{j <= i, j kept} w_j > u * sum_{j kept} w_j
 //
-// Bound by one read of the scores, so a long row is read once in full (stats pass: the
-// largest score of every segment of 256, and its mass where no top-k or top-p is asked
-// for); the finishing workgroup of a row then reads only segments whose largest score can
-// matter.  A row of up to 32768 scores takes one launch: its workgroup holds it in registers (up
-// to 4096) or reads it again from the cache.
+// Bound by one read of the scores, so a long row (> 32768) is read once in full where it can
+// be: the stats pass takes the largest score of every segment of 256 (and its mass, where
+// masses decide), and the finishing workgroup of a row then reads only segments whose
+// largest score can matter.  With a short top-k that is about k segments; without a cut it is
+// one.  Top-p alone needs the masses of all scores above its threshold: two more passes
+// over the row, spread over the chip (a histogram of mass, then the segments' masses above the
+// threshold's bin and a list of the scores inside it).  Shorter rows take one launch.
 //
-// Nothing is sorted.  Thresholds are found over 2048 bins of (max s - s) / T, 32 to an octave of
-// weight, and the few scores of the bin that holds the threshold are ranked against each
-// other; a bin with too many (ties, a very high T) is split by the bits of the scores.
-// Weights are computed in 64 bits: an answer depends on which side of u * total a sum of up
-// to N weights falls.  Where masses meet in atomics they are whole multiples of 2^-shift, so
-// their order does not matter; the other sums are in a fixed order.
+// Nothing is sorted.  Thresholds are found over bins of (max s - s) / T, and the scores of the
+// bin that holds the threshold are ranked against each other (up to 256 of them) or split
+// by the bits of the scores.  Weights are computed in 64 bits: an answer depends on
+// which side of u * total a sum of up to N weights falls.  Where masses meet in atomics they
+// are whole multiples of 2^-shift, so their order does not matter; the other sums are in a
+// fixed order.
 #include <hip/hip_fp16.h>
 
 #include "common.h"
@@ -31,16 +33,36 @@ enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
 
 constexpr int SEG = 256;        // scores per segment: one wave, four a lane
 constexpr int BINS = 2048;
-constexpr int THREADS = 1024;   // of the finishing workgroup
+constexpr int THREADS = 512;    // of a finishing workgroup
 constexpr int WAVES = THREADS / 64;
-constexpr int LIST = 2048;      // scores ranked against each other
-constexpr int SHORT_K = 512;    // top-k up to this may take its candidates from the segments' maxima
-constexpr int HIST_SEGS = 128;  // segments per workgroup of the histogram pass
+constexpr int PER = BINS / THREADS;   // bins per thread of a search
+constexpr int LIST = 2048;      // scores listed in LDS
+constexpr int RANK = 256;       // listed scores ranked against each other; more are split by bits
+constexpr int SHORT_K = 1024;   // top-k up to this lists its candidates
+constexpr int CACHED_SEGS = 128;     // segments of a row that takes one launch
+constexpr int PASS_SEGS = 128;  // segments per workgroup of the passes over long rows
+
+struct Entry {
+  uint32_t key;
+  int32_t idx;
+  uint64_t w;
+};
+
+// what the passes over a long row that cuts by mass alone share
+struct RowState {
+  int active;
+  float M, cb;     // largest score; bins per unit of score
+  int shift;
+  double target;   // p * total, in units of 2^-shift
+  uint64_t above;  // mass of the bins before `bin`
+  int bin;         // holds the threshold
+  uint32_t listed; // scores in it
+};
 
 struct Args {
   const void* s;
   int64_t ld, N, nseg;
-  int B, type, vec;
+  int B, vec;
   const float* u;
   // per row, or nullptr and the same for all rows
   const float* temperature; double temperature0;
@@ -50,11 +72,13 @@ struct Args {
   int32_t* out;
   float* prob;
   // workspace (long rows)
-  float* segmax;    // [B, nseg]
-  double* segmass;  // [B, nseg]
-  int32_t* segtie;  // [B, nseg]
-  uint32_t* hcount; // [B, BINS]
-  uint64_t* hmass;  // [B, BINS]
+  uint64_t* segmass; // [B, nseg] doubles (stats pass) or whole numbers (collect pass)
+  uint64_t* hmass;   // [B, BINS]     } rows that may cut by mass alone
+  Entry* list;       // [B, listcap]  }
+  RowState* state;   // [B]           }
+  float* segmax;     // [B, nseg]
+  int32_t* segtie;   // [B, nseg]
+  int listcap;
 };
 
 struct Row {
@@ -63,7 +87,7 @@ struct Row {
   int64_t k;     // 0: off
   bool cut_p, cut_min;
   __device__ bool direct() const { return k == 0 && !cut_p; }
-  __device__ bool short_list(int64_t nseg) const { return k > 0 && k <= SHORT_K && nseg >= k; }
+  __device__ bool by_mass() const { return k == 0 && cut_p; }
 };
 
 __device__ __forceinline__ Row row_settings(const Args& a, int b) {
@@ -95,11 +119,10 @@ __device__ __forceinline__ float score_of(uint32_t k) {
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // key_of(-inf)
 
 // 2^((s - M) c): interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 10
-// (relative error 3e-16), times the power of two
+// (relative error 3e-16), times the power of two.  Without branches: selects at the end.
 __device__ __forceinline__ double weight(float s, float M, double c) {
-  if (s == M) return 1.0;
-  const double t = ((double)s - (double)M) * c;
-  if (!(t > -1020.0)) return 0.0;
+  const double t0 = ((double)s - (double)M) * c;
+  const double t = t0 > -1020.0 ? t0 : -1020.0;  // also for NaN (both infinite)
   const double n = __builtin_rint(t), f = t - n;
   double p = 0x1.e6063bb9d7e13p-28;
   p = __builtin_fma(p, f, 0x1.b675bcea1ca08p-24);
@@ -112,7 +135,8 @@ __device__ __forceinline__ double weight(float s, float M, double c) {
   p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
   p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
   p = __builtin_fma(p, f, 1.0);
-  return __longlong_as_double(__double_as_longlong(p) + ((int64_t)(int)n << 52));
+  const double w = __longlong_as_double(__double_as_longlong(p) + ((int64_t)(int)n << 52));
+  return s == M ? 1.0 : t0 > -1020.0 ? w : 0.0;
 }
 
 // w in [0, 1] as a whole multiple of 2^-shift, shift <= 51 (rounded to nearest even)
@@ -121,31 +145,29 @@ __device__ __forceinline__ uint64_t fixed(double w, int shift) {
   const double d = __builtin_fma(w, (double)(1ull << shift), magic);
   return (uint64_t)__double_as_longlong(d) & 0x000fffffffffffffull;
 }
-// N weights must not pass 2^63
-__device__ __forceinline__ int shift_for(int64_t N) { return min(51, 62 - (64 - __clzll((uint64_t)N))); }
+// a total of weights up to `total` must not pass 2^62
+__device__ __forceinline__ int shift_for(double total) {
+  return min(51, 61 - (int)((__double_as_longlong(total) >> 52) - 1023));
+}
 
 __device__ __forceinline__ int bin_of(float s, float M, float cb) {
-  if (s == M) return 0;
-  return (int)fminf((M - s) * cb, (float)(BINS - 1));
+  const float x = fminf((M - s) * cb, (float)(BINS - 1));
+  return s == M ? 0 : (int)x;
 }
 
 template <int T>
 __device__ __forceinline__ float load1(const void* p, int64_t i) {
-  float f;
-  if (T == T_F32) f = ((const float*)p)[i];
-  else {
-    const uint16_t b = ((const uint16_t*)p)[i];
-    f = T == T_BF16 ? bf16_to_f32(b) : __half2float(__ushort_as_half(b));
-  }
-  return f;
+  if (T == T_F32) return ((const float*)p)[i];
+  const uint16_t b = ((const uint16_t*)p)[i];
+  return T == T_BF16 ? bf16_to_f32(b) : __half2float(__ushort_as_half(b));
 }
 
 // NaN is masked; -0 and +0 are one score
 __device__ __forceinline__ float clean(float f) { return f == f ? f + 0.f : -INFINITY; }
 
-// this lane's four scores of a segment; places past the row are masked
+// this lane's four scores of a segment as they lie in memory; places past the row are masked
 template <int T>
-__device__ __forceinline__ void load_seg(const Args& a, int b, int64_t seg, int lane, float v[4]) {
+__device__ __forceinline__ void load_raw(const Args& a, int b, int64_t seg, int lane, float v[4]) {
   const int64_t i = seg * SEG + lane * 4, at = (int64_t)b * a.ld + i;
   if (a.vec && i + 4 <= a.N) {
     if (T == T_F32) {
@@ -165,118 +187,151 @@ __device__ __forceinline__ void load_seg(const Args& a, int b, int64_t seg, int 
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = i + j < a.N ? load1<T>(a.s, at + j) : -INFINITY;
   }
+}
+template <int T>
+__device__ __forceinline__ void load_seg(const Args& a, int b, int64_t seg, int lane, float v[4]) {
+  load_raw<T>(a, b, seg, lane, v);
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = clean(v[j]);
 }
+__device__ __forceinline__ float max4(const float v[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
 
-__device__ __forceinline__ float wave_max(float v) { return group_max<64>(v); }
-
+// ---- wave and workgroup sums ---------------------------------------------------------------
+// A step of a 64-lane scan: the value `from` lanes below inside rows of 16 (CTRL 0x111 .. 0x118), or
+// the last of the row(s) before (0x142, 0x143); 0 where there is none.  Register moves
+// between lanes: a step costs a few cycles where a shuffle through LDS costs ~100.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lanes_below(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lanes_below(uint64_t v) {
+  return (uint64_t)lanes_below<CTRL, ROWS>((uint32_t)v) | ((uint64_t)lanes_below<CTRL, ROWS>((uint32_t)(v >> 32)) << 32);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lanes_below(double v) {
+  return __longlong_as_double((int64_t)lanes_below<CTRL, ROWS>((uint64_t)__double_as_longlong(v)));
+}
+// inclusive sum over the lanes of the wave (all 64 active)
 template <typename V>
-__device__ __forceinline__ V wave_sum(V v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+__device__ __forceinline__ V wave_scan(V v) {
+  v += lanes_below<0x111, 0xf>(v);
+  v += lanes_below<0x112, 0xf>(v);
+  v += lanes_below<0x114, 0xf>(v);
+  v += lanes_below<0x118, 0xf>(v);
+  v += lanes_below<0x142, 0xa>(v);
+  v += lanes_below<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int l) {
+  return (uint64_t)lane_value((uint32_t)v, l) | ((uint64_t)lane_value((uint32_t)(v >> 32), l) << 32);
+}
+__device__ __forceinline__ double lane_value(double v, int l) {
+  return __longlong_as_double((int64_t)lane_value((uint64_t)__double_as_longlong(v), l));
+}
+template <typename V>
+__device__ __forceinline__ V wave_sum(V v) { return lane_value(wave_scan(v), 63); }
 
-// ---- long rows, pass 1: the largest score of every segment, its mass for direct rows --------
-constexpr int STAT_SEGS = 8;  // per wave
-template <int T>
-__global__ void __launch_bounds__(256) stats_kernel(Args a, int hist) {
-  const int b = blockIdx.y, lane = threadIdx.x & 63;
-  const Row r = row_settings(a, b);
-  if (hist)  // the histogram pass adds to these
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < BINS; i += gridDim.x * 256) {
-      a.hcount[(int64_t)b * BINS + i] = 0;
-      a.hmass[(int64_t)b * BINS + i] = 0;
-    }
-  const int64_t seg0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * STAT_SEGS;
-  const bool mass = r.direct() && !r.cut_min;
-#pragma unroll 4
-  for (int j = 0; j < STAT_SEGS; ++j) {
-    const int64_t seg = seg0 + j;
-    if (seg >= a.nseg) return;
-    float v[4];
-    load_seg<T>(a, b, seg, lane, v);
-    const float m = wave_max(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-    double w = 0;
-    if (mass && m > -INFINITY) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w += weight(v[i], m, r.c);
-      w = wave_sum(w);
-    }
-    if (lane == 0) {
-      a.segmax[(int64_t)b * a.nseg + seg] = m;
-      if (mass) a.segmass[(int64_t)b * a.nseg + seg] = w;
-    }
-  }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_below(float v) {
+  const int none = (int)0xff800000u;  // -inf
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(none, __float_as_int(v), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = max_below<0x111, 0xf>(v);
+  v = max_below<0x112, 0xf>(v);
+  v = max_below<0x114, 0xf>(v);
+  v = max_below<0x118, 0xf>(v);
+  v = max_below<0x142, 0xa>(v);
+  v = max_below<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// inclusive sum over the workgroup in thread order, and the total; tmp: one V per wave
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* tmp, V& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  v = wave_scan(v);
+  __syncthreads();
+  if (lane == 63) tmp[wave] = v;
+  __syncthreads();
+  V t = lane < nw ? tmp[lane] : V(0);
+  t = wave_scan(t);
+  total = lane_value(t, nw - 1);
+  return wave ? lane_value(t, wave - 1) + v : v;
 }
 
 __device__ __forceinline__ float block_max(float v, float* tmp) {
   v = wave_max(v);
-  const int nw = blockDim.x >> 6;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
   __syncthreads();
+  const int nw = blockDim.x >> 6;
   float m = tmp[0];
   for (int i = 1; i < nw; ++i) m = fmaxf(m, tmp[i]);
   return m;
 }
 
+// ---- long rows, pass 1: the largest score of every segment, its mass where masses decide ----
+constexpr int STAT_SEGS = 8;  // per wave: 8 loads in flight a lane
+template <int T>
+__global__ void __launch_bounds__(256) stats_kernel(Args a) {
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const Row r = row_settings(a, b);
+  const int64_t seg0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * STAT_SEGS;
+  if (seg0 >= a.nseg) return;
+  const bool mass = r.k == 0 && !(r.direct() && r.cut_min);
+  float v[STAT_SEGS][4];
+#pragma unroll
+  for (int j = 0; j < STAT_SEGS; ++j) load_raw<T>(a, b, min(seg0 + j, a.nseg - 1), lane, v[j]);
+  float ms = -INFINITY;
+  double ws = 0;
+#pragma unroll
+  for (int j = 0; j < STAT_SEGS; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[j][i] = clean(v[j][i]);
+    const float m = wave_max(max4(v[j]));
+    if (lane == j) ms = m;
+    if (mass) {
+      double w = 0;
+      if (m > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w += weight(v[j][i], m, r.c);
+        w = wave_sum(w);
+      }
+      if (lane == j) ws = w;
+    }
+  }
+  if (lane < STAT_SEGS && seg0 + lane < a.nseg) {
+    const int64_t at = (int64_t)b * a.nseg + seg0 + lane;
+    a.segmax[at] = ms;
+    if (mass) a.segmass[at] = (uint64_t)__double_as_longlong(ws);
+  }
+}
+
+// ---- histograms ----------------------------------------------------------------------------
+
 // add one score to a histogram in LDS; a wave whose lanes all hit one bin adds once
+template <bool COUNT, bool MASS>
 __device__ __forceinline__ void hist_add(uint32_t* hc, unsigned long long* hm, bool on, int bin, uint64_t w) {
   const uint64_t live = __ballot(on);
   if (live == 0) return;
-  const int first = __shfl(bin, __ffsll((unsigned long long)live) - 1, 64);
+  const int first = __builtin_amdgcn_readlane(bin, __ffsll((unsigned long long)live) - 1);
   if (__ballot(on && bin == first) == live) {
-    const uint64_t sum = wave_sum(on ? w : 0ull);
+    uint64_t sum = 0;
+    if (MASS) sum = wave_sum(on ? w : (uint64_t)0);
     if ((threadIdx.x & 63) == 0) {
-      atomicAdd(hc + first, (uint32_t)__popcll(live));
-      atomicAdd(hm + first, (unsigned long long)sum);
+      if (COUNT) atomicAdd(hc + first, (uint32_t)__popcll(live));
+      if (MASS) atomicAdd(hm + first, (unsigned long long)sum);
     }
   } else if (on) {
-    atomicAdd(hc + bin, 1u);
-    atomicAdd(hm + bin, (unsigned long long)w);
+    if (COUNT) atomicAdd(hc + bin, 1u);
+    if (MASS) atomicAdd(hm + bin, (unsigned long long)w);
   }
 }
-
-// ---- long rows, pass 2 (rows that cut by mass, or by a long top-k): counts and masses by bin ---
-template <int T>
-__global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
-  __shared__ uint32_t hc[BINS];
-  __shared__ unsigned long long hm[BINS];
-  __shared__ float tmp[WAVES];
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Row r = row_settings(a, b);
-  if (r.direct() || r.short_list(a.nseg)) return;
-  for (int i = threadIdx.x; i < BINS; i += THREADS) { hc[i] = 0; hm[i] = 0; }
-  float m = -INFINITY;
-  for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) m = fmaxf(m, a.segmax[(int64_t)b * a.nseg + i]);
-  const float M = block_max(m, tmp);
-  if (M == -INFINITY) return;
-  const int shift = shift_for(a.N);
-  const float cb = (float)(r.c * 32);
-  const int64_t s0 = (int64_t)blockIdx.x * HIST_SEGS;
-  for (int64_t seg = s0 + wave; seg < s0 + HIST_SEGS && seg < a.nseg; seg += WAVES) {
-    float v[4];
-    load_seg<T>(a, b, seg, lane, v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) hist_add(hc, hm, v[j] > -INFINITY, bin_of(v[j], M, cb), fixed(weight(v[j], M, r.c), shift));
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += THREADS)
-    if (hc[i]) {
-      atomicAdd(a.hcount + (int64_t)b * BINS + i, hc[i]);
-      atomicAdd((unsigned long long*)a.hmass + (int64_t)b * BINS + i, hm[i]);
-    }
-}
-
-// ---- the finishing workgroup of a row ------------------------------------------------------
-
-struct Entry {
-  uint32_t key;
-  int32_t idx;
-  uint64_t w;
-};
 
 struct Shared {
   uint32_t hc[BINS];
@@ -284,21 +339,81 @@ struct Shared {
   Entry list[LIST];
   float tmp[WAVES];
   uint32_t scan_c[WAVES];
-  unsigned long long scan_m[WAVES];
+  uint64_t scan_m[WAVES];
   double scan_d[WAVES];
   // results of searches, written by one thread
   int bin, n, best;
   uint32_t kmin, ties, before_c;
-  unsigned long long before_m, total_m, kept_m;
-  int64_t seg;
-  double seg_before, seg_mass;
+  unsigned long long before_m, kept_m;
 };
 
-// Where the finishing workgroup has the row: its one segment per wave in registers
-// (ROW_REGS), or in memory, the segments' maxima in LDS (ROW_CACHED) or from the stats
-// pass (ROW_LONG).
+__device__ __forceinline__ void clear_hist(Shared& sh) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += THREADS) { sh.hc[i] = 0; sh.hm[i] = 0; }
+  __syncthreads();
+}
+
+// The bin of the histogram in sh (bin 0 best) in which the count first reaches `need` (by_mass
+// false) or the mass, added to `above`, first reaches `target`: sh.bin, and what lies before it:
+// sh.before_c, sh.before_m.  Where rounding lets no bin reach it: the last bin that holds
+// anything.  By count the masses are summed only with `masses`.
+__device__ __forceinline__ void find_bin(Shared& sh, bool by_mass, bool masses, uint32_t need, uint64_t above,
+                                         double target) {
+  const int i = threadIdx.x;
+  uint32_t c[PER], ct = 0, call;
+  uint64_t m[PER], mt = 0, mall;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    c[j] = sh.hc[PER * i + j];
+    m[j] = sh.hm[PER * i + j];
+    ct += c[j];
+    mt += m[j];
+  }
+  uint32_t cc = 0;
+  uint64_t mm = 0;
+  if (i == 0) { sh.bin = BINS; sh.best = -1; }
+  if (!by_mass) cc = block_scan(ct, sh.scan_c, call) - ct;
+  if (by_mass || masses) mm = block_scan(mt, sh.scan_m, mall) - mt;
+  int hit = -1, any = -1;
+  uint32_t c_at = 0;
+  uint64_t m_at = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const bool full = by_mass ? m[j] != 0 : c[j] != 0;
+    if (full) {
+      any = j;
+      if (hit < 0 && (by_mass ? (double)(above + mm + m[j]) >= target : cc + c[j] >= need)) { hit = j; c_at = cc; m_at = mm; }
+    }
+    cc += c[j];
+    mm += m[j];
+  }
+  if (hit >= 0) atomicMin(&sh.bin, PER * i + hit);
+  if (any >= 0) atomicMax(&sh.best, PER * i + any);
+  __syncthreads();
+  const bool none = sh.bin == BINS;
+  const int bin = none ? sh.best : sh.bin;
+  __syncthreads();
+  if (bin / PER == i && bin >= 0) {
+    if (none) {  // before the last bin: what this thread's scan holds, less that bin and the empty ones after it
+      const int j = bin - PER * i;
+      c_at = cc;
+      m_at = mm;
+#pragma unroll
+      for (int x = 0; x < PER; ++x)
+        if (x >= j) { c_at -= c[x]; m_at -= m[x]; }
+    }
+    sh.bin = bin;
+    sh.before_c = c_at;
+    sh.before_m = m_at;
+  }
+  __syncthreads();
+}
+
+// ---- the finishing workgroup of a row ------------------------------------------------------
+
+// Where it has the row: its one segment per wave in registers (ROW_REGS), or in memory, the
+// segments' maxima in LDS (ROW_CACHED) or from the stats pass (ROW_LONG).
 enum { ROW_REGS = 0, ROW_CACHED = 1, ROW_LONG = 2 };
-constexpr int CACHED_SEGS = 8 * WAVES;
 
 template <int T, int R>
 struct Source {
@@ -308,413 +423,484 @@ struct Source {
   float v[4];
   __device__ Source(const Args& a_, int b_, const float* sm)
       : a(a_), b(b_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), segmax(sm) {}
-  // f(segment, scores) for every segment whose largest score is >= bound, waves in turn
-  template <typename F>
-  __device__ __forceinline__ void each(float bound, F f) {
+  // f(segment, scores) for the segments whose largest score (not -inf) is wanted; the waves
+  // take them in turn.  64 maxima are looked at together, four segments are loaded together.
+  template <typename P, typename F>
+  __device__ __forceinline__ void each(P want, F f) {
     if constexpr (R == ROW_REGS) {
       if (wave < a.nseg) f((int64_t)wave, v);
     } else {
-      for (int64_t seg = wave; seg < a.nseg; seg += WAVES) {
-        if (segmax[seg] < bound || segmax[seg] == -INFINITY) continue;
-        float x[4];
-        load_seg<T>(a, b, seg, lane, x);
-        f(seg, x);
+      for (int64_t base = 0; base < a.nseg; base += 64 * WAVES) {
+        const int64_t at = base + wave + (int64_t)lane * WAVES;
+        float m = -INFINITY;
+        if (at < a.nseg) m = segmax[at];
+        uint64_t todo = __ballot(m > -INFINITY && want(m));
+        while (todo) {
+          float x[4][4];
+          int l[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            l[j] = todo ? __ffsll((unsigned long long)todo) - 1 : -1;
+            todo &= todo - 1;
+            if (l[j] >= 0) load_raw<T>(a, b, base + wave + (int64_t)l[j] * WAVES, lane, x[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (l[j] >= 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
+              f(base + wave + (int64_t)l[j] * WAVES, x[j]);
+            }
+        }
       }
     }
   }
 };
 
-// Inclusive sums over the workgroup of (count, mass), thread order.
-__device__ __forceinline__ void block_scan(uint32_t& c, uint64_t& m, Shared& sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t c2 = __shfl_up(c, o, 64);
-    const uint64_t m2 = __shfl_up((unsigned long long)m, o, 64);
-    if (lane >= o) { c += c2; m += m2; }
-  }
-  __syncthreads();
-  if (lane == 63) { sh.scan_c[wave] = c; sh.scan_m[wave] = m; }
-  __syncthreads();
-  for (int i = 0; i < wave; ++i) { c += sh.scan_c[i]; m += sh.scan_m[i]; }
-}
-
-__device__ __forceinline__ double block_scan_d(double d, Shared& sh, double& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double d2 = __shfl_up(d, o, 64);
-    if (lane >= o) d += d2;
-  }
-  __syncthreads();
-  if (lane == 63) sh.scan_d[wave] = d;
-  __syncthreads();
-  double before = 0;
-  total = 0;
-  for (int i = 0; i < WAVES; ++i) {
-    if (i == wave) before = total;
-    total += sh.scan_d[i];
-  }
-  return before + d;
-}
-
-// The bin of the histogram in sh (bin 0 best) in which the count first reaches `need` (by_mass
-// false) or the mass, added to `above`, first reaches `target`; sh.bin, sh.before_c, sh.before_m.
-// Where rounding lets no bin reach it: the last bin that holds anything.
-__device__ __forceinline__ void find_bin(Shared& sh, bool by_mass, uint32_t need, uint64_t above, double target) {
-  const int i = threadIdx.x;
-  const uint32_t c0 = sh.hc[2 * i], c1 = sh.hc[2 * i + 1];
-  const uint64_t m0 = sh.hm[2 * i], m1 = sh.hm[2 * i + 1];
-  uint32_t c = c0 + c1;
-  uint64_t m = m0 + m1;
-  block_scan(c, m, sh);
-  if (i == 0) { sh.bin = BINS; sh.best = -1; }
-  __syncthreads();
-  const uint32_t cb0 = c - c1;       // count through bin 2 i
-  const uint64_t mb0 = m - m1;
-  const bool h0 = c0 && (by_mass ? (double)(above + mb0) >= target : cb0 >= need);
-  const bool h1 = c1 && (by_mass ? (double)(above + m) >= target : c >= need);
-  if (h0) atomicMin(&sh.bin, 2 * i);
-  else if (h1) atomicMin(&sh.bin, 2 * i + 1);
-  if (c1) atomicMax(&sh.best, 2 * i + 1);
-  else if (c0) atomicMax(&sh.best, 2 * i);
-  __syncthreads();
-  const int bin = sh.bin < BINS ? sh.bin : sh.best;
-  if (bin == 2 * i) { sh.before_c = cb0 - c0; sh.before_m = mb0 - m0; }
-  else if (bin == 2 * i + 1) { sh.before_c = cb0; sh.before_m = mb0; }
-  if (i == THREADS - 1) sh.total_m = m;
-  __syncthreads();
-  if (i == 0) sh.bin = bin;
-  __syncthreads();
-}
-
-// Among the n listed scores, which stay: rank + above_c < k (k = 0: all), then, with `cut`,
-// mass before + above_m < p * total; sh.kept_m their mass after top-k alone, kept bits in the
-// caller's two slots (entries threadIdx.x and threadIdx.x + THREADS).
+// One listed score per thread (n <= RANK <= THREADS): is it among the best k (k = 0: all), given
+// above_c better ones outside the list, and what mass of the list is better than it.
 struct Slot {
-  bool in, kept;
+  bool kept;
   uint64_t before;
 };
 
-__device__ __forceinline__ void rank_list(Shared& sh, int n, int64_t k, uint32_t above_c, Slot s[2]) {
-  if (threadIdx.x == 0) sh.kept_m = 0;
+__device__ __forceinline__ Slot rank_list(Shared& sh, int n, int64_t k, uint32_t above_c) {
+  Slot s{false, 0};
+  const int i = threadIdx.x;
+  if (i == 0) sh.kept_m = 0;
   __syncthreads();
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = threadIdx.x + h * THREADS;
-    s[h].in = i < n;
-    s[h].kept = false;
-    s[h].before = 0;
-    if ((i & ~63) < n) {  // whole waves
-      const Entry e = sh.list[i < n ? i : 0];
-      uint32_t rank = 0;
-      uint64_t before = 0;
-      for (int j = 0; j < n; ++j) {
-        const Entry o = sh.list[j];
-        const bool better = o.key > e.key || (o.key == e.key && o.idx < e.idx);
-        rank += better;
-        before += better ? o.w : 0ull;
-      }
-      s[h].before = before;
-      s[h].kept = i < n && (k == 0 || (int64_t)above_c + rank < k);
-      const uint64_t sum = wave_sum(s[h].kept ? e.w : 0ull);
-      if ((threadIdx.x & 63) == 0) atomicAdd(&sh.kept_m, (unsigned long long)sum);
+  if ((i & ~63) < n) {  // whole waves
+    const Entry e = sh.list[i < n ? i : 0];
+    uint32_t rank = 0;
+    uint64_t before = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const Entry o = sh.list[j];
+      const bool better = o.key > e.key || (o.key == e.key && o.idx < e.idx);
+      rank += better;
+      before += better ? o.w : (uint64_t)0;
     }
+    s.before = before;
+    s.kept = i < n && (k == 0 || (int64_t)above_c + rank < k);
+    const uint64_t sum = wave_sum(s.kept ? e.w : (uint64_t)0);
+    if ((i & 63) == 0) atomicAdd(&sh.kept_m, (unsigned long long)sum);  // the mass that top-k keeps of the list
   }
   __syncthreads();
+  return s;
 }
 
-__device__ __forceinline__ void cut_by_mass(Slot s[2], uint64_t above_m, double target) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (s[h].kept) {
-      const uint64_t before = above_m + s[h].before;
-      s[h].kept = before == 0 || (double)before < target;  // the best one always stays
-    }
+__device__ __forceinline__ void cut_by_mass(Slot& s, uint64_t above_m, double target) {
+  const uint64_t before = above_m + s.before;
+  s.kept = s.kept && (before == 0 || (double)before < target);  // the best one always stays
+}
+
+// the kept entries of the list as a threshold: smallest key, and how many of it
+__device__ __forceinline__ void list_threshold(Shared& sh, const Slot& s) {
+  if (threadIdx.x == 0) { sh.kmin = 0xffffffffu; sh.ties = 0; }
+  __syncthreads();
+  const uint32_t key = s.kept ? sh.list[threadIdx.x].key : 0;
+  if (s.kept) atomicMin(&sh.kmin, key);
+  __syncthreads();
+  if (s.kept && key == sh.kmin) atomicAdd(&sh.ties, 1u);
+  __syncthreads();
 }
 
 // Put the scores for which pick(key, bin) holds into sh.list; sh.n counts them all.
-template <int T, int R, typename F>
-__device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float bound, float M, const Row& r, float cb,
-                                        int shift, F pick) {
+template <int T, int R, typename P, typename F>
+__device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, const Row& r, float cb, int shift,
+                                        P want, F pick) {
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  src.each(bound, [&](int64_t seg, const float* v) {
+  src.each(want, [&](int64_t seg, const float* v) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool on = v[j] > -INFINITY && pick(key_of(v[j]), bin_of(v[j], M, cb));
-      if (on) {
+    for (int j = 0; j < 4; ++j)
+      if (v[j] > -INFINITY && pick(key_of(v[j]), bin_of(v[j], M, cb))) {
         const int at = atomicAdd(&sh.n, 1);
         if (at < LIST)
           sh.list[at] = Entry{key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), fixed(weight(v[j], M, r.c), shift)};
       }
-    }
   });
   __syncthreads();
 }
 
-// Split bin `bin` by the bits of the scores until one score value is left: the threshold key
-// sh.kmin and how many scores equal to it stay (sh.ties).  By count: `need` of the bin's scores
-// stay; by mass: those before which above_m + mass < target.  Only keys >= floor take part.
-template <int T, int R>
-__device__ __forceinline__ void split_bin(Source<T, R>& src, Shared& sh, float bound, float M, const Row& r, float cb,
-                                          int shift, int bin, bool by_mass, uint32_t need, uint64_t above_m,
-                                          double target, uint32_t floor_key) {
+// Split a set of scores by their bits until one score value is left: the threshold key sh.kmin, how
+// many scores equal to it stay (sh.ties) and the mass above it (sh.before_m).  By count: `need` of
+// the set stay; by mass: those before which above_m + mass < target.  Only keys >= floor_key take
+// part.  each(g) calls g(on, key, w) for the set, all lanes of a wave together.
+template <typename E>
+__device__ __forceinline__ void split(Shared& sh, E each, bool by_mass, uint32_t need, uint64_t above_m, double target,
+                                      uint32_t floor_key) {
   uint32_t prefix = 0, mask = 0;
   for (int level = 0; level < 3; ++level) {
     const int sft = level == 0 ? 21 : level == 1 ? 10 : 0;
     const uint32_t width = level == 2 ? 1023u : 2047u;
-    __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += THREADS) { sh.hc[i] = 0; sh.hm[i] = 0; }
-    __syncthreads();
-    src.each(bound, [&](int64_t, const float* v) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t key = key_of(v[j]);
-        const bool on = v[j] > -INFINITY && bin_of(v[j], M, cb) == bin && (key & mask) == prefix && key >= floor_key;
-        hist_add(sh.hc, sh.hm, on, (int)(width - ((key >> sft) & width)), on ? fixed(weight(v[j], M, r.c), shift) : 0);
-      }
+    clear_hist(sh);
+    each([&](bool on, uint32_t key, uint64_t w) {
+      hist_add<true, true>(sh.hc, sh.hm, on && (key & mask) == prefix && key >= floor_key,
+                           (int)(width - ((key >> sft) & width)), w);
     });
     __syncthreads();
-    find_bin(sh, by_mass, need, above_m, target);
+    find_bin(sh, by_mass, true, need, above_m, target);
     prefix |= (width - (uint32_t)sh.bin) << sft;
     mask |= width << sft;
     need -= min(need, sh.before_c);
     above_m += sh.before_m;
-    if (level == 2) {
-      const uint32_t cnt = sh.hc[sh.bin];
-      uint32_t ties = need;
-      if (by_mass) {  // tie number j stays while above + j w < target
-        const uint64_t w = cnt ? sh.hm[sh.bin] / cnt : 0;
-        const double room = target - (double)above_m;
-        ties = w == 0 || room > (double)w * (double)cnt ? cnt : (uint32_t)fmax(0.0, ceil(room / (double)w));
-        if (above_m == 0 && ties == 0) ties = 1;
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) { sh.kmin = prefix; sh.ties = min(ties, cnt); sh.before_m = above_m; }
+  }
+  const uint32_t cnt = sh.hc[sh.bin];
+  uint32_t ties = need;
+  if (by_mass) {  // tie number j stays while above + j w < target
+    const uint64_t w = cnt ? sh.hm[sh.bin] / cnt : 0;
+    const double room = target - (double)above_m;
+    ties = w == 0 || room > (double)w * (double)cnt ? cnt : (uint32_t)fmax(0.0, ceil(room / (double)w));
+    if (above_m == 0 && ties == 0) ties = 1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) { sh.kmin = prefix; sh.ties = min(ties, cnt); sh.before_m = above_m; }
+  __syncthreads();
+}
+
+// the first n of `list` for split()
+template <typename G>
+__device__ __forceinline__ void each_listed(const Entry* list, int n, G g) {
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    const int i = i0 + threadIdx.x;
+    Entry e{0, 0, 0};
+    if (i < n) e = list[i];
+    g(i < n, e.key, e.w);
+  }
+}
+
+// Draw from the kept entries of the list (n <= RANK), in index order.
+__device__ __forceinline__ void draw_from_list(const Args& a, int b, Shared& sh, int n, Slot s, const Row& r, float M) {
+  const int i = threadIdx.x;
+  __syncthreads();
+  Entry mine{0, 0, 0};
+  if (i < n) mine = sh.list[i];
+  if (s.kept && r.cut_min) s.kept = weight(score_of(mine.key), M, r.c) >= r.minp;
+  if (!s.kept) mine.w = 0;
+  if (i < n) sh.list[i].w = mine.w;
+  if (i == 0) { sh.best = INT32_MAX; sh.bin = -1; }
+  uint64_t all;
+  block_scan(mine.w, sh.scan_m, all);
+  const double total = (double)all, target = (double)a.u[b] * total;
+  __syncthreads();
+  if ((i & ~63) < n) {
+    uint64_t cum = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const Entry o = sh.list[j];
+      cum += o.idx <= mine.idx ? o.w : (uint64_t)0;
     }
-    __syncthreads();
-  }
-}
-
-// the kept entries of the list as a threshold: smallest key, and how many of it
-__device__ __forceinline__ void list_threshold(Shared& sh, const Slot s[2]) {
-  if (threadIdx.x == 0) { sh.kmin = 0xffffffffu; sh.ties = 0; }
-  __syncthreads();
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (s[h].kept) atomicMin(&sh.kmin, sh.list[threadIdx.x + h * THREADS].key);
-  __syncthreads();
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (s[h].kept && sh.list[threadIdx.x + h * THREADS].key == sh.kmin) atomicAdd(&sh.ties, 1u);
-  __syncthreads();
-}
-
-// Draw from the kept entries of the list, in index order.
-__device__ __forceinline__ void draw_from_list(const Args& a, int b, Shared& sh, int n, Slot s[2], const Row& r, float M) {
-  __syncthreads();
-  if (threadIdx.x == 0) { sh.kept_m = 0; sh.best = INT32_MAX; sh.bin = -1; }
-  __syncthreads();
-  Entry mine[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = threadIdx.x + h * THREADS;
-    mine[h] = sh.list[i < n ? i : 0];
-    if (s[h].kept && r.cut_min) s[h].kept = weight(score_of(mine[h].key), M, r.c) >= r.minp;
-    if (!s[h].kept) mine[h].w = 0;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = threadIdx.x + h * THREADS;
-    if (i < n) sh.list[i].w = mine[h].w;
-    const uint64_t sum = wave_sum(mine[h].w);
-    if ((threadIdx.x & 63) == 0) atomicAdd(&sh.kept_m, (unsigned long long)sum);
-  }
-  __syncthreads();
-  const double total = (double)sh.kept_m, target = (double)a.u[b] * total;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = threadIdx.x + h * THREADS;
-    if ((i & ~63) < n) {
-      uint64_t cum = 0;
-      for (int j = 0; j < n; ++j) {
-        const Entry o = sh.list[j];
-        cum += o.idx <= mine[h].idx ? o.w : 0ull;
-      }
-      if (i < n && mine[h].w) {
-        if ((double)cum > target) atomicMin(&sh.best, mine[h].idx);
-        atomicMax(&sh.bin, mine[h].idx);
-      }
+    if (mine.w) {
+      if ((double)cum > target) atomicMin(&sh.best, mine.idx);
+      atomicMax(&sh.bin, mine.idx);
     }
   }
   __syncthreads();
   const int pick = sh.best != INT32_MAX ? sh.best : sh.bin;
-  if (threadIdx.x == 0) a.out[b] = pick;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (threadIdx.x + h * THREADS < n && mine[h].w && mine[h].idx == pick && a.prob) a.prob[b] = (float)((double)mine[h].w / total);
+  if (mine.w && mine.idx == pick) {
+    a.out[b] = pick;
+    if (a.prob) a.prob[b] = (float)((double)mine.w / total);
+  }
 }
 
-// Draw from the scores above key t and the first `ties` equal to it, in index order.
+// ---- a draw over a row's segments, given what stays: keys above t and the first `ties` equal to t
+
+// a kept score's mass, in the unit of the segments' masses
+struct AsDouble {
+  typedef double V;
+  float M;
+  double c;
+  __device__ double operator()(float s) const { return weight(s, M, c); }
+};
+struct AsFixed {
+  typedef uint64_t V;
+  float M;
+  double c;
+  int shift;
+  __device__ uint64_t operator()(float s) const { return fixed(weight(s, M, c), shift); }
+};
+
+template <typename V>
+struct Found {
+  int64_t seg;
+  V before;        // mass of the segments before it
+  uint32_t ties;   // ties in the segments before it
+  double total, target;
+};
+
+// The segment in which u * total falls: a thread sums its run of segments, the runs are scanned,
+// the thread that holds the target walks its run.  get(seg, mass, ties): a segment's mass of keys
+// above t and its count of ties (false: nothing of it stays).
+template <typename V, typename G>
+__device__ __forceinline__ Found<V> find_segment(const Args& a, int b, uint32_t ties, V wt, G get, int* best, int* last,
+                                                 uint32_t* tmp_c, V* tmp_v, Found<V>* found) {
+  const int64_t per = (a.nseg + THREADS - 1) / THREADS;
+  const int64_t s0 = per * threadIdx.x, s1 = min(s0 + per, a.nseg);
+  uint32_t tie0 = 0, tall;
+  if (ties) {
+    uint32_t c = 0;
+    for (int64_t s = s0; s < s1; ++s) {
+      V m;
+      uint32_t x = 0;
+      if (get(s, m, x)) c += x;
+    }
+    tie0 = block_scan(c, tmp_c, tall) - c;
+  }
+  auto mass = [&](int64_t s, uint32_t& tie) {
+    V m = 0;
+    uint32_t x = 0;
+    if (!get(s, m, x)) return V(0);
+    if (ties) {
+      m += (V)(tie < ties ? min(ties - tie, x) : 0u) * wt;
+      tie += x;
+    }
+    return m;
+  };
+  V sum = 0, all;
+  uint32_t tie = tie0;
+  for (int64_t s = s0; s < s1; ++s) sum += mass(s, tie);
+  if (threadIdx.x == 0) { *best = INT32_MAX; *last = -1; }
+  const V cum = block_scan(sum, tmp_v, all);
+  const double total = (double)all, target = (double)a.u[b] * total;
+  if (sum > 0) {
+    if ((double)cum > target) atomicMin(best, (int)threadIdx.x);
+    atomicMax(last, (int)threadIdx.x);
+  }
+  __syncthreads();
+  // rounding may put u * total past the last sum: then the last score of the last segment with mass
+  const bool over = *best == INT32_MAX;
+  if ((int)threadIdx.x == (over ? *last : *best)) {
+    V before = cum - sum;
+    tie = tie0;
+    Found<V> f{-1, before, tie0, total, over ? INFINITY : target};
+    for (int64_t s = s0; s < s1; ++s) {
+      const uint32_t t0 = tie;
+      const V m = mass(s, tie);
+      if (m > 0) {
+        f.seg = s;
+        f.before = before;
+        f.ties = t0;
+        if (!over && (double)(before + m) > target) break;
+      }
+      before += m;
+    }
+    *found = f;
+  }
+  __syncthreads();
+  return *found;
+}
+
+// One wave: the first kept score of the segment at which the mass passes the target (or its last).
+template <typename W, typename V = typename W::V>
+__device__ __forceinline__ void pick_in_segment(const Args& a, int b, const Found<V>& f, const float v[4], const Row& r,
+                                                W wt_of, uint32_t t, uint32_t ties) {
+  const int lane = threadIdx.x & 63;
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c += v[j] > -INFINITY && key_of(v[j]) == t;
+  uint32_t tie = f.ties + wave_scan(c) - c;
+  V w[4], m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t key = key_of(v[j]);
+    bool kept = v[j] > -INFINITY && (key > t || (key == t && tie < ties));
+    tie += v[j] > -INFINITY && key == t;
+    if (kept && r.cut_min) kept = weight(v[j], wt_of.M, r.c) >= r.minp;
+    w[j] = kept ? wt_of(v[j]) : V(0);
+    m += w[j];
+  }
+  V cum = f.before + (wave_scan(m) - m);
+  int hit = -1, end = -1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    cum += w[j];
+    if (w[j] > 0) {
+      if (hit < 0 && (double)cum > f.target) hit = j;
+      end = j;
+    }
+  }
+  const uint64_t hits = __ballot(hit >= 0), ends = __ballot(end >= 0);
+  const int win = hits ? __ffsll((unsigned long long)hits) - 1 : 63 - __clzll(ends);
+  if (lane == win) {
+    const int j = hits ? hit : end;
+    a.out[b] = (int32_t)(f.seg * SEG + lane * 4 + j);
+    if (a.prob) a.prob[b] = (float)((double)(j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]) / f.total);
+  }
+}
+
 template <int T, int R>
 __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>& src, Shared& sh, const Row& r, float M,
                                               uint32_t t, uint32_t ties, double* segmass, int32_t* segtie, bool have_mass) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float bound = score_of(max(t, KEY_NONE));
-  const float tie_score = bound;
+  __shared__ Found<double> found;
+  const float bound = score_of(max(t, KEY_NONE));
+  const AsDouble w_of{M, r.c};
   double wt = 0;
   if (ties) {
-    wt = weight(tie_score, M, r.c);
+    wt = w_of(bound);
     if (r.cut_min && wt < r.minp) { wt = 0; ties = 0; }
   }
   if (!have_mass)
-    src.each(bound, [&](int64_t seg, const float* v) {
+    src.each([&](float m) { return m >= bound; }, [&](int64_t seg, const float* v) {
       double m = 0;
-      int c = 0;
+      uint32_t c = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t key = key_of(v[j]);
         if (v[j] > -INFINITY && key > t) {
-          const double w = weight(v[j], M, r.c);
+          const double w = w_of(v[j]);
           m += !r.cut_min || w >= r.minp ? w : 0.0;
         }
         c += v[j] > -INFINITY && key == t;
       }
       m = wave_sum(m);
       c = wave_sum(c);
-      if (lane == 0) { segmass[seg] = m; segtie[seg] = c; }
+      if (src.lane == 0) { segmass[seg] = m; segtie[seg] = (int32_t)c; }
     });
   __syncthreads();
-  // two walks over the segments: the total, then the segment in which u * total falls
-  double total = 0, target = 0;
-  for (int walk = 0; walk < 2; ++walk) {
-    uint32_t tie_before = 0;
-    double before = 0;
-    if (threadIdx.x == 0 && walk) { sh.seg = -1; }
-    bool found = false;
-    int64_t last = -1;
-    for (int64_t base = 0; base < a.nseg; base += THREADS) {
-      const int64_t seg = base + threadIdx.x;
-      double m = 0;
-      uint32_t c = 0;
-      if (seg < a.nseg && src.segmax[seg] >= bound && src.segmax[seg] > -INFINITY) {
-        m = segmass[seg];
-        if (have_mass) m *= weight(src.segmax[seg], M, r.c);
-        else c = (uint32_t)segtie[seg];
-      }
-      uint32_t cc = c;
-      if (ties) {
-        uint64_t none = 0;
-        block_scan(cc, none, sh);
-        const uint32_t t0 = tie_before + cc - c;  // ties in earlier segments
-        const uint32_t kept = t0 < ties ? min(ties - t0, c) : 0;
-        m += kept * wt;
-        __syncthreads();
-        if (threadIdx.x == THREADS - 1) sh.before_c = cc;
-        __syncthreads();
-        tie_before += sh.before_c;
-      }
-      double part;
-      const double cum = before + block_scan_d(m, sh, part);
-      if (walk) {
-        if (threadIdx.x == 0) { sh.best = INT32_MAX; sh.bin = -1; }
-        __syncthreads();
-        if (m > 0) {
-          if (!found && cum > target) atomicMin(&sh.best, (int)threadIdx.x);
-          atomicMax(&sh.bin, (int)threadIdx.x);
-        }
-        __syncthreads();
-        const int hit = sh.best, any = sh.bin;
-        if (!found && (hit != INT32_MAX || any >= 0)) {
-          const int at = hit != INT32_MAX ? hit : any;
-          // ties kept before this segment, for its scan
-          if ((int)threadIdx.x == at) {
-            sh.seg = seg;
-            sh.seg_before = cum - m;
-            sh.ties = ties ? tie_before - sh.before_c + cc - c : 0;
-          }
-          last = 0;
-          if (hit != INT32_MAX) found = true;
-        }
-        __syncthreads();
-        if (found) break;
-      }
-      before += part;
-    }
-    if (!walk) {
-      total = before;
-      target = (double)a.u[b] * total;
-    } else if (!found && last == 0) {
-      target = INFINITY;  // rounding put u * total past the last mass: its last score
-    }
-    __syncthreads();
-  }
-  const int64_t seg = sh.seg;
-  if (wave == (R == ROW_REGS ? (int)seg : 0) && seg >= 0) {
+  const Found<double> f = find_segment<double>(
+      a, b, ties, wt,
+      [&](int64_t s, double& m, uint32_t& c) {
+        const float x = src.segmax[s];
+        if (!(x >= bound) || x == -INFINITY) return false;
+        m = segmass[s];
+        if (have_mass) m *= w_of(x);
+        else c = (uint32_t)segtie[s];
+        return true;
+      },
+      &sh.best, &sh.bin, sh.scan_c, sh.scan_d, &found);
+  if (src.wave == (R == ROW_REGS ? (int)f.seg : 0)) {
     float v[4];
     if constexpr (R == ROW_REGS) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = src.v[j];
     } else {
-      load_seg<T>(a, b, seg, lane, v);
+      load_seg<T>(a, b, f.seg, src.lane, v);
     }
-    int c = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c += v[j] > -INFINITY && key_of(v[j]) == t;
-    int cs = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int c2 = __shfl_up(cs, o, 64);
-      if (lane >= o) cs += c2;
-    }
-    uint32_t tie = sh.ties + cs - c;
-    double w[4], m = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t key = key_of(v[j]);
-      w[j] = 0;
-      if (v[j] > -INFINITY) {
-        if (key > t) {
-          w[j] = weight(v[j], M, r.c);
-          if (r.cut_min && w[j] < r.minp) w[j] = 0;
-        } else if (key == t) {
-          if (tie < ties) w[j] = wt;
-          ++tie;
-        }
-      }
-      m += w[j];
-    }
-    double ms = m;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double m2 = __shfl_up(ms, o, 64);
-      if (lane >= o) ms += m2;
-    }
-    double cum = sh.seg_before + (ms - m);
-    int hit = -1, end = -1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      cum += w[j];
-      if (w[j] > 0) {
-        if (hit < 0 && cum > target) hit = j;
-        end = j;
-      }
-    }
-    const uint64_t hits = __ballot(hit >= 0), ends = __ballot(end >= 0);
-    const int win = hits ? __ffsll((unsigned long long)hits) - 1 : 63 - __clzll(ends);
-    if (lane == win) {
-      const int j = hits ? hit : end;
-      a.out[b] = (int32_t)(seg * SEG + lane * 4 + j);
-      if (a.prob) a.prob[b] = (float)((j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]) / total);
-    }
+    pick_in_segment(a, b, f, v, r, w_of, t, ties);
   }
 }
 
+// A row from its scores alone (rows of one launch; long rows with a long top-k, or whose lists ran
+// over): histogram, threshold of top-k, threshold of top-p, draw.
 template <int T, int R>
-__global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int have_hist) {
+__device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R>& src, Shared& sh, const Row& r, float M,
+                                               double* segmass, int32_t* segtie) {
+  const float cb = (float)(r.c * 32);  // 32 bins to an octave of weight
+  const int shift = shift_for((double)a.N);
+  const auto any = [](float) { return true; };
+  clear_hist(sh);
+  src.each(any, [&](int64_t, const float* v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t w = r.cut_p ? fixed(weight(v[j], M, r.c), shift) : 0;
+      hist_add<true, true>(sh.hc, sh.hm, v[j] > -INFINITY, bin_of(v[j], M, cb), w);
+    }
+  });
+  __syncthreads();
+  const auto reaches = [&](int bin) { return [=](float m) { return bin_of(m, M, cb) <= bin; }; };
+  const auto split_row = [&](int bin, bool by_mass, uint32_t need, uint64_t above, double target, uint32_t floor_key) {
+    split(sh, [&](auto g) {
+      src.each(reaches(bin), [&](int64_t, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          g(v[j] > -INFINITY && bin_of(v[j], M, cb) == bin, key_of(v[j]), fixed(weight(v[j], M, r.c), shift));
+      });
+    }, by_mass, need, above, target, floor_key);
+  };
+  uint32_t t = KEY_NONE, ties = 0;
+  uint64_t total = 0;
+  int kbin = BINS;        // bin of the top-k threshold
+  uint32_t c[PER];        // this thread's bins, kept for the search by mass
+  uint64_t m[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    c[j] = sh.hc[PER * threadIdx.x + j];
+    m[j] = sh.hm[PER * threadIdx.x + j];
+  }
+  if (r.k > 0) {
+    find_bin(sh, false, true, (uint32_t)r.k, 0, 0.0);
+    kbin = sh.bin;
+    const uint64_t kbefore = sh.before_m;
+    const uint32_t cbefore = sh.before_c;
+    if (cbefore + sh.hc[kbin] <= (uint32_t)r.k) {  // the whole bin stays: above the key below its smallest
+      total = kbefore + sh.hm[kbin];
+      if (threadIdx.x == 0) sh.kmin = 0xffffffffu;
+      __syncthreads();
+      src.each(reaches(kbin), [&](int64_t, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v[j] > -INFINITY && bin_of(v[j], M, cb) == kbin) atomicMin(&sh.kmin, key_of(v[j]));
+      });
+      __syncthreads();
+      t = sh.kmin - 1;
+    } else {
+      collect<T, R>(src, sh, M, r, cb, shift, reaches(kbin), [&](uint32_t, int bin) { return bin == kbin; });
+      const int n = sh.n;
+      if (n <= RANK) {
+        const Slot s = rank_list(sh, n, r.k, cbefore);
+        total = kbefore + sh.kept_m;
+        list_threshold(sh, s);
+      } else {
+        const uint32_t need = (uint32_t)(r.k - cbefore);
+        if (n <= LIST) split(sh, [&](auto g) { each_listed(sh.list, n, g); }, false, need, kbefore, 0.0, 0);
+        else split_row(kbin, false, need, kbefore, 0.0, 0);
+        total = sh.before_m + (uint64_t)sh.ties * fixed(weight(score_of(sh.kmin), M, r.c), shift);
+      }
+      t = sh.kmin;
+      ties = sh.ties;
+    }
+    if (r.cut_p) {  // the histogram of the scores that top-k left: bins past its threshold's are empty
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int i = PER * threadIdx.x + j;
+        sh.hc[i] = i <= kbin ? c[j] : 0;
+        sh.hm[i] = i < kbin ? m[j] : i == kbin ? total - kbefore : 0;
+      }
+      __syncthreads();
+    }
+  }
+  if (r.cut_p) {
+    if (r.k == 0) {
+      uint64_t mt = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) mt += m[j];
+      block_scan(mt, sh.scan_m, total);
+      __syncthreads();
+    }
+    const double target = r.p * (double)total;
+    find_bin(sh, true, true, 0, 0, target);
+    const int bin = sh.bin;
+    const uint64_t above = sh.before_m;
+    const uint32_t floor_key = bin == kbin ? (ties ? t : t + 1) : 0;  // what top-k left of this bin
+    const uint32_t tie_cap = bin == kbin && ties ? ties : 0xffffffffu;
+    collect<T, R>(src, sh, M, r, cb, shift, reaches(bin),
+                  [&](uint32_t key, int x) { return x == bin && key >= floor_key; });
+    const int n = sh.n;
+    // (scores equal to top-k's threshold beyond its ties rank behind all that stay, and the mass
+    // before them has reached the total: the cut drops them)
+    if (n <= RANK) {
+      Slot s = rank_list(sh, n, 0, 0);
+      cut_by_mass(s, above, target);
+      list_threshold(sh, s);
+    } else if (n <= LIST) {
+      split(sh, [&](auto g) { each_listed(sh.list, n, g); }, true, 0, above, target, floor_key);
+    } else {
+      split_row(bin, true, 0, above, target, floor_key);
+    }
+    t = sh.kmin;
+    ties = t == floor_key ? min(sh.ties, tie_cap) : sh.ties;
+  }
+  __syncthreads();
+  draw_from_row<T, R>(a, b, src, sh, r, M, t, ties, segmass, segtie, false);
+}
+
+// One workgroup per row.  Rows of one launch and long rows that need no pass over all masses are
+// answered; `passes`: long rows that cut by mass alone get their RowState.
+template <int T, int R>
+__global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   __shared__ Shared sh;
   constexpr int SMALL = R == ROW_REGS ? WAVES : R == ROW_CACHED ? CACHED_SEGS : 1;
   __shared__ float small_max[SMALL];
@@ -722,18 +908,33 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int have_hist) 
   __shared__ int32_t small_tie[SMALL];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Row r = row_settings(a, b);
-  const bool own = R != ROW_LONG;
+  constexpr bool own = R != ROW_LONG;
   const float* segmax = own ? small_max : a.segmax + (int64_t)b * a.nseg;
-  double* segmass = own ? small_mass : a.segmass + (int64_t)b * a.nseg;
+  double* segmass = own ? small_mass : (double*)a.segmass + (int64_t)b * a.nseg;
   int32_t* segtie = own ? small_tie : a.segtie + (int64_t)b * a.nseg;
   Source<T, R> src(a, b, segmax);
   float m = -INFINITY;
-  if constexpr (R != ROW_LONG) {
-    for (int64_t seg = wave; seg < a.nseg; seg += WAVES) {  // (ROW_REGS: one)
-      load_seg<T>(a, b, seg, lane, src.v);
-      const float x = wave_max(fmaxf(fmaxf(src.v[0], src.v[1]), fmaxf(src.v[2], src.v[3])));
-      if (lane == 0) small_max[seg] = x;
-      m = fmaxf(m, x);
+  if constexpr (R == ROW_REGS) {
+    if (wave < a.nseg) {
+      load_seg<T>(a, b, wave, lane, src.v);
+      m = wave_max(max4(src.v));
+      if (lane == 0) small_max[wave] = m;
+    }
+  } else if constexpr (R == ROW_CACHED) {
+    for (int64_t seg0 = wave; seg0 < a.nseg; seg0 += 4 * WAVES) {
+      float x[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (seg0 + j * WAVES < a.nseg) load_raw<T>(a, b, seg0 + j * WAVES, lane, x[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (seg0 + j * WAVES < a.nseg) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
+          const float y = wave_max(max4(x[j]));
+          if (lane == 0) small_max[seg0 + j * WAVES] = y;
+          m = fmaxf(m, y);
+        }
     }
   } else {
     for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) m = fmaxf(m, segmax[i]);
@@ -743,162 +944,246 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int have_hist) 
     if (threadIdx.x == 0) {
       a.out[b] = -1;
       if (a.prob) a.prob[b] = 0.f;
+      if (passes) a.state[b].active = 0;
     }
     return;
   }
-  const float cb = (float)(r.c * 32);
+  if (R == ROW_LONG && passes) {
+    if (!r.by_mass()) {
+      if (threadIdx.x == 0) a.state[b].active = 0;
+    } else {
+      double sum = 0, total;
+      for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS)
+        if (segmax[i] > -INFINITY) sum += segmass[i] * weight(segmax[i], M, r.c);
+      block_scan(sum, sh.scan_d, total);
+      // N scores below (1 - p) total / N hold less than (1 - p) total: the threshold is not among
+      // them, and the bins span the octaves above that
+      const double least = fmax((1 - r.p) * total / (double)a.N, 0x1p-60);
+      const double octaves = fmax(-log2(least), 0.0) + 0.125;
+      for (int i = threadIdx.x; i < BINS; i += THREADS) a.hmass[(int64_t)b * BINS + i] = 0;
+      if (threadIdx.x == 0) {
+        const int shift = shift_for(total);
+        a.state[b] = RowState{1, M, (float)(r.c * (BINS - 1) / octaves), shift, r.p * total * (double)(1ull << shift), 0, 0, 0};
+      }
+      return;
+    }
+  }
   if (r.direct()) {
     draw_from_row<T, R>(a, b, src, sh, r, M, KEY_NONE, 0, segmass, segtie, R == ROW_LONG && !r.cut_min);
     return;
   }
-  if (r.short_list(a.nseg)) {
-    // The k best scores lie in bins up to the one in which the count of segment maxima
-    // reaches k: that many scores, one a segment, are already in them.
-    for (int i = threadIdx.x; i < BINS; i += THREADS) { sh.hc[i] = 0; sh.hm[i] = 0; }
-    __syncthreads();
-    for (int64_t i0 = 0; i0 < a.nseg; i0 += THREADS) {
-      const int64_t i = i0 + threadIdx.x;
-      const float x = i < a.nseg ? segmax[i] : -INFINITY;
-      if (x > -INFINITY) atomicAdd(&sh.hc[bin_of(x, M, cb)], 1u);
+  if (r.k > 0 && r.k <= SHORT_K && (R != ROW_LONG || r.k <= a.nseg / 2)) {
+    // A short list: the k best lie in bins up to the one in which the count of scores reaches k.  On a
+    // long row the segments' maxima are counted: that many scores, one a segment, are in
+    // those bins already, and few others (for k up to half the segments).
+    const float cb = (float)(r.c * 32);
+    const auto any = [](float) { return true; };
+    clear_hist(sh);
+    if constexpr (R == ROW_LONG) {
+      for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) {
+        const float x = segmax[i];
+        if (x > -INFINITY) atomicAdd(&sh.hc[bin_of(x, M, cb)], 1u);
+      }
+    } else {
+      src.each(any, [&](int64_t, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          hist_add<true, false>(sh.hc, sh.hm, v[j] > -INFINITY, bin_of(v[j], M, cb), 0);
+      });
     }
     __syncthreads();
-    find_bin(sh, false, (uint32_t)r.k, 0, 0.0);
-    // fewer unmasked segments than k: everything unmasked is a candidate
-    const bool all = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k;
-    const int edge = all ? BINS : sh.bin;
-    collect<T, R>(src, sh, -INFINITY, M, r, cb, 51, [&](uint32_t, int bin) { return bin <= edge; });
+    find_bin(sh, false, false, (uint32_t)r.k, 0, 0.0);
+    // fewer unmasked than k: everything unmasked is a candidate
+    const int edge = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k ? BINS : sh.bin;
+    collect<T, R>(src, sh, M, r, cb, 51, [&](float x) { return bin_of(x, M, cb) <= edge; },
+                  [&](uint32_t, int bin) { return bin <= edge; });
     const int n = sh.n;
-    if (n <= LIST) {
-      Slot s[2];
-      rank_list(sh, n, r.k, 0, s);
+    if (n <= RANK) {
+      Slot s = rank_list(sh, n, r.k, 0);
       if (r.cut_p) cut_by_mass(s, 0, r.p * (double)sh.kept_m);
       draw_from_list(a, b, sh, n, s, r, M);
       return;
     }
-  }
-  const int shift = shift_for(a.N);
-  const bool ready = have_hist && !r.short_list(a.nseg);
-  __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += THREADS) {
-    sh.hc[i] = ready ? a.hcount[(int64_t)b * BINS + i] : 0;
-    sh.hm[i] = ready ? a.hmass[(int64_t)b * BINS + i] : 0;
-  }
-  __syncthreads();
-  if (!ready) {
-    src.each(-INFINITY, [&](int64_t, const float* v) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        hist_add(sh.hc, sh.hm, v[j] > -INFINITY, bin_of(v[j], M, cb), fixed(weight(v[j], M, r.c), shift));
-    });
-    __syncthreads();
-  }
-  // threshold key and ties of the scores that stay
-  uint32_t t = KEY_NONE, ties = 0;
-  uint64_t total;
-  int kbin = BINS;        // bin of the top-k threshold
-  uint64_t kbefore = 0;   // mass of the bins before it
-  if (r.k > 0) {
-    const bool cut_p = r.cut_p;
-    // (the p search below needs the histogram again: keep this thread's two bins)
-    const uint32_t c0 = sh.hc[2 * threadIdx.x], c1 = sh.hc[2 * threadIdx.x + 1];
-    const uint64_t m0 = sh.hm[2 * threadIdx.x], m1 = sh.hm[2 * threadIdx.x + 1];
-    find_bin(sh, false, (uint32_t)min(r.k, (int64_t)UINT32_MAX), 0, 0.0);
-    kbin = sh.bin;
-    kbefore = sh.before_m;
-    const uint32_t cbefore = sh.before_c;
-    const float bound = -INFINITY;
-    if (cbefore + sh.hc[kbin] <= r.k) {  // the whole bin stays
-      t = KEY_NONE;
-      ties = 0;
-      total = kbefore + sh.hm[kbin];
-      // everything in bins <= kbin: the smallest key among them is the threshold
-      if (threadIdx.x == 0) sh.kmin = 0xffffffffu;
-      __syncthreads();
-      src.each(bound, [&](int64_t, const float* v) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (v[j] > -INFINITY && bin_of(v[j], M, cb) == kbin) atomicMin(&sh.kmin, key_of(v[j]));
-      });
-      __syncthreads();
-      t = sh.kmin - 1;  // keys above t stay
-    } else {
-      collect<T, R>(src, sh, bound, M, r, cb, shift, [&](uint32_t, int bin) { return bin == kbin; });
-      const int n = sh.n;
-      if (n <= LIST) {
-        Slot s[2];
-        rank_list(sh, n, r.k, cbefore, s);
-        total = kbefore + sh.kept_m;
-        list_threshold(sh, s);
+    if (n <= LIST) {
+      const auto listed = [&](auto g) { each_listed(sh.list, n, g); };
+      split(sh, listed, false, (uint32_t)r.k, 0, 0.0, 0);
+      uint32_t t = sh.kmin, ties = sh.ties;
+      if (r.cut_p) {
+        const uint64_t total = sh.before_m + (uint64_t)ties * fixed(weight(score_of(t), M, r.c), 51);
+        split(sh, listed, true, 0, 0, r.p * (double)total, t);
+        ties = sh.kmin == t ? min(ties, sh.ties) : sh.ties;
         t = sh.kmin;
-        ties = sh.ties;
-      } else {
-        split_bin<T, R>(src, sh, bound, M, r, cb, shift, kbin, false, (uint32_t)(r.k - cbefore), kbefore, 0.0, 0);
-        t = sh.kmin;
-        ties = sh.ties;
-        total = sh.before_m + (uint64_t)ties * fixed(weight(score_of(t), M, r.c), shift);
+      }
+      draw_from_row<T, R>(a, b, src, sh, r, M, t, ties, segmass, segtie, false);
+      return;
+    }
+  }
+  finish_general<T, R>(a, b, src, sh, r, M, segmass, segtie);
+}
+
+// ---- long rows that cut by mass alone: mass by bin, then what lies above and in the threshold's
+
+template <int T>
+__global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
+  __shared__ unsigned long long hm[BINS];
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const RowState st = a.state[b];
+  if (!st.active) return;
+  const Row r = row_settings(a, b);
+  for (int i = threadIdx.x; i < BINS; i += THREADS) hm[i] = 0;
+  __syncthreads();
+  const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
+  for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
+    float x[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_raw<T>(a, b, min(seg0 + j * WAVES, a.nseg - 1), lane, x[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (seg0 + j * WAVES >= s1) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = clean(x[j][i]);
+        const int bin = bin_of(v, st.M, st.cb);
+        const bool on = v > -INFINITY && bin < BINS - 1;
+        if (__ballot(on)) hist_add<false, true>(nullptr, hm, on, bin, fixed(weight(v, st.M, r.c), st.shift));
       }
     }
-    if (cut_p) {
-      __syncthreads();
-      // the histogram of the scores that top-k left: bins past its threshold's are empty
-      const int i0 = 2 * threadIdx.x, i1 = i0 + 1;
-      sh.hc[i0] = i0 <= kbin ? c0 : 0;
-      sh.hc[i1] = i1 <= kbin ? c1 : 0;
-      sh.hm[i0] = i0 < kbin ? m0 : i0 == kbin ? total - kbefore : 0;
-      sh.hm[i1] = i1 < kbin ? m1 : i1 == kbin ? total - kbefore : 0;
-      __syncthreads();
-    }
-  }
-  if (r.cut_p) {
-    if (r.k == 0) {
-      // the total is the last inclusive sum of the scan
-      find_bin(sh, true, 0, 0, INFINITY);
-      total = sh.total_m;
-    }
-    const double target = r.p * (double)total;
-    find_bin(sh, true, 0, 0, target);
-    const int bin = sh.bin;
-    const uint64_t above = sh.before_m;
-    const uint32_t floor_key = bin == kbin ? (ties ? t : t + 1) : 0;  // what top-k left of this bin
-    const uint32_t tie_cap = bin == kbin && ties ? ties : 0xffffffffu;
-    collect<T, R>(src, sh, -INFINITY, M, r, cb, shift,
-                  [&](uint32_t key, int x) { return x == bin && key >= floor_key; });
-    const int n = sh.n;
-    if (n <= LIST) {
-      // (scores equal to top-k's threshold beyond its ties are ranked behind all that stay, and
-      // the mass before them has reached the total: the cut drops them)
-      Slot s[2];
-      rank_list(sh, n, 0, 0, s);
-      cut_by_mass(s, above, target);
-      list_threshold(sh, s);
-    } else {
-      split_bin<T, R>(src, sh, -INFINITY, M, r, cb, shift, bin, true, 0, above, target, floor_key);
-    }
-    __syncthreads();
-    const uint32_t t2 = sh.kmin, ties2 = sh.ties;
-    ties = t2 == floor_key ? min(ties2, tie_cap) : ties2;
-    t = t2;
   }
   __syncthreads();
-  draw_from_row<T, R>(a, b, src, sh, r, M, t, ties, segmass, segtie, false);
+  for (int i = threadIdx.x; i < BINS - 1; i += THREADS)
+    if (hm[i]) atomicAdd((unsigned long long*)a.hmass + (int64_t)b * BINS + i, hm[i]);
 }
 
 template <int T>
-int run(Args& a, int hist, hipStream_t st) {
+__global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
+  __shared__ Shared sh;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const RowState st = a.state[b];  // (listed, bin and above are written by this kernel, and not read)
+  if (!st.active) return;
+  const Row r = row_settings(a, b);
+  for (int i = threadIdx.x; i < BINS; i += THREADS) { sh.hc[i] = 0; sh.hm[i] = a.hmass[(int64_t)b * BINS + i]; }
+  __syncthreads();
+  find_bin(sh, true, true, 0, 0, st.target);
+  const int bin = sh.bin;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.state[b].bin = bin;
+    a.state[b].above = sh.before_m;
+  }
+  const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
+  for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
+    float x[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_raw<T>(a, b, min(seg0 + j * WAVES, a.nseg - 1), lane, x[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t seg = seg0 + j * WAVES;
+      if (seg >= s1) continue;
+      uint64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = clean(x[j][i]);
+        const int at_bin = bin_of(v, st.M, st.cb);
+        const bool on = v > -INFINITY && at_bin <= bin;
+        if (__ballot(on)) {
+          const double w = weight(v, st.M, r.c);
+          const uint64_t fw = fixed(w, st.shift);
+          if (on && at_bin < bin) sum += !r.cut_min || w >= r.minp ? fw : (uint64_t)0;
+          if (on && at_bin == bin) {
+            const uint32_t at = atomicAdd(&a.state[b].listed, 1u);
+            if (at < (uint32_t)a.listcap)
+              a.list[(int64_t)b * a.listcap + at] = Entry{key_of(v), (int32_t)(seg * SEG + lane * 4 + i), fw};
+          }
+        }
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) a.segmass[(int64_t)b * a.nseg + seg] = sum;
+    }
+  }
+}
+
+// the threshold inside the listed bin, then the draw over whole-number masses
+template <int T>
+__global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
+  __shared__ Shared sh;
+  __shared__ Found<uint64_t> found;
+  const int b = blockIdx.x, lane = threadIdx.x & 63;
+  const RowState st = a.state[b];
+  if (!st.active) return;
+  const Row r = row_settings(a, b);
+  uint64_t* segmass = a.segmass + (int64_t)b * a.nseg;
+  if (st.listed > (uint32_t)a.listcap) {  // more than a list of equal or near-equal scores: the row again
+    Source<T, ROW_LONG> src(a, b, a.segmax + (int64_t)b * a.nseg);
+    finish_general<T, ROW_LONG>(a, b, src, sh, r, st.M, (double*)segmass, a.segtie + (int64_t)b * a.nseg);
+    return;
+  }
+  const int n = (int)st.listed;
+  const Entry* list = a.list + (int64_t)b * a.listcap;
+  if (n <= RANK) {
+    if ((int)threadIdx.x < n) sh.list[threadIdx.x] = list[threadIdx.x];
+    __syncthreads();
+    Slot s = rank_list(sh, n, 0, 0);
+    cut_by_mass(s, st.above, st.target);
+    list_threshold(sh, s);
+  } else {
+    split(sh, [&](auto g) { each_listed(list, n, g); }, true, 0, st.above, st.target, 0);
+  }
+  const uint32_t t = sh.kmin;
+  uint32_t ties = sh.ties;
+  const AsFixed w_of{st.M, r.c, st.shift};
+  uint64_t wt = w_of(score_of(t));
+  if (r.cut_min && weight(score_of(t), st.M, r.c) < r.minp) { wt = 0; ties = 0; }
+  // listed scores above t join their segments' masses; ties are counted per segment
+  int32_t* segtie = a.segtie + (int64_t)b * a.nseg;
+  if (ties)
+    for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS) segtie[s] = 0;
+  __threadfence();
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const Entry e = list[i];
+    if (e.key > t) {
+      if (!r.cut_min || weight(score_of(e.key), st.M, r.c) >= r.minp)
+        atomicAdd((unsigned long long*)segmass + e.idx / SEG, (unsigned long long)e.w);
+    } else if (e.key == t && ties) {
+      atomicAdd(segtie + e.idx / SEG, 1);
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  const Found<uint64_t> f = find_segment<uint64_t>(
+      a, b, ties, wt,
+      [&](int64_t s, uint64_t& m, uint32_t& c) {
+        m = __hip_atomic_load(segmass + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (ties) c = (uint32_t)__hip_atomic_load(segtie + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return true;
+      },
+      &sh.best, &sh.bin, sh.scan_c, sh.scan_m, &found);
+  if (threadIdx.x < 64) {
+    float v[4];
+    load_seg<T>(a, b, f.seg, lane, v);
+    pick_in_segment(a, b, f, v, r, w_of, t, ties);
+  }
+}
+
+template <int T>
+int run(Args& a, int passes, hipStream_t st) {
   if (a.nseg <= WAVES) {
     hipLaunchKernelGGL((finish_kernel<T, ROW_REGS>), dim3(a.B), dim3(THREADS), 0, st, a, 0);
   } else if (a.nseg <= CACHED_SEGS) {
     hipLaunchKernelGGL((finish_kernel<T, ROW_CACHED>), dim3(a.B), dim3(THREADS), 0, st, a, 0);
   } else {
     const int per = 4 * STAT_SEGS;
-    hipLaunchKernelGGL((stats_kernel<T>), dim3((unsigned)((a.nseg + per - 1) / per), a.B), dim3(256), 0, st, a, hist);
+    hipLaunchKernelGGL((stats_kernel<T>), dim3((unsigned)((a.nseg + per - 1) / per), a.B), dim3(256), 0, st, a);
     FPS_CHECK_LAUNCH();
-    if (hist) {
-      hipLaunchKernelGGL((hist_kernel<T>), dim3((unsigned)((a.nseg + HIST_SEGS - 1) / HIST_SEGS), a.B), dim3(THREADS), 0,
-                         st, a);
+    hipLaunchKernelGGL((finish_kernel<T, ROW_LONG>), dim3(a.B), dim3(THREADS), 0, st, a, passes);
+    if (passes) {
       FPS_CHECK_LAUNCH();
+      const dim3 grid((unsigned)((a.nseg + PASS_SEGS - 1) / PASS_SEGS), a.B);
+      hipLaunchKernelGGL((hist_kernel<T>), grid, dim3(THREADS), 0, st, a);
+      FPS_CHECK_LAUNCH();
+      hipLaunchKernelGGL((collect_kernel<T>), grid, dim3(THREADS), 0, st, a);
+      FPS_CHECK_LAUNCH();
+      hipLaunchKernelGGL((finish_mass_kernel<T>), dim3(a.B), dim3(THREADS), 0, st, a);
     }
-    hipLaunchKernelGGL((finish_kernel<T, ROW_LONG>), dim3(a.B), dim3(THREADS), 0, st, a, hist);
   }
   FPS_CHECK_LAUNCH();
   return 0;
@@ -906,13 +1191,17 @@ int run(Args& a, int hist, hipStream_t st) {
 
 constexpr int64_t kShortRow = (int64_t)CACHED_SEGS * SEG;  // rows up to this take no workspace
 
+int list_cap(int64_t N) { return (int)(N / 8 < 16384 ? N / 8 : 16384); }
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
 }  // namespace
 
 // bytes of workspace for B rows of N scores
 FPS_API int64_t fps_sample_scores_ws_bytes(int64_t B, int64_t N) {
   if (B <= 0 || N <= kShortRow) return 0;
   const int64_t nseg = (N + SEG - 1) / SEG;
-  return B * (BINS * 12 + nseg * 16);
+  return B * (list_cap(N) * (int64_t)sizeof(Entry)) + round16(B * sizeof(RowState)) + B * BINS * 8 + B * nseg * 16 + 16;
 }
 
 // s [B, N] (row stride ld, type 0 fp32 / 1 bf16 / 2 fp16); u [B]; temperature / top_k / top_p /
@@ -923,9 +1212,10 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
                               const float* top_p, double top_p0, const float* min_p, double min_p0, int32_t* out,
                               float* prob, void* ws, void* stream) {
   if (B <= 0) return 0;
-  if (N <= 0 || N > INT32_MAX || ld < N || type < 0 || type > 2 || (B > 65535 && N > kShortRow)) return (int)hipErrorInvalidValue;
+  if (N <= 0 || N > INT32_MAX || ld < N || type < 0 || type > 2 || (B > 65535 && N > kShortRow))
+    return (int)hipErrorInvalidValue;
   Args a;
-  a.s = s; a.ld = ld; a.N = N; a.nseg = (N + SEG - 1) / SEG; a.B = B; a.type = type;
+  a.s = s; a.ld = ld; a.N = N; a.nseg = (N + SEG - 1) / SEG; a.B = B;
   a.vec = (B == 1 || ld % 4 == 0) && ((uintptr_t)s & (type == T_F32 ? 15 : 7)) == 0;
   a.u = u;
   a.temperature = temperature; a.temperature0 = temperature0;
@@ -933,24 +1223,24 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
   a.top_p = top_p; a.top_p0 = top_p0;
   a.min_p = min_p; a.min_p0 = min_p0;
   a.out = out; a.prob = prob;
-  a.segmax = nullptr; a.segmass = nullptr; a.segtie = nullptr; a.hcount = nullptr; a.hmass = nullptr;
-  int hist = 0;
+  a.segmass = nullptr; a.hmass = nullptr; a.list = nullptr; a.state = nullptr; a.segmax = nullptr; a.segtie = nullptr;
+  a.listcap = 0;
+  int passes = 0;
   if (N > kShortRow) {
-    if (ws == nullptr) return (int)hipErrorInvalidValue;
+    if (ws == nullptr || ((uintptr_t)ws & 15)) return (int)hipErrorInvalidValue;
+    a.listcap = list_cap(N);
     char* p = (char*)ws;
+    a.list = (Entry*)p; p += (int64_t)B * a.listcap * sizeof(Entry);
+    a.state = (RowState*)p; p += round16(B * sizeof(RowState));
     a.hmass = (uint64_t*)p; p += (int64_t)B * BINS * 8;
-    a.segmass = (double*)p; p += (int64_t)B * a.nseg * 8;
-    a.hcount = (uint32_t*)p; p += (int64_t)B * BINS * 4;
+    a.segmass = (uint64_t*)p; p += (int64_t)B * a.nseg * 8;
     a.segmax = (float*)p; p += (int64_t)B * a.nseg * 4;
     a.segtie = (int32_t*)p;
-    // can a row need the histogram?  (scalars decide here, per-row settings on the device)
+    // can a row cut by mass alone?  (scalars decide here, per-row settings on the device)
     const bool greedy = !temperature && !(temperature0 > 0);
-    const int64_t k = top_k0 <= 0 || top_k0 >= N ? 0 : top_k0;
-    if (greedy) hist = 0;
-    else if (top_k) hist = 1;
-    else if (k) hist = k > SHORT_K || a.nseg < k;
-    else hist = top_p || top_p0 < 1;
+    const bool k = !top_k && top_k0 > 0 && top_k0 < N;
+    passes = !greedy && !k && (top_p || top_p0 < 1);
   }
   hipStream_t st = (hipStream_t)stream;
-  return type == T_F32 ? run<T_F32>(a, hist, st) : type == T_BF16 ? run<T_BF16>(a, hist, st) : run<T_F16>(a, hist, st);
+  return type == T_F32 ? run<T_F32>(a, passes, st) : type == T_BF16 ? run<T_BF16>(a, passes, st) : run<T_F16>(a, passes, st);
 }
