@@ -42,18 +42,24 @@ constexpr int SHORT_K = 1024;   // top-k up to this lists its candidates
 constexpr int CACHED_SEGS = 128;     // segments of a row that takes one launch
 constexpr int PASS_SEGS = 128;  // segments per workgroup of the passes over long rows
 
+// a listed score: its key above the complement of its index (the larger word is the better score,
+// equal scores by the lower index), and its weight
 struct Entry {
-  uint32_t key;
-  int32_t idx;
+  uint64_t at;
   uint64_t w;
+  __device__ uint32_t key() const { return (uint32_t)(at >> 32); }
+  __device__ int32_t idx() const { return (int32_t)~(uint32_t)at; }
 };
+__device__ __forceinline__ Entry make_entry(uint32_t key, int32_t idx, uint64_t w) {
+  return Entry{(uint64_t)key << 32 | (uint32_t)~idx, w};
+}
 
 // what the passes over a long row that cuts by mass alone share
 struct RowState {
   int active;
   float M, cb;     // largest score; bins per unit of score
   int shift;
-  double target;   // p * total, in units of 2^-shift
+  double target;   // p * total
   uint64_t above;  // mass of the bins before `bin`
   int bin;         // holds the threshold
   uint32_t listed; // scores in it
@@ -118,25 +124,26 @@ __device__ __forceinline__ float score_of(uint32_t k) {
 }
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // key_of(-inf)
 
-// 2^((s - M) c): interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 10
-// (relative error 3e-16), times the power of two.  Without branches: selects at the end.
+// 2^((s - M) c): interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 8 (relative
+// error 1.1e-12: two answers differ where u * total falls that near to a step), times the
+// power of two.  n = round(t) is read from the low bits of t + 1.5 * 2^52.
 __device__ __forceinline__ double weight(float s, float M, double c) {
-  const double t0 = ((double)s - (double)M) * c;
-  const double t = t0 > -1020.0 ? t0 : -1020.0;  // also for NaN (both infinite)
-  const double n = __builtin_rint(t), f = t - n;
-  double p = 0x1.e6063bb9d7e13p-28;
-  p = __builtin_fma(p, f, 0x1.b675bcea1ca08p-24);
-  p = __builtin_fma(p, f, 0x1.62bfd4792ba8bp-20);
-  p = __builtin_fma(p, f, 0x1.ffcb5405de21bp-17);
-  p = __builtin_fma(p, f, 0x1.430913096f0eap-13);
-  p = __builtin_fma(p, f, 0x1.5d87fe9d7a7abp-10);
-  p = __builtin_fma(p, f, 0x1.3b2ab6fba1de4p-7);
-  p = __builtin_fma(p, f, 0x1.c6b08d703ce47p-5);
-  p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
-  p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
-  p = __builtin_fma(p, f, 1.0);
-  const double w = __longlong_as_double(__double_as_longlong(p) + ((int64_t)(int)n << 52));
-  return s == M ? 1.0 : t0 > -1020.0 ? w : 0.0;
+  if (M == INFINITY) return s == M ? 1.0 : 0.0;  // (one branch for a whole row)
+  const double t0 = ((double)s - (double)M) * c;  // exactly 0 at the best score
+  const double t = fmax(t0, -1020.0);
+  const double u = t + 6755399441055744.0;
+  const double f = t - (u - 6755399441055744.0);
+  double p = 0x1.63d1363a7ecb6p-20;
+  p = __builtin_fma(p, f, 0x1.00dc4a534054dp-16);
+  p = __builtin_fma(p, f, 0x1.4308ac85a6c21p-13);
+  p = __builtin_fma(p, f, 0x1.5d8745a72827ap-10);
+  p = __builtin_fma(p, f, 0x1.3b2ab7181b778p-7);
+  p = __builtin_fma(p, f, 0x1.c6b08dd6fd236p-5);
+  p = __builtin_fma(p, f, 0x1.ebfbdff823cedp-3);
+  p = __builtin_fma(p, f, 0x1.62e42fef84cf0p-1);
+  p = __builtin_fma(p, f, 0x1.0000000000000p+0);
+  const double w = __longlong_as_double(__double_as_longlong(p) + ((__double_as_longlong(u) << 52)));
+  return t0 > -1020.0 ? w : 0.0;
 }
 
 // w in [0, 1] as a whole multiple of 2^-shift, shift <= 51 (rounded to nearest even)
@@ -250,6 +257,20 @@ __device__ __forceinline__ float wave_max(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t min_below(uint32_t v) {
+  return min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+  v = min_below<0x111, 0xf>(v);
+  v = min_below<0x112, 0xf>(v);
+  v = min_below<0x114, 0xf>(v);
+  v = min_below<0x118, 0xf>(v);
+  v = min_below<0x142, 0xa>(v);
+  v = min_below<0x143, 0xc>(v);
+  return lane_value(v, 63);
+}
+
 // inclusive sum over the workgroup in thread order, and the total; tmp: one V per wave
 template <typename V>
 __device__ __forceinline__ V block_scan(V v, V* tmp, V& total) {
@@ -283,7 +304,10 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   const Row r = row_settings(a, b);
   const int64_t seg0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * STAT_SEGS;
   if (seg0 >= a.nseg) return;
-  const bool mass = r.k == 0 && !(r.direct() && r.cut_min);
+  const bool mass = r.direct() && !r.cut_min;
+  // rows that cut by mass: fp32 sums, to place the histogram's bins
+  const bool rough = r.by_mass();
+  const float cf = (float)r.c;
   float v[STAT_SEGS][4];
 #pragma unroll
   for (int j = 0; j < STAT_SEGS; ++j) load_raw<T>(a, b, min(seg0 + j, a.nseg - 1), lane, v[j]);
@@ -303,12 +327,18 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
         w = wave_sum(w);
       }
       if (lane == j) ws = w;
+    } else if (rough) {
+      float w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w += v[j][i] == m ? 1.f : v[j][i] > -INFINITY ? exp2f((v[j][i] - m) * cf) : 0.f;
+      w = group_sum<64>(w);
+      if (lane == j) ws = w;
     }
   }
   if (lane < STAT_SEGS && seg0 + lane < a.nseg) {
     const int64_t at = (int64_t)b * a.nseg + seg0 + lane;
     a.segmax[at] = ms;
-    if (mass) a.segmass[at] = (uint64_t)__double_as_longlong(ws);
+    if (mass || rough) a.segmass[at] = (uint64_t)__double_as_longlong(ws);
   }
 }
 
@@ -333,17 +363,25 @@ __device__ __forceinline__ void hist_add(uint32_t* hc, unsigned long long* hm, b
   }
 }
 
+constexpr int WANTED = 4 * THREADS;  // segments looked at together
+
 struct Shared {
-  uint32_t hc[BINS];
   unsigned long long hm[BINS];
+  uint32_t hc[BINS];
   Entry list[LIST];
+  uint32_t rank[RANK];
+  unsigned long long before[RANK];
+  uint16_t segs[WANTED];
+  int nsegs;
+  int wave_hit[WAVES], wave_any[WAVES];
   float tmp[WAVES];
   uint32_t scan_c[WAVES];
   uint64_t scan_m[WAVES];
   double scan_d[WAVES];
   // results of searches, written by one thread
-  int bin, n, best;
+  int bin, n;
   uint32_t kmin, ties, before_c;
+  double target;
   unsigned long long before_m, kept_m;
 };
 
@@ -353,58 +391,71 @@ __device__ __forceinline__ void clear_hist(Shared& sh) {
   __syncthreads();
 }
 
-// The bin of the histogram in sh (bin 0 best) in which the count first reaches `need` (by_mass
-// false) or the mass, added to `above`, first reaches `target`: sh.bin, and what lies before it:
-// sh.before_c, sh.before_m.  Where rounding lets no bin reach it: the last bin that holds
-// anything.  By count the masses are summed only with `masses`.
-__device__ __forceinline__ void find_bin(Shared& sh, bool by_mass, bool masses, uint32_t need, uint64_t above,
-                                         double target) {
-  const int i = threadIdx.x;
-  uint32_t c[PER], ct = 0, call;
-  uint64_t m[PER], mt = 0, mall;
+// the first value of the wave's lanes that have one (-1: none), and the last
+__device__ __forceinline__ int first_of(int v) {
+  const uint64_t m = __ballot(v >= 0);
+  return m ? __builtin_amdgcn_readlane(v, __ffsll((unsigned long long)m) - 1) : -1;
+}
+__device__ __forceinline__ int last_of(int v) {
+  const uint64_t m = __ballot(v >= 0);
+  return m ? __builtin_amdgcn_readlane(v, 63 - __clzll(m)) : -1;
+}
+
+enum Search { BY_COUNT, BY_COUNT_WITH_MASS, BY_MASS };
+
+// The bin of the histogram in sh (bin 0 best) in which the count first reaches `need`, or the mass,
+// added to `above`, first reaches the target: sh.bin, and what lies before it: sh.before_c,
+// sh.before_m.  part >= 0: the target is that part of all mass (sh.target).  Where rounding lets no
+// bin reach it: the last bin that holds anything.
+template <Search S>
+__device__ __forceinline__ void find_bin(Shared& sh, uint32_t need, uint64_t above = 0, double target = 0, double part = -1) {
+  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+  uint32_t c[PER], ct = 0, cc = 0, call;
+  uint64_t m[PER], mt = 0, mm = 0, mall;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    c[j] = sh.hc[PER * i + j];
-    m[j] = sh.hm[PER * i + j];
+    c[j] = S == BY_MASS ? 0 : sh.hc[PER * i + j];
+    m[j] = S == BY_COUNT ? 0 : sh.hm[PER * i + j];
     ct += c[j];
     mt += m[j];
   }
-  uint32_t cc = 0;
-  uint64_t mm = 0;
-  if (i == 0) { sh.bin = BINS; sh.best = -1; }
-  if (!by_mass) cc = block_scan(ct, sh.scan_c, call) - ct;
-  if (by_mass || masses) mm = block_scan(mt, sh.scan_m, mall) - mt;
+  if (S != BY_MASS) cc = block_scan(ct, sh.scan_c, call) - ct;
+  if (S != BY_COUNT) mm = block_scan(mt, sh.scan_m, mall) - mt;
+  if (S == BY_MASS && part >= 0) target = part * (double)mall;
   int hit = -1, any = -1;
-  uint32_t c_at = 0;
-  uint64_t m_at = 0;
+  uint32_t c_hit = 0, c_any = 0;
+  uint64_t m_hit = 0, m_any = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const bool full = by_mass ? m[j] != 0 : c[j] != 0;
-    if (full) {
-      any = j;
-      if (hit < 0 && (by_mass ? (double)(above + mm + m[j]) >= target : cc + c[j] >= need)) { hit = j; c_at = cc; m_at = mm; }
+    if (S == BY_MASS ? m[j] != 0 : c[j] != 0) {
+      any = PER * i + j;
+      c_any = cc;
+      m_any = mm;
+      if (hit < 0 && (S == BY_MASS ? (double)(above + mm + m[j]) >= target : cc + c[j] >= need)) {
+        hit = any;
+        c_hit = cc;
+        m_hit = mm;
+      }
     }
     cc += c[j];
     mm += m[j];
   }
-  if (hit >= 0) atomicMin(&sh.bin, PER * i + hit);
-  if (any >= 0) atomicMax(&sh.best, PER * i + any);
+  const int wh = first_of(hit), wa = last_of(any);
+  if (lane == 0) { sh.wave_hit[wave] = wh; sh.wave_any[wave] = wa; }
   __syncthreads();
-  const bool none = sh.bin == BINS;
-  const int bin = none ? sh.best : sh.bin;
-  __syncthreads();
-  if (bin / PER == i && bin >= 0) {
-    if (none) {  // before the last bin: what this thread's scan holds, less that bin and the empty ones after it
-      const int j = bin - PER * i;
-      c_at = cc;
-      m_at = mm;
+  int bin = -1, last = -1;
 #pragma unroll
-      for (int x = 0; x < PER; ++x)
-        if (x >= j) { c_at -= c[x]; m_at -= m[x]; }
-    }
+  for (int w = 0; w < WAVES; ++w) {
+    if (bin < 0) bin = sh.wave_hit[w];
+    last = max(last, sh.wave_any[w]);
+  }
+  const bool found = bin >= 0;
+  if (!found) bin = last;
+  if (bin == (found ? hit : any)) {
     sh.bin = bin;
-    sh.before_c = c_at;
-    sh.before_m = m_at;
+    sh.before_c = found ? c_hit : c_any;
+    sh.before_m = found ? m_hit : m_any;
+    sh.target = target;
   }
   __syncthreads();
 }
@@ -423,33 +474,50 @@ struct Source {
   float v[4];
   __device__ Source(const Args& a_, int b_, const float* sm)
       : a(a_), b(b_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), segmax(sm) {}
-  // f(segment, scores) for the segments whose largest score (not -inf) is wanted; the waves
-  // take them in turn.  64 maxima are looked at together, four segments are loaded together.
+  // f(segment, scores) for the segments whose largest score (not -inf) is wanted.  Their maxima
+  // are looked at first, many together; the waves share out the wanted ones and load four at a time.
   template <typename P, typename F>
-  __device__ __forceinline__ void each(P want, F f) {
+  __device__ __forceinline__ void each(Shared& sh, P want, F f) {
     if constexpr (R == ROW_REGS) {
       if (wave < a.nseg) f((int64_t)wave, v);
     } else {
-      for (int64_t base = 0; base < a.nseg; base += 64 * WAVES) {
-        const int64_t at = base + wave + (int64_t)lane * WAVES;
-        float m = -INFINITY;
-        if (at < a.nseg) m = segmax[at];
-        uint64_t todo = __ballot(m > -INFINITY && want(m));
-        while (todo) {
+      for (int64_t base = 0; base < a.nseg; base += WANTED) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.nsegs = 0;
+        float m[WANTED / THREADS];
+#pragma unroll
+        for (int j = 0; j < WANTED / THREADS; ++j) {
+          const int64_t at = base + j * THREADS + threadIdx.x;
+          m[j] = at < a.nseg ? segmax[at] : -INFINITY;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < WANTED / THREADS; ++j) {
+          const bool on = m[j] > -INFINITY && want(m[j]);
+          const uint64_t mask = __ballot(on);
+          if (mask) {
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.nsegs, (int)__popcll(mask));
+            at = __builtin_amdgcn_readfirstlane(at);
+            if (on) sh.segs[at + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(j * THREADS + threadIdx.x);
+          }
+        }
+        __syncthreads();
+        const int n = sh.nsegs;
+        for (int q = wave * 4; q < n; q += 4 * WAVES) {
           float x[4][4];
-          int l[4];
+          int64_t seg[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            l[j] = todo ? __ffsll((unsigned long long)todo) - 1 : -1;
-            todo &= todo - 1;
-            if (l[j] >= 0) load_raw<T>(a, b, base + wave + (int64_t)l[j] * WAVES, lane, x[j]);
+            seg[j] = base + __builtin_amdgcn_readfirstlane((int)sh.segs[min(q + j, n - 1)]);
+            load_raw<T>(a, b, seg[j], lane, x[j]);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (l[j] >= 0) {
+            if (q + j < n) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
-              f(base + wave + (int64_t)l[j] * WAVES, x[j]);
+              f(seg[j], x[j]);
             }
         }
       }
@@ -457,34 +525,55 @@ struct Source {
   }
 };
 
-// One listed score per thread (n <= RANK <= THREADS): is it among the best k (k = 0: all), given
-// above_c better ones outside the list, and what mass of the list is better than it.
+// The walk of every listed score (n <= RANK) over the list is shared out: a group of G waves has a
+// lane per score, each of the WAVES / G groups takes a part of the list.
+struct Share {
+  int i, j0, j1;  // this lane's score; its part of the list
+};
+__device__ __forceinline__ Share share_list(int n) {
+  const int wave = threadIdx.x >> 6;
+  const int G = n <= 64 ? 1 : n <= 128 ? 2 : 4;
+  const int parts = WAVES / G, part = wave / G, per = (n + parts - 1) / parts;
+  return Share{(wave % G) * 64 + (int)(threadIdx.x & 63), min(n, part * per), min(n, (part + 1) * per)};
+}
+
+// Thread i < n: is score i among the best k (k = 0: all), given above_c better ones outside the list, and
+// what mass of the list is better than it; sh.kept_m: the mass that top-k keeps.
 struct Slot {
   bool kept;
   uint64_t before;
 };
 
 __device__ __forceinline__ Slot rank_list(Shared& sh, int n, int64_t k, uint32_t above_c) {
-  Slot s{false, 0};
   const int i = threadIdx.x;
-  if (i == 0) sh.kept_m = 0;
-  __syncthreads();
-  if ((i & ~63) < n) {  // whole waves
-    const Entry e = sh.list[i < n ? i : 0];
-    uint32_t rank = 0;
-    uint64_t before = 0;
+  if (i < RANK) { sh.rank[i] = 0; sh.before[i] = 0; }
+  const Share w = share_list(n);
+  uint64_t mine = 0;
+  if (w.i < n) mine = sh.list[w.i].at;
+  uint32_t rank = 0;
+  uint64_t before = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const Entry o = sh.list[j];
-      const bool better = o.key > e.key || (o.key == e.key && o.idx < e.idx);
-      rank += better;
-      before += better ? o.w : (uint64_t)0;
-    }
-    s.before = before;
-    s.kept = i < n && (k == 0 || (int64_t)above_c + rank < k);
-    const uint64_t sum = wave_sum(s.kept ? e.w : (uint64_t)0);
-    if ((i & 63) == 0) atomicAdd(&sh.kept_m, (unsigned long long)sum);  // the mass that top-k keeps of the list
+  for (int j = w.j0; j < w.j1; ++j) {
+    const Entry o = sh.list[j];
+    const bool better = o.at > mine;
+    rank += better;
+    before += better ? o.w : (uint64_t)0;
   }
+  __syncthreads();
+  if (w.i < n) {
+    atomicAdd(&sh.rank[w.i], rank);
+    atomicAdd(&sh.before[w.i], (unsigned long long)before);
+  }
+  __syncthreads();
+  Slot s{false, 0};
+  uint64_t weight = 0, all;
+  if (i < n) {
+    s.before = sh.before[i];
+    s.kept = k == 0 || (int64_t)above_c + sh.rank[i] < k;
+    if (s.kept) weight = sh.list[i].w;
+  }
+  block_scan(weight, sh.scan_m, all);
+  if (i == 0) sh.kept_m = all;
   __syncthreads();
   return s;
 }
@@ -498,8 +587,9 @@ __device__ __forceinline__ void cut_by_mass(Slot& s, uint64_t above_m, double ta
 __device__ __forceinline__ void list_threshold(Shared& sh, const Slot& s) {
   if (threadIdx.x == 0) { sh.kmin = 0xffffffffu; sh.ties = 0; }
   __syncthreads();
-  const uint32_t key = s.kept ? sh.list[threadIdx.x].key : 0;
-  if (s.kept) atomicMin(&sh.kmin, key);
+  const uint32_t key = s.kept ? sh.list[threadIdx.x].key() : 0xffffffffu;
+  const uint32_t least = wave_min(key);
+  if ((threadIdx.x & 63) == 0) atomicMin(&sh.kmin, least);
   __syncthreads();
   if (s.kept && key == sh.kmin) atomicAdd(&sh.ties, 1u);
   __syncthreads();
@@ -512,13 +602,13 @@ __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, 
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  src.each(want, [&](int64_t seg, const float* v) {
+  src.each(sh, want, [&](int64_t seg, const float* v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (v[j] > -INFINITY && pick(key_of(v[j]), bin_of(v[j], M, cb))) {
         const int at = atomicAdd(&sh.n, 1);
         if (at < LIST)
-          sh.list[at] = Entry{key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), fixed(weight(v[j], M, r.c), shift)};
+          sh.list[at] = make_entry(key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), fixed(weight(v[j], M, r.c), shift));
       }
   });
   __syncthreads();
@@ -528,8 +618,8 @@ __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, 
 // many scores equal to it stay (sh.ties) and the mass above it (sh.before_m).  By count: `need` of
 // the set stay; by mass: those before which above_m + mass < target.  Only keys >= floor_key take
 // part.  each(g) calls g(on, key, w) for the set, all lanes of a wave together.
-template <typename E>
-__device__ __forceinline__ void split(Shared& sh, E each, bool by_mass, uint32_t need, uint64_t above_m, double target,
+template <Search S, typename E>
+__device__ __forceinline__ void split(Shared& sh, E each, uint32_t need, uint64_t above_m, double target,
                                       uint32_t floor_key) {
   uint32_t prefix = 0, mask = 0;
   for (int level = 0; level < 3; ++level) {
@@ -541,15 +631,15 @@ __device__ __forceinline__ void split(Shared& sh, E each, bool by_mass, uint32_t
                            (int)(width - ((key >> sft) & width)), w);
     });
     __syncthreads();
-    find_bin(sh, by_mass, true, need, above_m, target);
+    find_bin<S>(sh, need, above_m, target);
     prefix |= (width - (uint32_t)sh.bin) << sft;
     mask |= width << sft;
-    need -= min(need, sh.before_c);
+    if (S != BY_MASS) need -= min(need, sh.before_c);
     above_m += sh.before_m;
   }
   const uint32_t cnt = sh.hc[sh.bin];
   uint32_t ties = need;
-  if (by_mass) {  // tie number j stays while above + j w < target
+  if (S == BY_MASS) {  // tie number j stays while above + j w < target
     const uint64_t w = cnt ? sh.hm[sh.bin] / cnt : 0;
     const double room = target - (double)above_m;
     ties = w == 0 || room > (double)w * (double)cnt ? cnt : (uint32_t)fmax(0.0, ceil(room / (double)w));
@@ -565,42 +655,50 @@ template <typename G>
 __device__ __forceinline__ void each_listed(const Entry* list, int n, G g) {
   for (int i0 = 0; i0 < n; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
-    Entry e{0, 0, 0};
+    Entry e{0, 0};
     if (i < n) e = list[i];
-    g(i < n, e.key, e.w);
+    g(i < n, e.key(), e.w);
   }
 }
 
 // Draw from the kept entries of the list (n <= RANK), in index order.
 __device__ __forceinline__ void draw_from_list(const Args& a, int b, Shared& sh, int n, Slot s, const Row& r, float M) {
   const int i = threadIdx.x;
-  __syncthreads();
-  Entry mine{0, 0, 0};
+  Entry mine{0, 0};
   if (i < n) mine = sh.list[i];
-  if (s.kept && r.cut_min) s.kept = weight(score_of(mine.key), M, r.c) >= r.minp;
+  if (s.kept && r.cut_min) s.kept = weight(score_of(mine.key()), M, r.c) >= r.minp;
   if (!s.kept) mine.w = 0;
-  if (i < n) sh.list[i].w = mine.w;
-  if (i == 0) { sh.best = INT32_MAX; sh.bin = -1; }
+  if (i < RANK) sh.before[i] = 0;
+  if (i == 0) { sh.kmin = 0xffffffffu; sh.ties = 0xffffffffu; }
   uint64_t all;
-  block_scan(mine.w, sh.scan_m, all);
-  const double total = (double)all, target = (double)a.u[b] * total;
+  block_scan(mine.w, sh.scan_m, all);  // (its barriers also close the reads of the list)
+  if (i < n) sh.list[i].w = mine.w;
   __syncthreads();
-  if ((i & ~63) < n) {
-    uint64_t cum = 0;
+  const double total = (double)all, target = (double)a.u[b] * total;
+  const Share w = share_list(n);
+  uint32_t idx = 0;
+  if (w.i < n) idx = (uint32_t)sh.list[w.i].idx();
+  uint64_t cum = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const Entry o = sh.list[j];
-      cum += o.idx <= mine.idx ? o.w : (uint64_t)0;
-    }
-    if (mine.w) {
-      if ((double)cum > target) atomicMin(&sh.best, mine.idx);
-      atomicMax(&sh.bin, mine.idx);
-    }
+  for (int j = w.j0; j < w.j1; ++j) {
+    const Entry o = sh.list[j];
+    cum += (uint32_t)o.idx() <= idx ? o.w : (uint64_t)0;
+  }
+  if (w.i < n) atomicAdd(&sh.before[w.i], (unsigned long long)cum);
+  __syncthreads();
+  // the lowest index past the target; else the highest kept one
+  const uint32_t at = (uint32_t)mine.idx();
+  const bool live = i < n && mine.w;
+  const uint32_t low = wave_min(live && (double)sh.before[i < RANK ? i : 0] > target ? at : 0xffffffffu);
+  const uint32_t high = wave_min(live ? ~at : 0xffffffffu);
+  if ((i & 63) == 0) {
+    atomicMin(&sh.kmin, low);
+    atomicMin(&sh.ties, high);
   }
   __syncthreads();
-  const int pick = sh.best != INT32_MAX ? sh.best : sh.bin;
-  if (mine.w && mine.idx == pick) {
-    a.out[b] = pick;
+  const uint32_t pick = sh.kmin != 0xffffffffu ? sh.kmin : ~sh.ties;
+  if (live && at == pick) {
+    a.out[b] = (int32_t)pick;
     if (a.prob) a.prob[b] = (float)((double)mine.w / total);
   }
 }
@@ -630,63 +728,93 @@ struct Found {
   double total, target;
 };
 
-// The segment in which u * total falls: a thread sums its run of segments, the runs are scanned,
-// the thread that holds the target walks its run.  get(seg, mass, ties): a segment's mass of keys
-// above t and its count of ties (false: nothing of it stays).
+// The segment in which u * total falls.  Each wave sums a run of segments, 64 at a time; the wave
+// whose run holds the target walks it again.  get(seg, mass, ties): a segment's mass of keys above t
+// and its count of ties (false: nothing of it stays).
 template <typename V, typename G>
-__device__ __forceinline__ Found<V> find_segment(const Args& a, int b, uint32_t ties, V wt, G get, int* best, int* last,
-                                                 uint32_t* tmp_c, V* tmp_v, Found<V>* found) {
-  const int64_t per = (a.nseg + THREADS - 1) / THREADS;
-  const int64_t s0 = per * threadIdx.x, s1 = min(s0 + per, a.nseg);
-  uint32_t tie0 = 0, tall;
+__device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& sh, uint32_t ties, V wt, G get, V* tmp_v,
+                                                 Found<V>* found) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t run = (a.nseg + 64 * WAVES - 1) / (64 * WAVES) * 64;
+  const int64_t s0 = run * wave, s1 = min(s0 + run, a.nseg);
+  uint32_t tie0 = 0;
   if (ties) {
     uint32_t c = 0;
-    for (int64_t s = s0; s < s1; ++s) {
+#pragma unroll 4
+    for (int64_t s = s0 + lane; s < s1; s += 64) {
       V m;
       uint32_t x = 0;
       if (get(s, m, x)) c += x;
     }
-    tie0 = block_scan(c, tmp_c, tall) - c;
+    c = wave_sum(c);
+    __syncthreads();
+    if (lane == 0) sh.scan_c[wave] = c;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) tie0 += sh.scan_c[w];
   }
-  auto mass = [&](int64_t s, uint32_t& tie) {
+  // mass of segment s (0 past the run's end); all lanes of the wave together when ties count
+  uint32_t tie = tie0;
+  const auto mass = [&](int64_t s, uint32_t& before) {
     V m = 0;
     uint32_t x = 0;
-    if (!get(s, m, x)) return V(0);
+    if (s >= s1 || !get(s, m, x)) { m = 0; x = 0; }
+    before = 0;
     if (ties) {
-      m += (V)(tie < ties ? min(ties - tie, x) : 0u) * wt;
-      tie += x;
+      const uint32_t sum = wave_scan(x);
+      before = tie + sum - x;
+      tie += lane_value(sum, 63);
+      m += (V)(before < ties ? min(ties - before, x) : 0u) * wt;
     }
     return m;
   };
-  V sum = 0, all;
-  uint32_t tie = tie0;
-  for (int64_t s = s0; s < s1; ++s) sum += mass(s, tie);
-  if (threadIdx.x == 0) { *best = INT32_MAX; *last = -1; }
-  const V cum = block_scan(sum, tmp_v, all);
-  const double total = (double)all, target = (double)a.u[b] * total;
-  if (sum > 0) {
-    if ((double)cum > target) atomicMin(best, (int)threadIdx.x);
-    atomicMax(last, (int)threadIdx.x);
+  V sum = 0;
+  uint32_t none;
+  if (ties) {
+    for (int64_t s = s0; s < s1; s += 64) sum += mass(s + lane, none);
+  } else {
+#pragma unroll 8
+    for (int64_t s = s0 + lane; s < s1; s += 64) sum += mass(s, none);
   }
+  sum = wave_sum(sum);
   __syncthreads();
-  // rounding may put u * total past the last sum: then the last score of the last segment with mass
-  const bool over = *best == INT32_MAX;
-  if ((int)threadIdx.x == (over ? *last : *best)) {
-    V before = cum - sum;
-    tie = tie0;
-    Found<V> f{-1, before, tie0, total, over ? INFINITY : target};
-    for (int64_t s = s0; s < s1; ++s) {
-      const uint32_t t0 = tie;
-      const V m = mass(s, tie);
-      if (m > 0) {
-        f.seg = s;
-        f.before = before;
-        f.ties = t0;
-        if (!over && (double)(before + m) > target) break;
-      }
-      before += m;
+  if (lane == 0) tmp_v[wave] = sum;
+  __syncthreads();
+  V all = 0;
+  for (int w = 0; w < WAVES; ++w) all += tmp_v[w];
+  const double total = (double)all, target = (double)a.u[b] * total;
+  int pick = -1, last = -1;
+  V cum = 0, pick_before = 0, last_before = 0;
+  for (int w = 0; w < WAVES; ++w) {
+    const V m = tmp_v[w];
+    if (m > 0) {
+      last = w;
+      last_before = cum;
+      if (pick < 0 && (double)(cum + m) > target) { pick = w; pick_before = cum; }
     }
-    *found = f;
+    cum += m;
+  }
+  // rounding may put u * total past the last sum: then the last score of the last segment with mass
+  const bool over = pick < 0;
+  if (wave == (over ? last : pick)) {
+    V before = over ? last_before : pick_before;
+    tie = tie0;
+    Found<V> f{-1, before, 0, total, over ? INFINITY : target};
+    for (int64_t s = s0; s < s1; s += 64) {
+      uint32_t tb;
+      const V m = mass(s + lane, tb);
+      const V upto = before + wave_scan(m);
+      const uint64_t has = __ballot(m > 0), hits = __ballot(m > 0 && (double)upto > target);
+      if (has) {
+        const int l = hits && !over ? __ffsll((unsigned long long)hits) - 1 : 63 - __clzll(has);
+        f.seg = s + l;
+        f.before = lane_value(upto, l) - lane_value(m, l);
+        f.ties = lane_value(tb, l);
+        if (hits && !over) break;
+      }
+      before = lane_value(upto, 63);
+    }
+    // (a run whose sum passed the target while its steps do not, by rounding: its last score)
+    if (lane == 0) *found = f;
   }
   __syncthreads();
   return *found;
@@ -742,7 +870,7 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
     if (r.cut_min && wt < r.minp) { wt = 0; ties = 0; }
   }
   if (!have_mass)
-    src.each([&](float m) { return m >= bound; }, [&](int64_t seg, const float* v) {
+    src.each(sh, [&](float m) { return m >= bound; }, [&](int64_t seg, const float* v) {
       double m = 0;
       uint32_t c = 0;
 #pragma unroll
@@ -760,7 +888,7 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
     });
   __syncthreads();
   const Found<double> f = find_segment<double>(
-      a, b, ties, wt,
+      a, b, sh, ties, wt,
       [&](int64_t s, double& m, uint32_t& c) {
         const float x = src.segmax[s];
         if (!(x >= bound) || x == -INFINITY) return false;
@@ -769,7 +897,7 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
         else c = (uint32_t)segtie[s];
         return true;
       },
-      &sh.best, &sh.bin, sh.scan_c, sh.scan_d, &found);
+      sh.scan_d, &found);
   if (src.wave == (R == ROW_REGS ? (int)f.seg : 0)) {
     float v[4];
     if constexpr (R == ROW_REGS) {
@@ -791,7 +919,7 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
   const int shift = shift_for((double)a.N);
   const auto any = [](float) { return true; };
   clear_hist(sh);
-  src.each(any, [&](int64_t, const float* v) {
+  src.each(sh, any, [&](int64_t, const float* v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint64_t w = r.cut_p ? fixed(weight(v[j], M, r.c), shift) : 0;
@@ -800,14 +928,14 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
   });
   __syncthreads();
   const auto reaches = [&](int bin) { return [=](float m) { return bin_of(m, M, cb) <= bin; }; };
-  const auto split_row = [&](int bin, bool by_mass, uint32_t need, uint64_t above, double target, uint32_t floor_key) {
-    split(sh, [&](auto g) {
-      src.each(reaches(bin), [&](int64_t, const float* v) {
+  const auto of_bin = [&](int bin) {
+    return [=, &src, &sh, &r](auto g) {
+      src.each(sh, [=](float m) { return bin_of(m, M, cb) <= bin; }, [&](int64_t, const float* v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           g(v[j] > -INFINITY && bin_of(v[j], M, cb) == bin, key_of(v[j]), fixed(weight(v[j], M, r.c), shift));
       });
-    }, by_mass, need, above, target, floor_key);
+    };
   };
   uint32_t t = KEY_NONE, ties = 0;
   uint64_t total = 0;
@@ -820,19 +948,22 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
     m[j] = sh.hm[PER * threadIdx.x + j];
   }
   if (r.k > 0) {
-    find_bin(sh, false, true, (uint32_t)r.k, 0, 0.0);
+    find_bin<BY_COUNT_WITH_MASS>(sh, (uint32_t)r.k);
     kbin = sh.bin;
     const uint64_t kbefore = sh.before_m;
     const uint32_t cbefore = sh.before_c;
     if (cbefore + sh.hc[kbin] <= (uint32_t)r.k) {  // the whole bin stays: above the key below its smallest
       total = kbefore + sh.hm[kbin];
       if (threadIdx.x == 0) sh.kmin = 0xffffffffu;
-      __syncthreads();
-      src.each(reaches(kbin), [&](int64_t, const float* v) {
+      uint32_t least = 0xffffffffu;
+      src.each(sh, reaches(kbin), [&](int64_t, const float* v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (v[j] > -INFINITY && bin_of(v[j], M, cb) == kbin) atomicMin(&sh.kmin, key_of(v[j]));
+          least = min(least, v[j] > -INFINITY && bin_of(v[j], M, cb) == kbin ? key_of(v[j]) : 0xffffffffu);
       });
+      __syncthreads();
+      least = wave_min(least);
+      if (src.lane == 0) atomicMin(&sh.kmin, least);
       __syncthreads();
       t = sh.kmin - 1;
     } else {
@@ -844,8 +975,8 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
         list_threshold(sh, s);
       } else {
         const uint32_t need = (uint32_t)(r.k - cbefore);
-        if (n <= LIST) split(sh, [&](auto g) { each_listed(sh.list, n, g); }, false, need, kbefore, 0.0, 0);
-        else split_row(kbin, false, need, kbefore, 0.0, 0);
+        if (n <= LIST) split<BY_COUNT_WITH_MASS>(sh, [&](auto g) { each_listed(sh.list, n, g); }, need, kbefore, 0.0, 0);
+        else split<BY_COUNT_WITH_MASS>(sh, of_bin(kbin), need, kbefore, 0.0, 0);
         total = sh.before_m + (uint64_t)sh.ties * fixed(weight(score_of(sh.kmin), M, r.c), shift);
       }
       t = sh.kmin;
@@ -863,15 +994,8 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
     }
   }
   if (r.cut_p) {
-    if (r.k == 0) {
-      uint64_t mt = 0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) mt += m[j];
-      block_scan(mt, sh.scan_m, total);
-      __syncthreads();
-    }
-    const double target = r.p * (double)total;
-    find_bin(sh, true, true, 0, 0, target);
+    find_bin<BY_MASS>(sh, 0, 0, 0, fmax(r.p, 0.0));
+    const double target = sh.target;
     const int bin = sh.bin;
     const uint64_t above = sh.before_m;
     const uint32_t floor_key = bin == kbin ? (ties ? t : t + 1) : 0;  // what top-k left of this bin
@@ -886,9 +1010,9 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
       cut_by_mass(s, above, target);
       list_threshold(sh, s);
     } else if (n <= LIST) {
-      split(sh, [&](auto g) { each_listed(sh.list, n, g); }, true, 0, above, target, floor_key);
+      split<BY_MASS>(sh, [&](auto g) { each_listed(sh.list, n, g); }, 0, above, target, floor_key);
     } else {
-      split_row(bin, true, 0, above, target, floor_key);
+      split<BY_MASS>(sh, of_bin(bin), 0, above, target, floor_key);
     }
     t = sh.kmin;
     ties = t == floor_key ? min(sh.ties, tie_cap) : sh.ties;
@@ -957,14 +1081,12 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
         if (segmax[i] > -INFINITY) sum += segmass[i] * weight(segmax[i], M, r.c);
       block_scan(sum, sh.scan_d, total);
       // N scores below (1 - p) total / N hold less than (1 - p) total: the threshold is not among
-      // them, and the bins span the octaves above that
+      // them, and the bins but the last span the octaves above that
       const double least = fmax((1 - r.p) * total / (double)a.N, 0x1p-60);
       const double octaves = fmax(-log2(least), 0.0) + 0.125;
       for (int i = threadIdx.x; i < BINS; i += THREADS) a.hmass[(int64_t)b * BINS + i] = 0;
-      if (threadIdx.x == 0) {
-        const int shift = shift_for(total);
-        a.state[b] = RowState{1, M, (float)(r.c * (BINS - 1) / octaves), shift, r.p * total * (double)(1ull << shift), 0, 0, 0};
-      }
+      if (threadIdx.x == 0)
+        a.state[b] = RowState{1, M, (float)(r.c * (BINS - 1) / octaves), shift_for(2 * total), 0, 0, 0, 0};
       return;
     }
   }
@@ -985,14 +1107,14 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
         if (x > -INFINITY) atomicAdd(&sh.hc[bin_of(x, M, cb)], 1u);
       }
     } else {
-      src.each(any, [&](int64_t, const float* v) {
+      src.each(sh, any, [&](int64_t, const float* v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           hist_add<true, false>(sh.hc, sh.hm, v[j] > -INFINITY, bin_of(v[j], M, cb), 0);
       });
     }
     __syncthreads();
-    find_bin(sh, false, false, (uint32_t)r.k, 0, 0.0);
+    find_bin<BY_COUNT>(sh, (uint32_t)r.k);
     // fewer unmasked than k: everything unmasked is a candidate
     const int edge = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k ? BINS : sh.bin;
     collect<T, R>(src, sh, M, r, cb, 51, [&](float x) { return bin_of(x, M, cb) <= edge; },
@@ -1006,11 +1128,11 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     }
     if (n <= LIST) {
       const auto listed = [&](auto g) { each_listed(sh.list, n, g); };
-      split(sh, listed, false, (uint32_t)r.k, 0, 0.0, 0);
+      split<BY_COUNT_WITH_MASS>(sh, listed, (uint32_t)r.k, 0, 0.0, 0);
       uint32_t t = sh.kmin, ties = sh.ties;
       if (r.cut_p) {
         const uint64_t total = sh.before_m + (uint64_t)ties * fixed(weight(score_of(t), M, r.c), 51);
-        split(sh, listed, true, 0, 0, r.p * (double)total, t);
+        split<BY_MASS>(sh, listed, 0, 0, r.p * (double)total, t);
         ties = sh.kmin == t ? min(ties, sh.ties) : sh.ties;
         t = sh.kmin;
       }
@@ -1032,6 +1154,7 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
   const Row r = row_settings(a, b);
   for (int i = threadIdx.x; i < BINS; i += THREADS) hm[i] = 0;
   __syncthreads();
+  uint64_t rest = 0;  // the last bin's mass: scores that cannot hold the threshold
   const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
   for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
     float x[4][4];
@@ -1044,13 +1167,17 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
       for (int i = 0; i < 4; ++i) {
         const float v = clean(x[j][i]);
         const int bin = bin_of(v, st.M, st.cb);
+        const uint64_t w = v > -INFINITY ? fixed(weight(v, st.M, r.c), st.shift) : (uint64_t)0;
         const bool on = v > -INFINITY && bin < BINS - 1;
-        if (__ballot(on)) hist_add<false, true>(nullptr, hm, on, bin, fixed(weight(v, st.M, r.c), st.shift));
+        if (!on) rest += w;
+        hist_add<false, true>(nullptr, hm, on, bin, w);
       }
     }
   }
+  rest = wave_sum(rest);
+  if (lane == 0 && rest) atomicAdd(&hm[BINS - 1], (unsigned long long)rest);
   __syncthreads();
-  for (int i = threadIdx.x; i < BINS - 1; i += THREADS)
+  for (int i = threadIdx.x; i < BINS; i += THREADS)
     if (hm[i]) atomicAdd((unsigned long long*)a.hmass + (int64_t)b * BINS + i, hm[i]);
 }
 
@@ -1058,14 +1185,15 @@ template <int T>
 __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   __shared__ Shared sh;
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const RowState st = a.state[b];  // (listed, bin and above are written by this kernel, and not read)
+  const RowState st = a.state[b];  // (target, bin, above and listed are written by this kernel, and not read)
   if (!st.active) return;
   const Row r = row_settings(a, b);
-  for (int i = threadIdx.x; i < BINS; i += THREADS) { sh.hc[i] = 0; sh.hm[i] = a.hmass[(int64_t)b * BINS + i]; }
+  for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hm[i] = a.hmass[(int64_t)b * BINS + i];
   __syncthreads();
-  find_bin(sh, true, true, 0, 0, st.target);
+  find_bin<BY_MASS>(sh, 0, 0, 0, fmax(r.p, 0.0));
   const int bin = sh.bin;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.state[b].target = sh.target;
     a.state[b].bin = bin;
     a.state[b].above = sh.before_m;
   }
@@ -1091,7 +1219,7 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
           if (on && at_bin == bin) {
             const uint32_t at = atomicAdd(&a.state[b].listed, 1u);
             if (at < (uint32_t)a.listcap)
-              a.list[(int64_t)b * a.listcap + at] = Entry{key_of(v), (int32_t)(seg * SEG + lane * 4 + i), fw};
+              a.list[(int64_t)b * a.listcap + at] = make_entry(key_of(v), (int32_t)(seg * SEG + lane * 4 + i), fw);
           }
         }
       }
@@ -1125,38 +1253,58 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
     cut_by_mass(s, st.above, st.target);
     list_threshold(sh, s);
   } else {
-    split(sh, [&](auto g) { each_listed(list, n, g); }, true, 0, st.above, st.target, 0);
+    split<BY_MASS>(sh, [&](auto g) { each_listed(list, n, g); }, 0, st.above, st.target, 0);
   }
   const uint32_t t = sh.kmin;
   uint32_t ties = sh.ties;
   const AsFixed w_of{st.M, r.c, st.shift};
   uint64_t wt = w_of(score_of(t));
   if (r.cut_min && weight(score_of(t), st.M, r.c) < r.minp) { wt = 0; ties = 0; }
-  // listed scores above t join their segments' masses; ties are counted per segment
-  int32_t* segtie = a.segtie + (int64_t)b * a.nseg;
-  if (ties)
-    for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS) segtie[s] = 0;
-  __threadfence();
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const Entry e = list[i];
-    if (e.key > t) {
-      if (!r.cut_min || weight(score_of(e.key), st.M, r.c) >= r.minp)
-        atomicAdd((unsigned long long*)segmass + e.idx / SEG, (unsigned long long)e.w);
-    } else if (e.key == t && ties) {
-      atomicAdd(segtie + e.idx / SEG, 1);
+  // Listed scores above t add to their segments' masses, ties are counted per segment: in LDS (the
+  // list's and the histogram's) for up to 2 LIST segments, else in the workspace.
+  const auto add = [&](auto plus_mass, auto plus_tie) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const Entry e = list[i];
+      if (e.key() > t) {
+        if (!r.cut_min || weight(score_of(e.key()), st.M, r.c) >= r.minp) plus_mass(e.idx() / SEG, e.w);
+      } else if (e.key() == t && ties) {
+        plus_tie(e.idx() / SEG);
+      }
     }
+  };
+  Found<uint64_t> f;
+  if (a.nseg <= 2 * LIST) {
+    unsigned long long* more = (unsigned long long*)sh.list;
+    uint32_t* tied = (uint32_t*)sh.hm;
+    static_assert(2 * LIST * 4 <= BINS * 8, "a tie count per segment");
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.nseg; s += THREADS) { more[s] = 0; tied[s] = 0; }
+    __syncthreads();
+    add([&](int s, uint64_t w) { atomicAdd(more + s, (unsigned long long)w); }, [&](int s) { atomicAdd(tied + s, 1u); });
+    __syncthreads();
+    f = find_segment<uint64_t>(a, b, sh, ties, wt, [&](int64_t s, uint64_t& m, uint32_t& c) {
+      m = segmass[s] + more[s];
+      c = tied[s];
+      return true;
+    }, sh.scan_m, &found);
+  } else {
+    // agent-scope accesses meet in the L2 that this one workgroup works through; the waits put the
+    // zeros before the sums and the sums before the reads
+    int32_t* segtie = a.segtie + (int64_t)b * a.nseg;
+    for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS)
+      __hip_atomic_store(segtie + s, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    add([&](int s, uint64_t w) { atomicAdd((unsigned long long*)segmass + s, (unsigned long long)w); },
+        [&](int s) { atomicAdd(segtie + s, 1); });
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    f = find_segment<uint64_t>(a, b, sh, ties, wt, [&](int64_t s, uint64_t& m, uint32_t& c) {
+      m = __hip_atomic_load(segmass + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      c = (uint32_t)__hip_atomic_load(segtie + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return true;
+    }, sh.scan_m, &found);
   }
-  __threadfence();
-  __syncthreads();
-  const Found<uint64_t> f = find_segment<uint64_t>(
-      a, b, ties, wt,
-      [&](int64_t s, uint64_t& m, uint32_t& c) {
-        m = __hip_atomic_load(segmass + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (ties) c = (uint32_t)__hip_atomic_load(segtie + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return true;
-      },
-      &sh.best, &sh.bin, sh.scan_c, sh.scan_m, &found);
   if (threadIdx.x < 64) {
     float v[4];
     load_seg<T>(a, b, f.seg, lane, v);
