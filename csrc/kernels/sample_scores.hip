@@ -40,7 +40,7 @@ constexpr int LIST = 2048;      // scores listed in LDS
 constexpr int RANK = 256;       // listed scores ranked against each other; more are split by bits
 constexpr int SHORT_K = 1024;   // top-k up to this lists its candidates
 constexpr int CACHED_SEGS = 128;     // segments of a row that takes one launch
-constexpr int PASS_SEGS = 128;  // segments per workgroup of the passes over long rows
+constexpr int PASS_SEGS = 64;   // segments per workgroup of the passes over long rows
 
 // a listed score: its key above the complement of its index (the larger word is the better score,
 // equal scores by the lower index), and its weight
@@ -124,6 +124,14 @@ __device__ __forceinline__ float score_of(uint32_t k) {
 }
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // key_of(-inf)
 
+// p f + c with the coefficient in scalar registers (the compiler's form copies each coefficient
+// into vector registers first: 152 cycles a wave for one weight() against FILLME here)
+__device__ __forceinline__ double horner(double p, double f, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(p), "v"(f), "s"(c));
+  return r;
+}
+
 // 2^((s - M) c): interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 8 (relative
 // error 1.1e-12: two answers differ where u * total falls that near to a step), times the
 // power of two.  n = round(t) is read from the low bits of t + 1.5 * 2^52.
@@ -134,14 +142,14 @@ __device__ __forceinline__ double weight(float s, float M, double c) {
   const double u = t + 6755399441055744.0;
   const double f = t - (u - 6755399441055744.0);
   double p = 0x1.63d1363a7ecb6p-20;
-  p = __builtin_fma(p, f, 0x1.00dc4a534054dp-16);
-  p = __builtin_fma(p, f, 0x1.4308ac85a6c21p-13);
-  p = __builtin_fma(p, f, 0x1.5d8745a72827ap-10);
-  p = __builtin_fma(p, f, 0x1.3b2ab7181b778p-7);
-  p = __builtin_fma(p, f, 0x1.c6b08dd6fd236p-5);
-  p = __builtin_fma(p, f, 0x1.ebfbdff823cedp-3);
-  p = __builtin_fma(p, f, 0x1.62e42fef84cf0p-1);
-  p = __builtin_fma(p, f, 0x1.0000000000000p+0);
+  p = horner(p, f, 0x1.00dc4a534054dp-16);
+  p = horner(p, f, 0x1.4308ac85a6c21p-13);
+  p = horner(p, f, 0x1.5d8745a72827ap-10);
+  p = horner(p, f, 0x1.3b2ab7181b778p-7);
+  p = horner(p, f, 0x1.c6b08dd6fd236p-5);
+  p = horner(p, f, 0x1.ebfbdff823cedp-3);
+  p = horner(p, f, 0x1.62e42fef84cf0p-1);
+  p = horner(p, f, 0x1.0000000000000p+0);
   const double w = __longlong_as_double(__double_as_longlong(p) + ((__double_as_longlong(u) << 52)));
   return t0 > -1020.0 ? w : 0.0;
 }
@@ -219,6 +227,10 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ double lanes_below(double v) {
   return __longlong_as_double((int64_t)lanes_below<CTRL, ROWS>((uint64_t)__double_as_longlong(v)));
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float lanes_below(float v) {
+  return __uint_as_float(lanes_below<CTRL, ROWS>(__float_as_uint(v)));
+}
 // inclusive sum over the lanes of the wave (all 64 active)
 template <typename V>
 __device__ __forceinline__ V wave_scan(V v) {
@@ -236,6 +248,7 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) {
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int l) {
   return (uint64_t)lane_value((uint32_t)v, l) | ((uint64_t)lane_value((uint32_t)(v >> 32), l) << 32);
 }
+__device__ __forceinline__ float lane_value(float v, int l) { return __uint_as_float(lane_value(__float_as_uint(v), l)); }
 __device__ __forceinline__ double lane_value(double v, int l) {
   return __longlong_as_double((int64_t)lane_value((uint64_t)__double_as_longlong(v), l));
 }
@@ -297,7 +310,7 @@ __device__ __forceinline__ float block_max(float v, float* tmp) {
 }
 
 // ---- long rows, pass 1: the largest score of every segment, its mass where masses decide ----
-constexpr int STAT_SEGS = 8;  // per wave: 8 loads in flight a lane
+constexpr int STAT_SEGS = 4;  // per wave
 template <int T>
 __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   const int b = blockIdx.y, lane = threadIdx.x & 63;
@@ -330,8 +343,8 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
     } else if (rough) {
       float w = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w += v[j][i] == m ? 1.f : v[j][i] > -INFINITY ? exp2f((v[j][i] - m) * cf) : 0.f;
-      w = group_sum<64>(w);
+      for (int i = 0; i < 4; ++i) w += v[j][i] == m ? 1.f : v[j][i] > -INFINITY ? __builtin_amdgcn_exp2f((v[j][i] - m) * cf) : 0.f;
+      w = wave_sum(w);
       if (lane == j) ws = w;
     }
   }
@@ -365,24 +378,30 @@ __device__ __forceinline__ void hist_add(uint32_t* hc, unsigned long long* hm, b
 
 constexpr int WANTED = 4 * THREADS;  // segments looked at together
 
-struct Shared {
+template <bool COUNTS>
+struct Hist {
   unsigned long long hm[BINS];
-  uint32_t hc[BINS];
+  uint32_t hc[COUNTS ? BINS : 1];
+  uint64_t scan_m[WAVES];
+  uint32_t scan_c[WAVES];
+  int wave_hit[WAVES], wave_any[WAVES];
+  // what a search found, written by one thread
+  int bin;
+  uint32_t before_c;
+  unsigned long long before_m;
+  double target;
+};
+
+struct Shared : Hist<true> {
   Entry list[LIST];
   uint32_t rank[RANK];
   unsigned long long before[RANK];
   uint16_t segs[WANTED];
-  int nsegs;
-  int wave_hit[WAVES], wave_any[WAVES];
+  int nsegs, n;
   float tmp[WAVES];
-  uint32_t scan_c[WAVES];
-  uint64_t scan_m[WAVES];
   double scan_d[WAVES];
-  // results of searches, written by one thread
-  int bin, n;
-  uint32_t kmin, ties, before_c;
-  double target;
-  unsigned long long before_m, kept_m;
+  uint32_t kmin, ties;
+  unsigned long long kept_m;
 };
 
 __device__ __forceinline__ void clear_hist(Shared& sh) {
@@ -407,8 +426,8 @@ enum Search { BY_COUNT, BY_COUNT_WITH_MASS, BY_MASS };
 // added to `above`, first reaches the target: sh.bin, and what lies before it: sh.before_c,
 // sh.before_m.  part >= 0: the target is that part of all mass (sh.target).  Where rounding lets no
 // bin reach it: the last bin that holds anything.
-template <Search S>
-__device__ __forceinline__ void find_bin(Shared& sh, uint32_t need, uint64_t above = 0, double target = 0, double part = -1) {
+template <Search S, typename H>
+__device__ __forceinline__ void find_bin(H& sh, uint32_t need, uint64_t above = 0, double target = 0, double part = -1) {
   const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
   uint32_t c[PER], ct = 0, cc = 0, call;
   uint64_t m[PER], mt = 0, mm = 0, mall;
@@ -475,8 +494,8 @@ struct Source {
   __device__ Source(const Args& a_, int b_, const float* sm)
       : a(a_), b(b_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), segmax(sm) {}
   // f(segment, scores) for the segments whose largest score (not -inf) is wanted.  Their maxima
-  // are looked at first, many together; the waves share out the wanted ones and load four at a time.
-  template <typename P, typename F>
+  // are looked at first, many together; the waves share out the wanted ones and load G at a time.
+  template <int G = 4, typename P, typename F>
   __device__ __forceinline__ void each(Shared& sh, P want, F f) {
     if constexpr (R == ROW_REGS) {
       if (wave < a.nseg) f((int64_t)wave, v);
@@ -504,16 +523,16 @@ struct Source {
         }
         __syncthreads();
         const int n = sh.nsegs;
-        for (int q = wave * 4; q < n; q += 4 * WAVES) {
-          float x[4][4];
-          int64_t seg[4];
+        for (int q = wave * G; q < n; q += G * WAVES) {
+          float x[G][4];
+          int64_t seg[G];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < G; ++j) {
             seg[j] = base + __builtin_amdgcn_readfirstlane((int)sh.segs[min(q + j, n - 1)]);
             load_raw<T>(a, b, seg[j], lane, x[j]);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < G; ++j)
             if (q + j < n) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
@@ -595,6 +614,26 @@ __device__ __forceinline__ void list_threshold(Shared& sh, const Slot& s) {
   __syncthreads();
 }
 
+// Places in a list for the scores of a segment that the lanes want (on[4]): one atomic on its count per
+// segment.  Returns how many the wave took.
+__device__ __forceinline__ int take_places(const bool on[4], int* count, int place[4]) {
+  const int lane = threadIdx.x & 63;
+  int total = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t mask = __ballot(on[j]);
+    place[j] = total + __popcll(mask & ((1ull << lane) - 1));
+    total += __popcll(mask);
+  }
+  if (total == 0) return 0;
+  int at = 0;
+  if (lane == 0) at = atomicAdd(count, total);
+  at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) place[j] += at;
+  return total;
+}
+
 // Put the scores for which pick(key, bin) holds into sh.list; sh.n counts them all.
 template <int T, int R, typename P, typename F>
 __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, const Row& r, float cb, int shift,
@@ -602,15 +641,19 @@ __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, 
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  src.each(sh, want, [&](int64_t seg, const float* v) {
+  src.template each<8>(sh, want, [&](int64_t seg, const float* v) {
+    bool on[4];
+    int place[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) on[j] = v[j] > -INFINITY && pick(key_of(v[j]), bin_of(v[j], M, cb));
+    if (take_places(on, &sh.n, place) == 0) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (v[j] > -INFINITY && pick(key_of(v[j]), bin_of(v[j], M, cb))) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < LIST)
-          sh.list[at] = make_entry(key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), fixed(weight(v[j], M, r.c), shift));
-      }
+      if (on[j] && place[j] < LIST) sh.list[place[j]].at = make_entry(key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), 0).at;
   });
+  __syncthreads();
+  if (sh.n <= LIST)
+    for (int i = threadIdx.x; i < sh.n; i += THREADS) sh.list[i].w = fixed(weight(score_of(sh.list[i].key()), M, r.c), shift);
   __syncthreads();
 }
 
@@ -728,56 +771,42 @@ struct Found {
   double total, target;
 };
 
-// The segment in which u * total falls.  Each wave sums a run of segments, 64 at a time; the wave
-// whose run holds the target walks it again.  get(seg, mass, ties): a segment's mass of keys above t
-// and its count of ties (false: nothing of it stays).
+// The segment in which u * total falls: every lane sums a run of segments, the lane whose run holds
+// the target has its wave walk it.  get(seg, mass, ties): a segment's mass of keys above t and its
+// count of ties (false: nothing of it stays).
 template <typename V, typename G>
 __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& sh, uint32_t ties, V wt, G get, V* tmp_v,
                                                  Found<V>* found) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t run = (a.nseg + 64 * WAVES - 1) / (64 * WAVES) * 64;
-  const int64_t s0 = run * wave, s1 = min(s0 + run, a.nseg);
-  uint32_t tie0 = 0;
+  const int64_t run = (a.nseg + THREADS - 1) / THREADS;
+  const int64_t s0 = min(run * threadIdx.x, a.nseg), s1 = min(s0 + run, a.nseg);
+  uint32_t tie0 = 0, tall;
   if (ties) {
     uint32_t c = 0;
 #pragma unroll 4
-    for (int64_t s = s0 + lane; s < s1; s += 64) {
+    for (int64_t s = s0; s < s1; ++s) {
       V m;
       uint32_t x = 0;
       if (get(s, m, x)) c += x;
     }
-    c = wave_sum(c);
-    __syncthreads();
-    if (lane == 0) sh.scan_c[wave] = c;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) tie0 += sh.scan_c[w];
+    tie0 = block_scan(c, sh.scan_c, tall) - c;
   }
-  // mass of segment s (0 past the run's end); all lanes of the wave together when ties count
+  V sum = 0;
   uint32_t tie = tie0;
-  const auto mass = [&](int64_t s, uint32_t& before) {
+#pragma unroll 8
+  for (int64_t s = s0; s < s1; ++s) {
     V m = 0;
     uint32_t x = 0;
-    if (s >= s1 || !get(s, m, x)) { m = 0; x = 0; }
-    before = 0;
+    if (!get(s, m, x)) { m = 0; x = 0; }
     if (ties) {
-      const uint32_t sum = wave_scan(x);
-      before = tie + sum - x;
-      tie += lane_value(sum, 63);
-      m += (V)(before < ties ? min(ties - before, x) : 0u) * wt;
+      m += (V)(tie < ties ? min(ties - tie, x) : 0u) * wt;
+      tie += x;
     }
-    return m;
-  };
-  V sum = 0;
-  uint32_t none;
-  if (ties) {
-    for (int64_t s = s0; s < s1; s += 64) sum += mass(s + lane, none);
-  } else {
-#pragma unroll 8
-    for (int64_t s = s0 + lane; s < s1; s += 64) sum += mass(s, none);
+    sum += m;
   }
-  sum = wave_sum(sum);
+  const V in_wave = wave_scan(sum);
   __syncthreads();
-  if (lane == 0) tmp_v[wave] = sum;
+  if (lane == 63) tmp_v[wave] = in_wave;
   __syncthreads();
   V all = 0;
   for (int w = 0; w < WAVES; ++w) all += tmp_v[w];
@@ -796,24 +825,42 @@ __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& s
   // rounding may put u * total past the last sum: then the last score of the last segment with mass
   const bool over = pick < 0;
   if (wave == (over ? last : pick)) {
-    V before = over ? last_before : pick_before;
-    tie = tie0;
-    Found<V> f{-1, before, 0, total, over ? INFINITY : target};
-    for (int64_t s = s0; s < s1; s += 64) {
-      uint32_t tb;
-      const V m = mass(s + lane, tb);
+    // the first of 64 values, in order after `before`, that has mass and passes the target (or the last
+    // with mass): lane -1 if none has mass
+    const auto choose = [&](V m, V before, bool& hit) {
       const V upto = before + wave_scan(m);
-      const uint64_t has = __ballot(m > 0), hits = __ballot(m > 0 && (double)upto > target);
-      if (has) {
-        const int l = hits && !over ? __ffsll((unsigned long long)hits) - 1 : 63 - __clzll(has);
-        f.seg = s + l;
-        f.before = lane_value(upto, l) - lane_value(m, l);
-        f.ties = lane_value(tb, l);
-        if (hits && !over) break;
+      const uint64_t has = __ballot(m > 0), hits = over ? 0 : __ballot(m > 0 && (double)upto > target);
+      hit = hits != 0;
+      return hits ? __ffsll((unsigned long long)hits) - 1 : has ? 63 - __clzll(has) : -1;
+    };
+    bool hit;
+    V before = over ? last_before : pick_before;
+    const int l = choose(sum, before, hit);
+    before += lane_value(in_wave, l) - lane_value(sum, l);
+    tie = lane_value(tie0, l);
+    const int64_t first = run * (wave * 64 + l), end = min(first + run, a.nseg);
+    Found<V> f{-1, before, 0, total, over ? INFINITY : target};
+    for (int64_t s = first; s < end; s += 64) {
+      V m = 0;
+      uint32_t x = 0;
+      if (s + lane >= end || !get(s + lane, m, x)) { m = 0; x = 0; }
+      uint32_t tb = tie;
+      if (ties) {
+        const uint32_t scan = wave_scan(x);
+        tb = tie + scan - x;
+        tie += lane_value(scan, 63);
+        m += (V)(tb < ties ? min(ties - tb, x) : 0u) * wt;
       }
-      before = lane_value(upto, 63);
+      const int at = choose(m, before, hit);
+      const V upto = wave_scan(m);
+      if (at >= 0) {
+        f.seg = s + at;
+        f.before = before + (lane_value(upto, at) - lane_value(m, at));
+        f.ties = lane_value(tb, at);
+        if (hit) break;
+      }
+      before += lane_value(upto, 63);
     }
-    // (a run whose sum passed the target while its steps do not, by rounding: its last score)
     if (lane == 0) *found = f;
   }
   __syncthreads();
@@ -1169,8 +1216,8 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
         const int bin = bin_of(v, st.M, st.cb);
         const uint64_t w = v > -INFINITY ? fixed(weight(v, st.M, r.c), st.shift) : (uint64_t)0;
         const bool on = v > -INFINITY && bin < BINS - 1;
-        if (!on) rest += w;
-        hist_add<false, true>(nullptr, hm, on, bin, w);
+        if (on) atomicAdd(&hm[bin], (unsigned long long)w);
+        else rest += w;
       }
     }
   }
@@ -1181,9 +1228,14 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
     if (hm[i]) atomicAdd((unsigned long long*)a.hmass + (int64_t)b * BINS + i, hm[i]);
 }
 
+constexpr int PASS_LIST = 512;  // scores of the threshold's bin that a workgroup lists
+
 template <int T>
 __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
-  __shared__ Shared sh;
+  __shared__ Hist<false> sh;
+  __shared__ Entry listed[PASS_LIST];
+  __shared__ float above[WAVES][SEG];
+  __shared__ int count;
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const RowState st = a.state[b];  // (target, bin, above and listed are written by this kernel, and not read)
   if (!st.active) return;
@@ -1197,6 +1249,12 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
     a.state[b].bin = bin;
     a.state[b].above = sh.before_m;
   }
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  const auto put = [&](uint32_t at, Entry e) {
+    e.w = fixed(weight(score_of(e.key()), st.M, r.c), st.shift);
+    if (at < (uint32_t)a.listcap) a.list[(int64_t)b * a.listcap + at] = e;
+  };
   const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
   for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
     float x[4][4];
@@ -1206,27 +1264,42 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
     for (int j = 0; j < 4; ++j) {
       const int64_t seg = seg0 + j * WAVES;
       if (seg >= s1) continue;
-      uint64_t sum = 0;
+      // scores above the threshold's bin are moved together, so that a wave computes 64 weights at once
+      bool up[4], in[4];
+      int place[4], n = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float v = clean(x[j][i]);
-        const int at_bin = bin_of(v, st.M, st.cb);
-        const bool on = v > -INFINITY && at_bin <= bin;
-        if (__ballot(on)) {
-          const double w = weight(v, st.M, r.c);
-          const uint64_t fw = fixed(w, st.shift);
-          if (on && at_bin < bin) sum += !r.cut_min || w >= r.minp ? fw : (uint64_t)0;
-          if (on && at_bin == bin) {
-            const uint32_t at = atomicAdd(&a.state[b].listed, 1u);
-            if (at < (uint32_t)a.listcap)
-              a.list[(int64_t)b * a.listcap + at] = make_entry(key_of(v), (int32_t)(seg * SEG + lane * 4 + i), fw);
-          }
-        }
+        x[j][i] = clean(x[j][i]);
+        const int at_bin = x[j][i] > -INFINITY ? bin_of(x[j][i], st.M, st.cb) : BINS;
+        in[i] = at_bin == bin;
+        up[i] = at_bin < bin;
+        const uint64_t mask = __ballot(up[i]);
+        if (up[i]) above[wave][n + __popcll(mask & ((1ull << lane) - 1))] = x[j][i];
+        n += __popcll(mask);
+      }
+      uint64_t sum = 0;
+      for (int i = lane; i < n; i += 64) {
+        const double w = weight(above[wave][i], st.M, r.c);
+        if (!r.cut_min || w >= r.minp) sum += fixed(w, st.shift);
       }
       sum = wave_sum(sum);
       if (lane == 0) a.segmass[(int64_t)b * a.nseg + seg] = sum;
+      if (take_places(in, &count, place))
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (in[i]) {
+            const Entry e = make_entry(key_of(x[j][i]), (int32_t)(seg * SEG + lane * 4 + i), 0);
+            if (place[i] < PASS_LIST) listed[place[i]] = e;
+            else put(atomicAdd(&a.state[b].listed, 1u), e);  // more than this workgroup lists
+          }
     }
   }
+  __syncthreads();
+  const int n = min(count, PASS_LIST);
+  __syncthreads();
+  if (threadIdx.x == 0 && n) count = (int)atomicAdd(&a.state[b].listed, (uint32_t)n);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += THREADS) put((uint32_t)(count + i), listed[i]);
 }
 
 // the threshold inside the listed bin, then the draw over whole-number masses
