@@ -9,15 +9,20 @@
 // of the sum of magnitudes on this card, the 4-bit and the bf16 ones 2^-24.)
 //
 // Layout.  The queries are the A operand (rows of the result), the table the B operand
-// (columns), so a lane holds one table row's scores for 16 queries.  A wave owns IT * 32
+// (columns), so a lane holds table rows' scores for 16 queries.  A wave owns IT * 32
 // consecutive table rows, lane l the rows IT * (l % 32) .. + IT - 1: its IT scores of a query are
 // neighbours and leave in one store, 32 lanes cover IT * 32 consecutive scores.
 // The sum over d may be taken in any order as long as both operands agree: in a chunk of
-// 2 * S blocks (S <= 4) the lower half of the wave takes blocks 0 .. S-1, the upper half S .. 2S-1,
-// so a lane reads 16 * S (fp4) contiguous bytes of its row and its S scales are neighbours.
-// The table goes from memory to registers, one chunk ahead of its use; nothing of it is
-// shared between waves.  The queries go through LDS, rows 16 bytes off a power of two
+// 2 * S blocks (S <= CS) the lower half of the wave takes blocks 0 .. S-1, the upper half S .. 2S-1,
+// so a lane reads 16 * S (fp4) or 32 * S (fp8) contiguous bytes of its row and its S scales are
+// neighbours.  The table goes from memory to registers, one chunk ahead of its use; nothing of
+// it is shared between waves.  The queries go through LDS, rows 16 bytes off a power of two
 // (the eight lanes of a 16-byte access phase then fall into distinct banks).
+//
+// Short rows (the queries' 32 QT rows fit in LDS whole): a workgroup stages its queries once and
+// walks the table; bound by memory, the scores' writes above all.  Long rows: one tile per
+// workgroup, the queries' next chunk on its way into the other half of LDS during the present
+// one's products.
 #include <hip/hip_fp16.h>
 
 #include "mx.h"
@@ -34,10 +39,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
 
 constexpr int WAVES = 4;      // waves per workgroup
-constexpr int IT = 2;         // table rows per lane
+constexpr int THREADS = WAVES * 64;
 
-// acc register r of a lane: query row (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) of the 32
-__device__ __forceinline__ int acc_row(int lane, int r) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
+// (acc register r of a lane: query row (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) of the 32)
 
 // one block (32 elements) of a table row
 template <int XB> struct Block;
@@ -66,9 +70,9 @@ __device__ __forceinline__ bf16x8 to_bf16(const Block<8>& b, int s, float f) {
 }
 
 // a lane's blocks of one chunk, for its IT rows, with their scale bytes
-template <int XB>
+template <int XB, int IT, int CS>
 struct Chunk {
-  Block<XB> b[IT][4];
+  Block<XB> b[IT][CS];
   uint32_t s[IT];  // byte j: block j's scale
 };
 
@@ -80,109 +84,156 @@ struct Args {
   void* out;
   int64_t ld, N;
   int B, D, nblk;
-  int out_type, pair;    // pair: every even column starts a 2-score store
-  int q_vec;             // bf16 queries: rows start on 16 bytes
-  int s_word;            // nblk % 4 == 0: four scales in one load
+  int vec;               // every lane's IT scores start on their own size
+  int q_align;           // bytes on which every 8th value of every bf16 query starts (at most 16)
+  int s_word;            // nblk % 4 == 0: scales in loads of four
   int qtiles, itiles;
 };
 
-// blocks half h of the wave takes from the chunk at block c0: [first, first + S)
-__device__ __forceinline__ int chunk_s(int nblk, int c0) { return min(4, (nblk - c0 + 1) >> 1); }
+// blocks half h of the wave takes from the chunk at block c0: [c0 + h S, c0 + h S + S)
+template <int CS>
+__device__ __forceinline__ int chunk_s(int nblk, int c0) { return min(CS, (nblk - c0 + 1) >> 1); }
 
-template <int XB>
-__device__ __forceinline__ void load_chunk(const Args& a, int64_t row0, int c0, int h, Chunk<XB>& ch) {
-  const int S = chunk_s(a.nblk, c0), first = c0 + h * S;
+template <int XB, int IT, int CS>
+__device__ __forceinline__ void load_chunk(const Args& a, int64_t row0, int c0, int h, Chunk<XB, IT, CS>& ch) {
+  const int S = chunk_s<CS>(a.nblk, c0), first = c0 + h * S;
 #pragma unroll
   for (int t = 0; t < IT; ++t) {
     const int64_t row = min(row0 + t, a.N - 1);  // rows past the end: loaded again, not stored
     const uint8_t* p = a.x + (row * a.nblk + first) * (MX_BLOCK * XB / 8);
     const uint8_t* sp = a.xs + row * a.nblk + first;
     uint32_t s = 0x7f7f7f7fu;  // a block that is not there: zeros times one
-    if (S == 4 && a.s_word) s = *(const uint32_t*)sp;  // nblk % 4 == 0: first + 4 <= nblk
+    const bool word = CS == 4 && S == 4 && a.s_word;
+    if (word) s = *(const uint32_t*)sp;  // nblk % 4 == 0: first + 4 <= nblk
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < CS; ++j) {
       Block<XB>& b = ch.b[t][j];
       b.v = make_uint4(0, 0, 0, 0);
       if constexpr (XB == 8) b.w = make_uint4(0, 0, 0, 0);
       if (j < S && first + j < a.nblk) {
         b.v = *(const uint4*)(p + j * (MX_BLOCK * XB / 8));
         if constexpr (XB == 8) b.w = *(const uint4*)(p + j * 32 + 16);
-        if (!(S == 4 && a.s_word)) s = (s & ~(255u << (8 * j))) | ((uint32_t)sp[j] << (8 * j));
+        if (!word) s = (s & ~(255u << (8 * j))) | ((uint32_t)sp[j] << (8 * j));
       }
     }
     ch.s[t] = s;
   }
 }
 
-// Stage queries [q0, q0 + 32 QT) x blocks [c0, c0 + nb) into LDS rows of `stride` bytes.
-// A bf16 block is 64 bytes, an E2M1 block 16 (its scale goes to qsl, one byte per block).
-template <bool Q4, int QT>
-__device__ __forceinline__ void stage_queries(const Args& a, int q0, int c0, int nb, uint8_t* ql, uint8_t* qsl,
-                                              int stride, int sstride) {
-  constexpr int CB = Q4 ? 1 : 4;  // 16-byte pieces per block
-  const int pieces = nb * CB;
-  for (int e = threadIdx.x; e < 32 * QT * pieces; e += WAVES * 64) {
-    const int r = e / pieces, c = e - r * pieces;
-    const int q = q0 + r, blk = c0 + c / CB;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (q < a.B && blk < a.nblk) {
-      if (Q4) {
-        v = *(const uint4*)((const uint8_t*)a.q + ((int64_t)q * a.nblk + blk) * 16);
-      } else {
-        const int d = blk * 32 + (c % CB) * 8;
-        const uint16_t* p = (const uint16_t*)a.q + (int64_t)q * a.D + d;
-        if (a.q_vec && d + 8 <= a.D) {
-          v = *(const uint4*)p;
-        } else {
-          uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (d + j < a.D) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-          v = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+// eight bf16 of a query from value d on; values >= D are zero
+__device__ __forceinline__ uint4 load_query8(const Args& a, int q, int d) {
+  const uint16_t* p = (const uint16_t*)a.q + (int64_t)q * a.D + d;
+  if (d + 8 <= a.D) {
+    if (a.q_align == 16) return *(const uint4*)p;
+    if (a.q_align == 8) {
+      const uint2 lo = *(const uint2*)p, hi = *(const uint2*)(p + 4);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
-    *(uint4*)(ql + r * stride + c * 16) = v;
-    if (Q4) qsl[r * sstride + c] = (q < a.B && blk < a.nblk) ? a.qs[(int64_t)q * a.nblk + blk] : 127;
+    if (a.q_align == 4) {
+      const uint32_t* w = (const uint32_t*)p;
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (d + j < a.D) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int T>
-__device__ __forceinline__ uint16_t to16(float f) {
-  return T == T_BF16 ? f32_to_bf16(f) : __half_as_ushort(__float2half_rn(f));
+// 16 bytes of a query: piece c of block blk (bf16: 4 pieces a block, E2M1: 1)
+template <bool Q4>
+__device__ __forceinline__ uint4 load_piece(const Args& a, int q, int blk, int c) {
+  if (q >= a.B || blk >= a.nblk) return make_uint4(0, 0, 0, 0);
+  if (Q4) return *(const uint4*)((const uint8_t*)a.q + ((int64_t)q * a.nblk + blk) * 16);
+  return load_query8(a, q, blk * 32 + c * 8);
+}
+__device__ __forceinline__ uint8_t load_qscale(const Args& a, int q, int blk) {
+  return q < a.B && blk < a.nblk ? a.qs[(int64_t)q * a.nblk + blk] : (uint8_t)127;
 }
 
+typedef __bf16 bf16_2 __attribute__((ext_vector_type(2)));
+typedef float f32_2 __attribute__((ext_vector_type(2)));
 template <int T>
-__device__ __forceinline__ void store_pair(const Args& a, int64_t at, int64_t row, float v0, float v1) {
-  if (row >= a.N) return;
-  const bool two = row + 1 < a.N;
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {  // round to nearest even
+  if (T == T_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32_2){lo, hi}, bf16_2));
+  return (uint32_t)__half_as_ushort(__float2half_rn(lo)) | (uint32_t)__half_as_ushort(__float2half_rn(hi)) << 16;
+}
+
+// IT neighbouring scores to o; `left` of them exist
+template <int T, int IT>
+__device__ __forceinline__ void store_scores(char* at, bool whole, int left, const float v[IT]) {
   if (T == T_F32) {
-    float* o = (float*)a.out + at;
-    if (two && a.pair) *(float2*)o = make_float2(v0, v1);
-    else { o[0] = v0; if (two) o[1] = v1; }
+    float* o = (float*)at;
+    if (whole) {
+      if constexpr (IT == 4) *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
+      else *(float2*)o = make_float2(v[0], v[1]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < IT; ++t)
+        if (t < left) o[t] = v[t];
+    }
   } else {
-    uint16_t* o = (uint16_t*)a.out + at;
-    const uint16_t x = to16<T>(v0), y = to16<T>(v1);
-    if (two && a.pair) *(uint32_t*)o = (uint32_t)x | ((uint32_t)y << 16);
-    else { o[0] = x; if (two) o[1] = y; }
+    uint16_t* o = (uint16_t*)at;
+    uint32_t w[IT / 2];
+#pragma unroll
+    for (int t = 0; t < IT / 2; ++t) w[t] = pack16<T>(v[2 * t], v[2 * t + 1]);
+    if (whole) {
+      if constexpr (IT == 4) *(uint2*)o = make_uint2(w[0], w[1]);
+      else *(uint32_t*)o = w[0];
+    } else {
+#pragma unroll
+      for (int t = 0; t < IT; ++t)
+        if (t < left) o[t] = (uint16_t)(w[t / 2] >> (16 * (t & 1)));
+    }
   }
 }
 
-// KC: blocks of the queries held in LDS at a time.
-template <int XB, bool Q4, int QT, int KC, int T>
-__global__ void __launch_bounds__(256) mx_score_kernel(Args a) {
-  constexpr int QBYTES = Q4 ? 16 : 64;
-  constexpr int STRIDE = KC * QBYTES + 16, SSTRIDE = KC + 4;
+// LB: blocks of a query held in LDS
+template <int XB, bool Q4, int QT, int IT, int CS, int LB, int T>
+__global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
+  constexpr int QBYTES = Q4 ? 16 : 64, CB = QBYTES / 16;
+  constexpr int STRIDE = LB * QBYTES + 16, SSTRIDE = LB + 4;
+  constexpr int KC = 2 * CS;  // blocks per chunk
+  constexpr int QREGS = 32 * QT * KC * CB / THREADS > 0 ? 32 * QT * KC * CB / THREADS : 1;
+  static_assert(CS == 1 || LB >= 2 * KC, "two chunks of queries");
   __shared__ __attribute__((aligned(16))) uint8_t ql[32 * QT * STRIDE];
   __shared__ __attribute__((aligned(16))) uint8_t qsl[Q4 ? 32 * QT * SSTRIDE : 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const bool once = a.nblk <= KC;  // the queries fit: staged once for all tiles of this workgroup
-  const int total = a.qtiles * a.itiles;
-  int staged = -1;
-  for (int w = blockIdx.x; w < total; w += gridDim.x) {
-    const int tile = xcd_remap(w, total);  // query tiles of one table panel are neighbours on one XCD
-    const int q0 = (tile % a.qtiles) * 32 * QT;
-    const int64_t row0 = (int64_t)(tile / a.qtiles) * (WAVES * 32 * IT) + wave * (32 * IT) + (lane & 31) * IT;
+  const bool once = CS == 1 || a.nblk <= LB;
+  // once: one query tile, every stride-th table tile (the workgroups of one table tile are on one XCD);
+  // else one tile
+  int qt, it, step;
+  if (once) {
+    const int u = blockIdx.x >> 3;
+    qt = u % a.qtiles;
+    it = (u / a.qtiles) * 8 + (blockIdx.x & 7);
+    step = gridDim.x / a.qtiles;
+  } else {
+    const int tile = xcd_remap(blockIdx.x, a.qtiles * a.itiles);
+    qt = tile % a.qtiles;
+    it = tile / a.qtiles;
+    step = a.itiles;
+  }
+  if (it >= a.itiles) return;
+  const int q0 = qt * 32 * QT;
+  {  // all of the queries, or their first chunk
+    const int nb = once ? (a.nblk + KC - 1) / KC * KC : KC, pieces = min(nb, LB) * CB;
+    for (int e = threadIdx.x; e < 32 * QT * pieces; e += THREADS) {
+      const int r = e / pieces, c = e - r * pieces;
+      *(uint4*)(ql + r * STRIDE + c * 16) = load_piece<Q4>(a, q0 + r, c / CB, c % CB);
+      if (Q4) qsl[r * SSTRIDE + c] = load_qscale(a, q0 + r, c);
+    }
+    __syncthreads();
+  }
+  const uint8_t* qrow = ql + (lane & 31) * STRIDE;
+  const uint8_t* qsrow = qsl + (lane & 31) * SSTRIDE;
+  const auto row_of_tile = [&](int i) { return (int64_t)i * (WAVES * 32 * IT) + wave * (32 * IT) + (lane & 31) * IT; };
+  Chunk<XB, IT, CS> cur, nxt;
+  load_chunk<XB, IT, CS>(a, row_of_tile(it), 0, h, cur);
+  int half = 0;  // not once: the half of LDS that holds the present chunk's queries
+  for (; it < a.itiles; it += step) {
+    const int64_t row0 = row_of_tile(it);
     f32x16 acc[IT][QT];
 #pragma unroll
     for (int t = 0; t < IT; ++t)
@@ -190,86 +241,117 @@ __global__ void __launch_bounds__(256) mx_score_kernel(Args a) {
       for (int q = 0; q < QT; ++q)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][q][r] = 0.f;
-    Chunk<XB> cur, nxt;
-    load_chunk<XB>(a, row0, 0, h, cur);
-    for (int k0 = 0; k0 < a.nblk; k0 += KC) {
-      const int kn = min(KC, a.nblk - k0);
-      if (!once || staged != q0) {
-        __syncthreads();
-        stage_queries<Q4, QT>(a, q0, k0, (kn + 7) / 8 * 8, ql, qsl, STRIDE, SSTRIDE);
-        __syncthreads();
-        staged = q0;
-      }
-      for (int c0 = k0; c0 < k0 + kn; c0 += 8) {
-        if (c0 + 8 < a.nblk) load_chunk<XB>(a, row0, c0 + 8, h, nxt);
-        const int S = chunk_s(a.nblk, c0), first = c0 - k0 + h * S;
+    for (int c0 = 0; c0 < a.nblk; c0 += KC) {
+      const bool more = c0 + KC < a.nblk;
+      if (more) load_chunk<XB, IT, CS>(a, row0, c0 + KC, h, nxt);
+      else if (it + step < a.itiles) load_chunk<XB, IT, CS>(a, row_of_tile(it + step), 0, h, nxt);
+      uint4 qn[QREGS];
+      uint8_t qsn[QREGS];
+      if (CS > 1 && !once && more) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j < S) {
-            if constexpr (Q4) {
-              i32x8 qa[QT];
-              int qsc[QT];
+        for (int i = 0; i < QREGS; ++i) {
+          const int e = threadIdx.x + i * THREADS, r = e / (KC * CB), c = e % (KC * CB);
+          qn[i] = load_piece<Q4>(a, q0 + r, c0 + KC + c / CB, c % CB);
+          if (Q4) qsn[i] = load_qscale(a, q0 + r, c0 + KC + c);
+        }
+      }
+      const int S = chunk_s<CS>(a.nblk, c0), first = (once ? c0 : half * KC) + h * S;
+#pragma unroll
+      for (int j = 0; j < CS; ++j) {
+        if (j < S) {
+          if constexpr (Q4) {
+            i32x8 qa[QT];
+            int qsc[QT];
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+              const uint4 v = *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 16);
+              qa[q] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+              qsc[q] = qsrow[q * 32 * SSTRIDE + first + j];
+            }
+#pragma unroll
+            for (int t = 0; t < IT; ++t) {
+              const uint4 v = cur.b[t][j].v;
+              const i32x8 xb = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+#pragma unroll
+              for (int q = 0; q < QT; ++q)
+                acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
+                                                                            (int)(cur.s[t] >> (8 * j)));
+            }
+          } else {
+            float f[IT];
+#pragma unroll
+            for (int t = 0; t < IT; ++t) {
+              const uint32_t s = (cur.s[t] >> (8 * j)) & 255u;
+              f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              bf16x8 xb[IT];
+#pragma unroll
+              for (int t = 0; t < IT; ++t) xb[t] = to_bf16(cur.b[t][j], s, f[t]);
 #pragma unroll
               for (int q = 0; q < QT; ++q) {
-                const uint4 v = *(const uint4*)(ql + (q * 32 + (lane & 31)) * STRIDE + (first + j) * 16);
-                qa[q] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-                qsc[q] = qsl[(q * 32 + (lane & 31)) * SSTRIDE + first + j];
-              }
+                const bf16x8 qa = __builtin_bit_cast(bf16x8, *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 64 + s * 16));
 #pragma unroll
-              for (int t = 0; t < IT; ++t) {
-                const uint4 v = cur.b[t][j].v;
-                const i32x8 xb = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-#pragma unroll
-                for (int q = 0; q < QT; ++q)
-                  acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
-                                                                              (int)(cur.s[t] >> (8 * j)));
-              }
-            } else {
-              float f[IT];
-#pragma unroll
-              for (int t = 0; t < IT; ++t) {
-                const uint32_t s = (cur.s[t] >> (8 * j)) & 255u;
-                f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
-              }
-#pragma unroll
-              for (int s = 0; s < 4; ++s) {
-                bf16x8 xb[IT];
-#pragma unroll
-                for (int t = 0; t < IT; ++t) xb[t] = to_bf16(cur.b[t][j], s, f[t]);
-#pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                  const uint4 v = *(const uint4*)(ql + (q * 32 + (lane & 31)) * STRIDE + (first + j) * 64 + s * 16);
-                  const bf16x8 qa = __builtin_bit_cast(bf16x8, v);
-#pragma unroll
-                  for (int t = 0; t < IT; ++t)
-                    acc[t][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, xb[t], acc[t][q], 0, 0, 0);
-                }
+                for (int t = 0; t < IT; ++t) acc[t][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, xb[t], acc[t][q], 0, 0, 0);
               }
             }
           }
         }
-        cur = nxt;
       }
+      if (CS > 1 && !once && more) {
+#pragma unroll
+        for (int i = 0; i < QREGS; ++i) {
+          const int e = threadIdx.x + i * THREADS, r = e / (KC * CB), c = e % (KC * CB);
+          *(uint4*)(ql + r * STRIDE + (half ^ 1) * (KC * QBYTES) + c * 16) = qn[i];
+          if (Q4) qsl[r * SSTRIDE + (half ^ 1) * KC + c] = qsn[i];
+        }
+        half ^= 1;
+        __syncthreads();
+      }
+      cur = nxt;
     }
+    // (one pointer, moved from row to row: kept per row, the addresses would fill the registers)
+    constexpr int ES = T == T_F32 ? 4 : 2;
+    const int left = (int)min(a.N - row0, (int64_t)IT), rows = a.B - q0 - 4 * h;
+    const bool whole = a.vec && left == IT;
+    char* o = (char*)a.out + ((int64_t)(q0 + 4 * h) * a.ld + row0) * ES;
+    const int64_t down = a.ld * ES;
+    if (left > 0) {
 #pragma unroll
-    for (int q = 0; q < QT; ++q)
+      for (int q = 0; q < QT; ++q)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int b = q0 + q * 32 + acc_row(lane, r);
-        if (b < a.B) store_pair<T>(a, (int64_t)b * a.ld + row0, row0, acc[0][q][r], acc[1][q][r]);
-      }
+        for (int r = 0; r < 16; ++r) {
+          float v[IT];
+#pragma unroll
+          for (int t = 0; t < IT; ++t) v[t] = acc[t][q][r];
+          if (q * 32 + (r & 3) + 8 * (r >> 2) < rows) store_scores<T, IT>(o, whole, left, v);
+          o += (r & 3) == 3 ? 5 * down : down;
+        }
+    }
   }
 }
 
-template <int XB, bool Q4, int QT, int KC>
-void launch(Args& a, hipStream_t st) {
+template <int XB, bool Q4, int QT, int IT, int CS, int LB, int T>
+void launch_as(Args& a, hipStream_t st) {
+  const int es = T == T_F32 ? 4 : 2;
+  a.vec = (a.B == 1 || a.ld % IT == 0) && ((uintptr_t)a.out & (IT * es - 1)) == 0;
   a.qtiles = (a.B + 32 * QT - 1) / (32 * QT);
   a.itiles = (int)((a.N + WAVES * 32 * IT - 1) / (WAVES * 32 * IT));
-  const int64_t total = (int64_t)a.qtiles * a.itiles;
-  const int grid = (int)(total < 2048 ? total : 2048);
-  if (a.out_type == T_F32) hipLaunchKernelGGL((mx_score_kernel<XB, Q4, QT, KC, T_F32>), dim3(grid), dim3(256), 0, st, a);
-  else if (a.out_type == T_BF16) hipLaunchKernelGGL((mx_score_kernel<XB, Q4, QT, KC, T_BF16>), dim3(grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((mx_score_kernel<XB, Q4, QT, KC, T_F16>), dim3(grid), dim3(256), 0, st, a);
+  int64_t grid = (int64_t)a.qtiles * a.itiles;
+  if (CS == 1 || a.nblk <= LB) {
+    // about four workgroups a CU, a multiple of 8 per query tile
+    const int64_t per = max((int64_t)1, min(((int64_t)a.itiles + 7) / 8, (int64_t)1024 / (8 * a.qtiles)));
+    grid = per * 8 * a.qtiles;
+  }
+  hipLaunchKernelGGL((mx_score_kernel<XB, Q4, QT, IT, CS, LB, T>), dim3((unsigned)grid), dim3(THREADS), 0, st, a);
+}
+
+template <int XB, bool Q4, int QT, int IT, int CS, int LB>
+void launch(Args& a, int type, hipStream_t st) {
+  if (type == T_F32) launch_as<XB, Q4, QT, IT, CS, LB, T_F32>(a, st);
+  else if (type == T_BF16) launch_as<XB, Q4, QT, IT, CS, LB, T_BF16>(a, st);
+  else launch_as<XB, Q4, QT, IT, CS, LB, T_F16>(a, st);
 }
 
 }  // namespace
@@ -281,24 +363,26 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
   if (B <= 0 || N <= 0) return 0;
   if (D <= 0 || (xbits != 4 && xbits != 8) || (qs && xbits != 4) || ld < N || out_type < 0 || out_type > 2)
     return (int)hipErrorInvalidValue;
+  if (N > (int64_t)INT32_MAX * 32 || (int64_t)((B + 31) / 32) * ((N + 255) / 256) > INT32_MAX)
+    return (int)hipErrorInvalidValue;
   Args a;
   a.q = q; a.qs = (const uint8_t*)qs; a.x = (const uint8_t*)x; a.xs = (const uint8_t*)xs;
   a.out = out; a.ld = ld; a.N = N; a.B = B; a.D = D;
   a.nblk = (D + MX_BLOCK - 1) / MX_BLOCK;
-  a.out_type = out_type;
-  a.pair = ld % 2 == 0 && ((uintptr_t)out & (out_type == T_F32 ? 7 : 3)) == 0;
-  a.q_vec = D % 8 == 0 && ((uintptr_t)q & 15) == 0;
+  const uintptr_t qp = (uintptr_t)q | (uintptr_t)(2 * D);  // D even, a multiple of 4, of 8
+  a.q_align = qp & 2 ? 2 : qp & 4 ? 4 : qp & 8 ? 8 : 16;
   a.s_word = a.nblk % 4 == 0 && ((uintptr_t)xs & 3) == 0;
-  if (N > (int64_t)INT32_MAX * 32 || (int64_t)((B + 31) / 32) * ((N + 255) / 256) > INT32_MAX)
-    return (int)hipErrorInvalidValue;
   hipStream_t st = (hipStream_t)stream;
-  const bool few = B <= 32;
+  const bool few = B <= 32, narrow = a.nblk <= 2;
   if (qs) {
-    if (few) launch<4, true, 1, 32>(a, st); else launch<4, true, 4, 16>(a, st);
+    if (narrow) { if (few) launch<4, true, 1, 4, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
+    else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 4, 2, 4, 16>(a, out_type, st); }
   } else if (xbits == 4) {
-    if (few) launch<4, false, 1, 16>(a, st); else launch<4, false, 4, 8>(a, st);
+    if (narrow) { if (few) launch<4, false, 1, 4, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
+    else { if (few) launch<4, false, 1, 2, 4, 32>(a, out_type, st); else launch<4, false, 2, 2, 4, 16>(a, out_type, st); }
   } else {
-    if (few) launch<8, false, 1, 16>(a, st); else launch<8, false, 4, 8>(a, st);
+    if (narrow) { if (few) launch<8, false, 1, 4, 1, 2>(a, out_type, st); else launch<8, false, 2, 4, 1, 2>(a, out_type, st); }
+    else { if (few) launch<8, false, 1, 2, 2, 32>(a, out_type, st); else launch<8, false, 2, 2, 2, 16>(a, out_type, st); }
   }
   FPS_CHECK_LAUNCH();
   return 0;
