@@ -354,6 +354,148 @@ void launch(Args& a, int type, hipStream_t st) {
   else launch_as<XB, Q4, QT, IT, CS, LB, T_F16>(a, st);
 }
 
+// Both sides in 4 bits, many queries, long rows: bound by the matrix instructions, so both operands
+// go through LDS (a table row is used by two waves, a query by four) and the loads are whole cache
+// lines.  A workgroup of 8 waves owns 256 queries x 256 table rows, a wave 128 x 64.  A chunk is 256
+// values of every row, 8 pieces of 16 bytes: the next chunk moves from memory to the other LDS
+// buffer, past the registers, during the present one's products.  Piece p of row r lies in slot
+// p ^ (r' & 7) of its 128 bytes (r' = r for queries; r / 2 for table rows, of which a lane takes
+// two neighbours), so the lanes of an access phase, 8 rows of one piece, fall into distinct banks.
+// Blocks past the row's end are loaded as some block that is there and given the scale 2^-127 on
+// both sides: their products vanish below fp32's range.
+typedef __attribute__((address_space(1))) void GlobalVoid;
+typedef __attribute__((address_space(3))) void LdsVoid;
+// 16 bytes a lane from base + off to LDS, lane after lane from `to` on
+__device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const GlobalVoid*)(base + off), (LdsVoid*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+constexpr int WT = 256;   // queries and table rows per workgroup
+constexpr int WTHREADS = 512;
+constexpr int WCHUNK = 8; // blocks per chunk
+
+struct WideLds {
+  uint8_t data[2][2][WT * 128];     // buffer, operand (0: queries)
+  uint32_t scale[2][2][2][WT];      // buffer, operand, half of the chunk
+};
+
+template <int T>
+__global__ void __launch_bounds__(WTHREADS, 2) mx_score_wide_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) WideLds lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l = lane & 31;
+  const int tile = xcd_remap(blockIdx.x, a.qtiles * a.itiles);
+  const int q0 = tile % a.qtiles * WT;
+  const int64_t i0 = (int64_t)(tile / a.qtiles) * WT;
+  const int wq = (wave & 1) * 128, wi = (wave >> 1) * 64;
+  // This wave brings in 8 x 8 rows, 4 x 8 of each operand: a lane moves 16 bytes straight to LDS, eight
+  // lanes one row's 128; slot i of a row gets the piece that the rule above puts there.
+  const uint32_t row_bytes = (uint32_t)a.nblk * 16;
+  const uint8_t* qbase = (const uint8_t*)a.q + (int64_t)q0 * row_bytes;
+  const uint8_t* xbase = a.x + i0 * row_bytes;
+  const int qlast = min(a.B - q0, WT) - 1, xlast = (int)min(a.N - i0, (int64_t)WT) - 1;  // rows past the end: the last again
+  const int srow = tid & (WT - 1), sop = tid >> 8;
+  const uint8_t* ssrc = sop ? a.xs + (i0 + min(srow, xlast)) * a.nblk : a.qs + (int64_t)(q0 + min(srow, qlast)) * a.nblk;
+  uint32_t sin0 = 0, sin1 = 0;
+  const auto load = [&](int c0, int buf) {
+    const int there = c0 + WCHUNK <= a.nblk ? 7 : 3;  // nblk % 4 == 0: the last chunk may hold half
+    const uint32_t at = c0 * 16;
+    uint8_t* to = lds.data[buf][0] + wave * 4096;
+    const int i = lane & 7;
+    int r = lane >> 3;  // row & 7 == r, (row >> 1) & 7 == (r >> 1) + 4 (k & 1)
+    asm("" : "+v"(r));  // the offsets are computed here: kept over the loop they would not fit the registers
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = (wave * 4 + k) * 8 + r;
+      load_to_lds(qbase, min(row, qlast) * row_bytes + at + ((i ^ r) & there) * 16, to + k * 1024);
+      load_to_lds(xbase, min(row, xlast) * row_bytes + at + ((i ^ ((r >> 1) + 4 * (k & 1))) & there) * 16,
+                  to + WT * 128 + k * 1024);
+    }
+    sin0 = *(const uint32_t*)(ssrc + c0);
+    sin1 = c0 + 4 < a.nblk ? *(const uint32_t*)(ssrc + c0 + 4) : 0u;
+  };
+  const auto put_scales = [&](int buf) {
+    lds.scale[buf][sop][0][srow] = sin0;
+    lds.scale[buf][sop][1][srow] = sin1;
+  };
+  f32x16 acc[2][4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][q][r] = 0.f;
+  load(0, 0);
+  put_scales(0);
+  wait_loads();
+  __syncthreads();
+  int buf = 0;
+  for (int c0 = 0; c0 < a.nblk; c0 += WCHUNK) {
+    const bool more = c0 + WCHUNK < a.nblk;
+    const uint8_t* qd = lds.data[buf][0] + (wq + l) * 128;
+    const uint8_t* xd = lds.data[buf][1] + (wi + 2 * l) * 128;
+    // The whole chunk comes into registers before the next one's loads are issued: the compiler does not tell
+    // the buffers apart and waits for such loads before any later read of LDS.
+    uint4 qa[4][4], xb[4][2];
+    uint32_t qsc[4], xsc[2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) qsc[q] = lds.scale[buf][0][h][wq + 32 * q + l];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) xsc[t] = lds.scale[buf][1][h][wi + 2 * l + t];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = ((h * 4 + j) ^ (l & 7)) * 16;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) qa[j][q] = *(const uint4*)(qd + q * 32 * 128 + at);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) xb[j][t] = *(const uint4*)(xd + t * 128 + at);
+    }
+    if (more) load(c0 + WCHUNK, buf ^ 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint4 u = qa[j][q], v = xb[j][t];
+          acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+              i32x8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, 0, 0, 0, 0}, i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0},
+              acc[t][q], 4, 4, 0, (int)(qsc[q] >> (8 * j)), 0, (int)(xsc[t] >> (8 * j)));
+        }
+    __builtin_amdgcn_sched_barrier(0);  // the products are not moved behind the wait
+    put_scales(buf ^ 1);  // (after the last chunk: not read)
+    wait_loads();
+    __syncthreads();
+    buf ^= 1;
+  }
+  constexpr int ES = T == T_F32 ? 4 : 2;
+  const int64_t row0 = i0 + wi + 2 * l;
+  const int left = (int)min(a.N - row0, (int64_t)2), rows = a.B - q0 - wq - 4 * h;
+  const bool whole = a.vec && left == 2;
+  char* o = (char*)a.out + ((int64_t)(q0 + wq + 4 * h) * a.ld + row0) * ES;
+  const int64_t down = a.ld * ES;
+  if (left > 0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float v[2] = {acc[0][q][r], acc[1][q][r]};
+        if (q * 32 + (r & 3) + 8 * (r >> 2) < rows) store_scores<T, 2>(o, whole, left, v);
+        o += (r & 3) == 3 ? 5 * down : down;
+      }
+  }
+}
+
+void launch_wide(Args& a, int type, hipStream_t st) {
+  a.vec = (a.B == 1 || a.ld % 2 == 0) && ((uintptr_t)a.out & (type == T_F32 ? 7 : 3)) == 0;
+  a.qtiles = (a.B + WT - 1) / WT;
+  a.itiles = (int)((a.N + WT - 1) / WT);
+  const dim3 grid((unsigned)(a.qtiles * a.itiles));
+  if (type == T_F32) hipLaunchKernelGGL((mx_score_wide_kernel<T_F32>), grid, dim3(WTHREADS), 0, st, a);
+  else if (type == T_BF16) hipLaunchKernelGGL((mx_score_wide_kernel<T_BF16>), grid, dim3(WTHREADS), 0, st, a);
+  else hipLaunchKernelGGL((mx_score_wide_kernel<T_F16>), grid, dim3(WTHREADS), 0, st, a);
+}
+
 }  // namespace
 
 // out [B, N] (row stride ld, type 0 fp32 / 1 bf16 / 2 fp16) = q . x^T.  qs == nullptr: q is bf16
@@ -376,7 +518,8 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
   const bool few = B <= 32, narrow = a.nblk <= 2;
   if (qs) {
     if (narrow) { if (few) launch<4, true, 1, 4, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
-    else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 4, 2, 4, 16>(a, out_type, st); }
+    else if (a.B > 64 && a.nblk > 16 && a.s_word) launch_wide(a, out_type, st);
+    else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 4, 2, 2, 16>(a, out_type, st); }
   } else if (xbits == 4) {
     if (narrow) { if (few) launch<4, false, 1, 4, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
     else { if (few) launch<4, false, 1, 2, 4, 32>(a, out_type, st); else launch<4, false, 2, 2, 4, 16>(a, out_type, st); }
