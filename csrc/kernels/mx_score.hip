@@ -363,11 +363,13 @@ void launch(Args& a, int type, hipStream_t st) {
 // two neighbours), so the lanes of an access phase, 8 rows of one piece, fall into distinct banks.
 // Blocks past the row's end are loaded as some block that is there and given the scale 2^-127 on
 // both sides: their products vanish below fp32's range.
-typedef __attribute__((address_space(1))) void GlobalVoid;
-typedef __attribute__((address_space(3))) void LdsVoid;
-// 16 bytes a lane from base + off to LDS, lane after lane from `to` on
-__device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint8_t* to) {
-  __builtin_amdgcn_global_load_lds((const GlobalVoid*)(base + off), (LdsVoid*)to, 16, 0, 0);
+typedef __attribute__((address_space(3))) uint8_t LdsByte;
+// 16 bytes a lane from base + off to LDS, lane after lane from byte `to` on.  In assembly because the
+// compiler waits for every such load of its own before the next read of LDS, whichever buffer that
+// is of; here wait_loads() does, before the barrier that hands the buffer over.  (m0, the
+// destination, is not in use by anything else in this kernel; nothing is returned in registers.)
+__device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -394,13 +396,14 @@ __global__ void __launch_bounds__(WTHREADS, 2) mx_score_wide_kernel(Args a) {
   const uint8_t* qbase = (const uint8_t*)a.q + (int64_t)q0 * row_bytes;
   const uint8_t* xbase = a.x + i0 * row_bytes;
   const int qlast = min(a.B - q0, WT) - 1, xlast = (int)min(a.N - i0, (int64_t)WT) - 1;  // rows past the end: the last again
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(LdsByte*)lds.data[0][0] + wave * 4096);
   const int srow = tid & (WT - 1), sop = tid >> 8;
   const uint8_t* ssrc = sop ? a.xs + (i0 + min(srow, xlast)) * a.nblk : a.qs + (int64_t)(q0 + min(srow, qlast)) * a.nblk;
   uint32_t sin0 = 0, sin1 = 0;
   const auto load = [&](int c0, int buf) {
     const int there = c0 + WCHUNK <= a.nblk ? 7 : 3;  // nblk % 4 == 0: the last chunk may hold half
     const uint32_t at = c0 * 16;
-    uint8_t* to = lds.data[buf][0] + wave * 4096;
+    const uint32_t to = lds0 + buf * (2 * WT * 128);
     const int i = lane & 7;
     int r = lane >> 3;  // row & 7 == r, (row >> 1) & 7 == (r >> 1) + 4 (k & 1)
     asm("" : "+v"(r));  // the offsets are computed here: kept over the loop they would not fit the registers
@@ -434,35 +437,37 @@ __global__ void __launch_bounds__(WTHREADS, 2) mx_score_wide_kernel(Args a) {
     const bool more = c0 + WCHUNK < a.nblk;
     const uint8_t* qd = lds.data[buf][0] + (wq + l) * 128;
     const uint8_t* xd = lds.data[buf][1] + (wi + 2 * l) * 128;
-    // The whole chunk comes into registers before the next one's loads are issued: the compiler does not tell
-    // the buffers apart and waits for such loads before any later read of LDS.
-    uint4 qa[4][4], xb[4][2];
+    if (more) load(c0 + WCHUNK, buf ^ 1);
     uint32_t qsc[4], xsc[2];
 #pragma unroll
     for (int q = 0; q < 4; ++q) qsc[q] = lds.scale[buf][0][h][wq + 32 * q + l];
 #pragma unroll
     for (int t = 0; t < 2; ++t) xsc[t] = lds.scale[buf][1][h][wi + 2 * l + t];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    // step j's operands are read during step j - 1's products
+    uint4 qa[2][4], xb[2][2];
+    const auto read = [&](int j) {
       const int at = ((h * 4 + j) ^ (l & 7)) * 16;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) qa[j][q] = *(const uint4*)(qd + q * 32 * 128 + at);
+      for (int q = 0; q < 4; ++q) qa[j & 1][q] = *(const uint4*)(qd + q * 32 * 128 + at);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) xb[j][t] = *(const uint4*)(xd + t * 128 + at);
-    }
-    if (more) load(c0 + WCHUNK, buf ^ 1);
+      for (int t = 0; t < 2; ++t) xb[j & 1][t] = *(const uint4*)(xd + t * 128 + at);
+    };
+    read(0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
+      if (j < 3) read(j + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint4 u = qa[j][q], v = xb[j][t];
+          const uint4 u = qa[j & 1][q], v = xb[j & 1][t];
           acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
               i32x8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, 0, 0, 0, 0}, i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0},
               acc[t][q], 4, 4, 0, (int)(qsc[q] >> (8 * j)), 0, (int)(xsc[t] >> (8 * j)));
         }
-    __builtin_amdgcn_sched_barrier(0);  // the products are not moved behind the wait
+      __builtin_amdgcn_sched_barrier(0);  // (also: the products are not moved behind the wait)
+    }
     put_scales(buf ^ 1);  // (after the last chunk: not read)
     wait_loads();
     __syncthreads();
