@@ -71,8 +71,6 @@ class MXTable:
     def _set(self, data, scale, dim, fmt):
         self.data, self.scale, self.dim, self.fmt = data, scale, int(dim), fmt
         self.bits = MX_FORMATS[fmt]
-        #: per-slot claim of an indexed write (-1 between writes), allocated by the first one
-        self._owner: Optional[torch.Tensor] = None
 
     @classmethod
     def wrap(cls, data: torch.Tensor, scale: torch.Tensor, dim: int, fmt: str = "fp4") -> "MXTable":
@@ -141,8 +139,7 @@ def mx_set_rows(table: MXTable, idx: Optional[torch.Tensor], rows: torch.Tensor)
     padding slot and skipped (as ``idx < 0`` of ``apply_rows``; ``FPS_DEBUG=1`` raises for one past
     the table); where an index repeats, the last of its rows is stored whole.  Slots that no row
     names stay as they were.  Calls on one table from several streams must not name the same slot.
-    The first indexed write of a table (of more than one row) allocates 4 bytes per slot, waits
-    for its stream once and cannot be captured into a graph; later ones can."""
+    An indexed write of more than one row takes a workspace of 4 bytes per slot."""
     if rows.dim() != 2 or rows.shape[1] != table.dim or rows.dtype not in _TYPE:
         raise ValueError(f"mx_set_rows: rows must be fp32 / bf16 / fp16 [n, {table.dim}], got {rows.dtype} "
                          f"{tuple(rows.shape)}")
@@ -161,17 +158,13 @@ def mx_set_rows(table: MXTable, idx: Optional[torch.Tensor], rows: torch.Tensor)
         R.mx_set_rows(table.data, table.scale, table.bits, idx, rows)
         return table
     with _device_of(rows):
-        if idx is not None and n > 1 and table._owner is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("mx_set_rows: a table's first indexed write allocates its claims: run it once "
-                                   "before capturing")
-            table._owner = torch.full((table.rows,), -1, dtype=torch.int32, device=table.device)
-            torch.cuda.current_stream().synchronize()  # once: writes from any stream find it filled
+        owner = None
+        if idx is not None and n > 1:  # which row a slot's repeated index leaves there
+            owner = torch.empty(table.rows, dtype=torch.int32, device=table.device)
         N.check(N.require().fps_mx_set_rows(rows.data_ptr(), _TYPE[rows.dtype], N.ptr(idx),
                                             int(idx is not None and idx.dtype == torch.int64), n, table.dim, table.rows,
                                             table.data.data_ptr(), table.scale.data_ptr(), table.bits,
-                                            N.ptr(table._owner) if idx is not None else None,
-                                            N.stream_ptr(rows.device)), "mx_set_rows")
+                                            N.ptr(owner), N.stream_ptr(rows.device)), "mx_set_rows")
     return table
 
 
