@@ -19,7 +19,7 @@ written from rows that the update kernels already produced.
 """
 from __future__ import annotations
 
-import contextlib
+import sys
 from typing import Optional
 
 import torch
@@ -33,17 +33,25 @@ MX_FORMATS = {"fp4": 4, "fp8": 8}
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _device_of(t: torch.Tensor):
-    """Context that makes ``t``'s GPU the current one (kernels launch on the current device)."""
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
-        return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
+_pkg = sys.modules[__package__]  # (for the debug switch; an import inside the calls costs a microsecond)
 
 
-def _same_device(what: str, *ts) -> None:
-    for t in ts[1:]:
-        if t is not None and t.device != ts[0].device:
-            raise ValueError(f"{what}: operands on {ts[0].device} and {t.device}")
+def _launch(what: str, device: int, *args) -> None:
+    """``fps_<what>(*args, stream)`` on the current stream of GPU ``device``, made current for the launch."""
+    fn = getattr(N.require(), "fps_" + what)
+    if device == torch.cuda.current_device():
+        rc = fn(*args, N.stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, N.stream_ptr())
+    N.check(rc, what)
+
+
+def _same_device(what: str, a: torch.Tensor, *ts) -> None:
+    d = a.get_device()  # -1: the CPU
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"{what}: operands on {a.device} and {t.device}")
 
 
 class MXTable:
@@ -71,6 +79,7 @@ class MXTable:
     def _set(self, data, scale, dim, fmt):
         self.data, self.scale, self.dim, self.fmt = data, scale, int(dim), fmt
         self.bits = MX_FORMATS[fmt]
+        self.rows = data.shape[0]
 
     @classmethod
     def wrap(cls, data: torch.Tensor, scale: torch.Tensor, dim: int, fmt: str = "fp4") -> "MXTable":
@@ -105,10 +114,6 @@ class MXTable:
         return mx_set_rows(t, None, rows)
 
     @property
-    def rows(self) -> int:
-        return self.data.shape[0]
-
-    @property
     def device(self) -> torch.device:
         return self.data.device
 
@@ -122,13 +127,11 @@ class MXTable:
 
 
 def _index(what: str, table: MXTable, idx: torch.Tensor) -> torch.Tensor:
-    from . import DEBUG, check_index
-
     if idx.dtype not in (torch.int32, torch.int64) or idx.dim() != 1 or not idx.is_contiguous():
         raise ValueError(f"{what}: idx must be a contiguous 1-d int32 or int64 tensor")
     _same_device(what, table.data, idx)
-    if DEBUG:
-        check_index(idx, table.rows, what, allow_negative=True)
+    if _pkg.DEBUG:
+        _pkg.check_index(idx, table.rows, what, allow_negative=True)
     return idx
 
 
@@ -157,14 +160,12 @@ def mx_set_rows(table: MXTable, idx: Optional[torch.Tensor], rows: torch.Tensor)
     if not rows.is_cuda:
         R.mx_set_rows(table.data, table.scale, table.bits, idx, rows)
         return table
-    with _device_of(rows):
-        owner = None
-        if idx is not None and n > 1:  # which row a slot's repeated index leaves there
-            owner = torch.empty(table.rows, dtype=torch.int32, device=table.device)
-        N.check(N.require().fps_mx_set_rows(rows.data_ptr(), _TYPE[rows.dtype], N.ptr(idx),
-                                            int(idx is not None and idx.dtype == torch.int64), n, table.dim, table.rows,
-                                            table.data.data_ptr(), table.scale.data_ptr(), table.bits,
-                                            N.ptr(owner), N.stream_ptr(rows.device)), "mx_set_rows")
+    owner = None
+    if idx is not None and n > 1:  # which of a repeated index's rows its slot gets
+        owner = torch.empty(table.rows, dtype=torch.int32, device=table.device)
+    _launch("mx_set_rows", rows.get_device(), rows.data_ptr(), _TYPE[rows.dtype], N.ptr(idx),
+            int(idx is not None and idx.dtype == torch.int64), n, table.dim, table.rows, table.data.data_ptr(),
+            table.scale.data_ptr(), table.bits, N.ptr(owner))
     return table
 
 
@@ -188,11 +189,8 @@ def mx_gather_rows(table: MXTable, idx: Optional[torch.Tensor] = None, out: Opti
     if not out.is_cuda:
         out.copy_(R.mx_gather_rows(table.data, table.scale, table.bits, table.dim, idx))
         return out
-    with _device_of(out):
-        N.check(N.require().fps_mx_gather_rows(table.data.data_ptr(), table.scale.data_ptr(), table.rows, table.dim,
-                                               table.bits, N.ptr(idx),
-                                               int(idx is not None and idx.dtype == torch.int64), n, out.data_ptr(),
-                                               _TYPE[out.dtype], N.stream_ptr(out.device)), "mx_gather_rows")
+    _launch("mx_gather_rows", out.get_device(), table.data.data_ptr(), table.scale.data_ptr(), table.rows, table.dim,
+            table.bits, N.ptr(idx), int(idx is not None and idx.dtype == torch.int64), n, out.data_ptr(), _TYPE[out.dtype])
     return out
 
 
@@ -235,8 +233,6 @@ def mx_score(Q, X: MXTable, out: Optional[torch.Tensor] = None, out_dtype=torch.
         out.copy_(q @ R.mx_decode(X.data, X.scale, X.bits, dim).t())
         return out
     ld = out.stride(0) if B > 1 else X.rows
-    with _device_of(out):
-        N.check(N.require().fps_mx_score(Q.data.data_ptr() if mx else Q.data_ptr(), Q.scale.data_ptr() if mx else None,
-                                         X.data.data_ptr(), X.scale.data_ptr(), X.bits, B, X.rows, dim,
-                                         out.data_ptr(), _TYPE[out.dtype], ld, N.stream_ptr(out.device)), "mx_score")
+    _launch("mx_score", out.get_device(), Q.data.data_ptr() if mx else Q.data_ptr(), Q.scale.data_ptr() if mx else None,
+            X.data.data_ptr(), X.scale.data_ptr(), X.bits, B, X.rows, dim, out.data_ptr(), _TYPE[out.dtype], ld)
     return out

@@ -14,7 +14,7 @@ import torch
 
 from . import _native as N
 from . import reference as R
-from .mx import _TYPE, _device_of, _same_device
+from .mx import _TYPE, _launch, _same_device
 
 Setting = Union[float, int, torch.Tensor]
 
@@ -83,11 +83,9 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
         if with_prob:
             prob.copy_(q)
     elif B:
-        lib = N.require()
-        with _device_of(S):
-            size = lib.fps_sample_scores_ws_bytes(B, n)
-            ws = torch.empty(size, dtype=torch.uint8, device=S.device) if size else None
-            N.check(lib.fps_sample_scores(S.data_ptr(), _TYPE[S.dtype], B, n, S.stride(0) if B > 1 else n, u.data_ptr(),
-                                          N.ptr(t), t0, N.ptr(k), k0, N.ptr(p), p0, N.ptr(m), m0, out.data_ptr(),
-                                          N.ptr(prob), N.ptr(ws), N.stream_ptr(S.device)), "sample_scores")
+        size = N.require().fps_sample_scores_ws_bytes(B, n) if n > 32768 else 0
+        ws = torch.empty(size, dtype=torch.uint8, device=S.device) if size else None
+        _launch("sample_scores", S.get_device(), S.data_ptr(), _TYPE[S.dtype], B, n, S.stride(0) if B > 1 else n,
+                u.data_ptr(), N.ptr(t), t0, N.ptr(k), k0, N.ptr(p), p0, N.ptr(m), m0, out.data_ptr(), N.ptr(prob),
+                N.ptr(ws))
     return (out, prob) if with_prob else out
