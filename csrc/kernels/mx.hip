@@ -17,8 +17,10 @@
 // read, and each was stored by this call: the entries need no clearing.  (One pass of integer
 // maxima over cleared entries in place of the first two: 37 us for 1M rows, against 20.)
 //
-// A wave owns whole rows, 64 / lanes-per-row of them, so that nothing but registers is shared; it
-// takes UNROLL such groups together, their loads all in flight before the first store.
+// The lanes' shares of all rows lie one after another over the waves, whatever the width of a row
+// (whole rows per wave left a quarter of the lanes of 300-wide rows idle: 36 us for a read that
+// takes FILLME so).  Nothing but registers is shared; a wave takes UNROLL units of 64 together, their
+// loads all in flight before the first store.
 #include <hip/hip_fp16.h>
 
 #include "mx.h"
@@ -73,7 +75,7 @@ __device__ __forceinline__ void load8(const void* x, int64_t row, int D, int d, 
   }
 }
 
-constexpr int UNROLL = 4;  // groups of rows a wave takes together
+constexpr int UNROLL = 4;  // units a wave takes together
 
 __global__ void __launch_bounds__(256) mx_claim_kernel(const void* __restrict__ idx, int idx64, int64_t n,
                                                        int64_t rows, int32_t* __restrict__ owner) {
@@ -92,14 +94,43 @@ __global__ void __launch_bounds__(256) mx_raise_kernel(const void* __restrict__ 
   }
 }
 
-// where a lane works: `lpr` lanes per row (LPB per block); rows wider than a wave are walked in steps of 64
-struct Lane {
-  int row, g0;   // row within the wave's group, first group of VPL values
+// `lpr` lanes per row; lane l of unit u has share 64 u + l of the n * lpr.
+struct RowShape {
+  int lpr, grid;
+  float inv;                       // 1 / lpr
+  int unit_rows, unit_rem;         // 64 shares further: so many rows and shares
+  int64_t units, step_rows;        // a step of the whole grid
+  int step_rem;
+};
+struct Place {
+  int64_t row;
+  int g;        // the lane's share within the row
   bool on;
 };
-__device__ __forceinline__ Lane lane_of(int lpr, int rpw) {
-  const int lane = threadIdx.x & 63, row = lane / lpr;
-  return Lane{row, lane - row * lpr, row < rpw};
+// the first share of a unit; moved along without divisions
+struct Walk {
+  int64_t row;
+  int rem;
+  __device__ __forceinline__ void move(int64_t rows, int more, int lpr) {
+    row += rows;
+    rem += more;
+    if (rem >= lpr) { rem -= lpr; ++row; }
+  }
+  __device__ __forceinline__ Place place(const RowShape& s, int64_t n) const {
+    const int t = rem + (threadIdx.x & 63);
+    int q = (int)((float)t * s.inv);  // t / lpr, one off at most
+    int g = t - q * s.lpr;
+    if (g < 0) { g += s.lpr; --q; }
+    if (g >= s.lpr) { g -= s.lpr; ++q; }
+    return Place{row + q, g, row + q < n};
+  }
+};
+__device__ __forceinline__ int64_t first_unit() {
+  return ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * UNROLL;
+}
+__device__ __forceinline__ Walk walk_from(const RowShape& s, int64_t unit) {
+  const int64_t share = unit * 64, row = share / s.lpr;
+  return Walk{row, (int)(share - row * s.lpr)};
 }
 
 template <int BITS>
@@ -135,43 +166,41 @@ template <int T, int BITS, bool VEC, bool CLAIM>
 __global__ void __launch_bounds__(256) mx_set_rows_kernel(const void* __restrict__ x, const void* __restrict__ idx,
                                                           int idx64, int64_t n, int D, int64_t rows,
                                                           uint8_t* __restrict__ data, uint8_t* __restrict__ scale,
-                                                          int lpr, int rpw, const int32_t* __restrict__ owner) {
-  const Lane w = lane_of(lpr, rpw);
-  const int nblk = lpr / LPB;
+                                                          RowShape shape, const int32_t* __restrict__ owner) {
+  const int nblk = shape.lpr / LPB;
   const int64_t row_bytes = (int64_t)nblk * MX_BLOCK * BITS / 8;
-  const int64_t waves = (int64_t)gridDim.x * (blockDim.x >> 6);
-  for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6); u0 * UNROLL * rpw < n; u0 += waves) {
+  Walk walk = walk_from(shape, first_unit());
+  for (int64_t u0 = first_unit(); u0 < shape.units; u0 += (int64_t)gridDim.x * 4 * UNROLL) {
+    Place w[UNROLL];
     int64_t slot[UNROLL];
     float v[UNROLL][VPL];
+    Walk unit = walk;
+    walk.move(shape.step_rows, shape.step_rem, shape.lpr);
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const int64_t r = (u0 * UNROLL + k) * rpw + w.row;
+      w[k] = unit.place(shape, n);
+      unit.move(shape.unit_rows, shape.unit_rem, shape.lpr);
       slot[k] = -1;
-      if (w.on && r < n) {
-        slot[k] = row_of(idx, idx64, r);
-        load8<T, VEC>(x, r, D, w.g0 * VPL, v[k]);
+      if (w[k].on) {
+        slot[k] = row_of(idx, idx64, w[k].row);
+        load8<T, VEC>(x, w[k].row, D, w[k].g * VPL, v[k]);
       }
     }
-    int32_t own[UNROLL];
     if (CLAIM) {
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k) own[k] = slot[k] >= 0 && slot[k] < rows ? owner[slot[k]] : -1;
+      for (int k = 0; k < UNROLL; ++k)
+        if (slot[k] >= 0 && slot[k] < rows && owner[slot[k]] != (int32_t)w[k].row) slot[k] = -1;
     }
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const int64_t r = (u0 * UNROLL + k) * rpw + w.row;
-      if (CLAIM && own[k] != (int32_t)r) slot[k] = -1;
       if (slot[k] < 0 || slot[k] >= rows) continue;
-      for (int g = w.g0; g < lpr; g += 64) {
-        if (g != w.g0) load8<T, VEC>(x, r, D, g * VPL, v[k]);
-        uint32_t s;
-        uint2 q;
-        quantise<BITS>(v[k], s, q);
-        const int64_t at = slot[k] * row_bytes + (int64_t)g * (VPL * BITS / 8);
-        if (BITS == 4) *(uint32_t*)(data + at) = q.x;
-        else *(uint2*)(data + at) = q;
-        if ((g & (LPB - 1)) == 0) scale[slot[k] * nblk + g / LPB] = (uint8_t)s;
-      }
+      uint32_t s;
+      uint2 q;
+      quantise<BITS>(v[k], s, q);
+      const int64_t at = slot[k] * row_bytes + (int64_t)w[k].g * (VPL * BITS / 8);
+      if (BITS == 4) *(uint32_t*)(data + at) = q.x;
+      else *(uint2*)(data + at) = q;
+      if ((w[k].g & (LPB - 1)) == 0) scale[slot[k] * nblk + w[k].g / LPB] = (uint8_t)s;
     }
   }
 }
@@ -238,53 +267,55 @@ template <int T, int BITS, bool VEC>
 __global__ void __launch_bounds__(256) mx_gather_rows_kernel(const uint8_t* __restrict__ data,
                                                              const uint8_t* __restrict__ scale, int64_t rows, int D,
                                                              const void* __restrict__ idx, int idx64, int64_t n,
-                                                             void* __restrict__ out, int lpr, int rpw) {
+                                                             void* __restrict__ out, RowShape shape) {
   constexpr int V = T == T_F32 ? 4 : 8, PER = MX_BLOCK / V;
-  const Lane w = lane_of(lpr, rpw);
-  const int nblk = lpr / PER;
+  const int nblk = shape.lpr / PER;
   const int64_t row_bytes = (int64_t)nblk * MX_BLOCK * BITS / 8;
-  const int64_t waves = (int64_t)gridDim.x * (blockDim.x >> 6);
-  for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6); u0 * UNROLL * rpw < n; u0 += waves) {
+  Walk walk = walk_from(shape, first_unit());
+  for (int64_t u0 = first_unit(); u0 < shape.units; u0 += (int64_t)gridDim.x * 4 * UNROLL) {
+    Place w[UNROLL];
     int64_t slot[UNROLL];
+    uint2 q[UNROLL];
+    uint32_t s[UNROLL];
+    Walk unit = walk;
+    walk.move(shape.step_rows, shape.step_rem, shape.lpr);
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const int64_t r = (u0 * UNROLL + k) * rpw + w.row;
+      w[k] = unit.place(shape, n);
+      unit.move(shape.unit_rows, shape.unit_rem, shape.lpr);
+      w[k].on = w[k].on && w[k].g * V < D;
       slot[k] = -1;
-      if (w.on && r < n) slot[k] = row_of(idx, idx64, r);
-      if (slot[k] >= rows) slot[k] = -1;
+      if (w[k].on) slot[k] = row_of(idx, idx64, w[k].row);
     }
-    for (int g = w.g0; g < lpr && g * V < D; g += 64) {
-      uint2 q[UNROLL];
-      uint32_t s[UNROLL];
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k) {
-        q[k] = make_uint2(0, 0);
-        s[k] = 127;
-        if (slot[k] >= 0) {
-          q[k] = load_packed<BITS, V>(data + slot[k] * row_bytes + (int64_t)g * (V * BITS / 8));
-          s[k] = scale[slot[k] * nblk + g / PER];
-        }
+    for (int k = 0; k < UNROLL; ++k) {
+      q[k] = make_uint2(0, 0);
+      s[k] = 127;
+      if (slot[k] >= 0 && slot[k] < rows) {
+        q[k] = load_packed<BITS, V>(data + slot[k] * row_bytes + (int64_t)w[k].g * (V * BITS / 8));
+        s[k] = scale[slot[k] * nblk + w[k].g / PER];
       }
+    }
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k) {
-        const int64_t r = (u0 * UNROLL + k) * rpw + w.row;
-        float v[V];
-        values<BITS, V>(q[k], s[k], v);
-        if (w.on && r < n) store_values<T, V, VEC>(out, r, D, g * V, v);
-      }
+    for (int k = 0; k < UNROLL; ++k) {
+      float v[V];
+      values<BITS, V>(q[k], s[k], v);
+      if (w[k].on) store_values<T, V, VEC>(out, w[k].row, D, w[k].g * V, v);
     }
   }
 }
 
-struct RowShape {
-  int lpr, rpw, grid;
-};
-
 RowShape row_shape(int64_t n, int D, int lanes_per_block) {
   RowShape s;
   s.lpr = (D + MX_BLOCK - 1) / MX_BLOCK * lanes_per_block;
-  s.rpw = s.lpr >= 64 ? 1 : 64 / s.lpr;
-  s.grid = grid_for((n + s.rpw - 1) / s.rpw, 4 * UNROLL, 256 * 32);
+  s.inv = 1.f / (float)s.lpr;
+  s.unit_rows = 64 / s.lpr;
+  s.unit_rem = 64 % s.lpr;
+  s.units = (n * s.lpr + 63) / 64;
+  s.grid = grid_for(s.units, 4 * UNROLL, 256 * 32);
+  const int64_t step = (int64_t)s.grid * 4 * UNROLL * 64;
+  s.step_rows = step / s.lpr;
+  s.step_rem = (int)(step % s.lpr);
   return s;
 }
 
@@ -296,7 +327,7 @@ void set_rows(bool vec, bool claim, const RowShape& s, hipStream_t st, const voi
               int64_t n, int D, int64_t rows, uint8_t* data, uint8_t* scale, int32_t* owner) {
 #define FPS_MX_SET(V, C)                                                                                         \
   hipLaunchKernelGGL((mx_set_rows_kernel<T, BITS, V, C>), dim3(s.grid), dim3(256), 0, st, x, idx, idx64, n, \
-                     D, rows, data, scale, s.lpr, s.rpw, owner)
+                     D, rows, data, scale, s, owner)
   if (vec) { if (claim) FPS_MX_SET(true, true); else FPS_MX_SET(true, false); }
   else { if (claim) FPS_MX_SET(false, true); else FPS_MX_SET(false, false); }
 #undef FPS_MX_SET
@@ -307,10 +338,10 @@ void gather_rows(bool vec, const RowShape& s, hipStream_t st, const uint8_t* dat
                  int D, const void* idx, int idx64, int64_t n, void* out) {
   if (vec)
     hipLaunchKernelGGL((mx_gather_rows_kernel<T, BITS, true>), dim3(s.grid), dim3(256), 0, st, data, scale, rows,
-                       D, idx, idx64, n, out, s.lpr, s.rpw);
+                       D, idx, idx64, n, out, s);
   else
     hipLaunchKernelGGL((mx_gather_rows_kernel<T, BITS, false>), dim3(s.grid), dim3(256), 0, st, data, scale,
-                       rows, D, idx, idx64, n, out, s.lpr, s.rpw);
+                       rows, D, idx, idx64, n, out, s);
 }
 
 }  // namespace

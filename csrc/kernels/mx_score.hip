@@ -522,14 +522,14 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
   hipStream_t st = (hipStream_t)stream;
   const bool few = B <= 32, narrow = a.nblk <= 2;
   if (qs) {
-    if (narrow) { if (few) launch<4, true, 1, 4, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
+    if (narrow) { if (few) launch<4, true, 1, 2, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
     else if (a.B > 64 && a.nblk > 16 && a.s_word) launch_wide(a, out_type, st);
     else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 4, 2, 2, 16>(a, out_type, st); }
   } else if (xbits == 4) {
-    if (narrow) { if (few) launch<4, false, 1, 4, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
+    if (narrow) { if (few) launch<4, false, 1, 2, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
     else { if (few) launch<4, false, 1, 2, 4, 32>(a, out_type, st); else launch<4, false, 2, 2, 4, 16>(a, out_type, st); }
   } else {
-    if (narrow) { if (few) launch<8, false, 1, 4, 1, 2>(a, out_type, st); else launch<8, false, 2, 4, 1, 2>(a, out_type, st); }
+    if (narrow) { if (few) launch<8, false, 1, 2, 1, 2>(a, out_type, st); else launch<8, false, 2, 4, 1, 2>(a, out_type, st); }
     else { if (few) launch<8, false, 1, 2, 2, 32>(a, out_type, st); else launch<8, false, 2, 2, 2, 16>(a, out_type, st); }
   }
   FPS_CHECK_LAUNCH();
