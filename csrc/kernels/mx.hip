@@ -18,8 +18,8 @@
 // maxima over cleared entries in place of the first two: 37 us for 1M rows, against 20.)
 //
 // The lanes' shares of all rows lie one after another over the waves, whatever the width of a row
-// (whole rows per wave left a quarter of the lanes of 300-wide rows idle: 36 us for a read that
-// takes FILLME so).  Nothing but registers is shared; a wave takes UNROLL units of 64 together, their
+// (whole rows per wave left half of the lanes of 300-wide rows idle: 36 us for a read that takes
+// 28 so).  Nothing but registers is shared; a wave takes UNROLL units of 64 together, their
 // loads all in flight before the first store.
 #include <hip/hip_fp16.h>
 
@@ -33,6 +33,9 @@ constexpr int VPL = 8;            // values per lane of a write
 constexpr int LPB = MX_BLOCK / VPL;  // lanes per block
 
 enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ int64_t row_of(const void* idx, int idx64, int64_t r) {
   if (idx == nullptr) return r;
@@ -54,14 +57,13 @@ __device__ __forceinline__ void load8(const void* x, int64_t row, int D, int d, 
       const float* p = (const float*)x + row * D + d;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // D is a multiple of 4: a group of four is in or out whole
-        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (d + 4 * h < D) f = *(const float4*)(p + 4 * h);
-        v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
+        f32x4 f = {0.f, 0.f, 0.f, 0.f};
+        if (d + 4 * h < D) f = *(const f32x4*)(p + 4 * h);
+        v[4 * h] = f[0]; v[4 * h + 1] = f[1]; v[4 * h + 2] = f[2]; v[4 * h + 3] = f[3];
       }
     } else {  // D is a multiple of 8
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (d < D) u = *(const uint4*)((const uint16_t*)x + row * D + d);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      u32x4 w = {0, 0, 0, 0};
+      if (d < D) w = *(const u32x4*)((const uint16_t*)x + row * D + d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint16_t lo = (uint16_t)w[j], hi = (uint16_t)(w[j] >> 16);
@@ -211,7 +213,8 @@ __device__ __forceinline__ uint16_t to16(float f) {
 }
 
 // Read back V values a lane: 16 bytes of output, so that a wave's store is one run of whole lines (8 fp32
-// values a lane, two stores 32 bytes apart: 74 us for 1M x 64 against FILLME).
+// values a lane, two stores 32 bytes apart: 74 us for 1M x 64 in order against 56), past the
+// caches, which keep the table instead (42 us; rows in random order 70 -> 64 us).
 template <int BITS, int V>
 __device__ __forceinline__ void values(uint2 q, uint32_t s, float v[V]) {
   const float f = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
@@ -238,12 +241,12 @@ template <int T, int V, bool VEC>
 __device__ __forceinline__ void store_values(void* out, int64_t r, int D, int d, const float v[V]) {
   if (VEC) {  // D is a multiple of V
     if constexpr (T == T_F32) {
-      *(float4*)((float*)out + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+      __builtin_nontemporal_store((f32x4){v[0], v[1], v[2], v[3]}, (f32x4*)((float*)out + r * D + d));
     } else {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = (uint32_t)to16<T>(v[2 * j]) | ((uint32_t)to16<T>(v[2 * j + 1]) << 16);
-      *(uint4*)((uint16_t*)out + r * D + d) = make_uint4(w[0], w[1], w[2], w[3]);
+      __builtin_nontemporal_store((u32x4){w[0], w[1], w[2], w[3]}, (u32x4*)((uint16_t*)out + r * D + d));
     }
   } else {
 #pragma unroll
