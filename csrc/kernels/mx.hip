@@ -96,6 +96,31 @@ __global__ void __launch_bounds__(256) mx_raise_kernel(const void* __restrict__ 
   }
 }
 
+// Both in one launch for few rows: one workgroup, the barrier between the stores and the reads.  (4096 rows: 5.5 us, against 4.8 us in two
+// launches and what the second costs the host.)
+constexpr int FEW_ROWS = 4096;
+__global__ void __launch_bounds__(1024) mx_claim_few_kernel(const void* __restrict__ idx, int idx64, int n, int64_t rows,
+                                                            int32_t* owner) {
+  int64_t slot[FEW_ROWS / 1024];
+#pragma unroll
+  for (int k = 0; k < FEW_ROWS / 1024; ++k) {
+    const int r = threadIdx.x + k * 1024;
+    slot[k] = r < n ? row_of(idx, idx64, r) : -1;
+    if (slot[k] >= rows) slot[k] = -1;
+  }
+#pragma unroll
+  for (int k = 0; k < FEW_ROWS / 1024; ++k)
+    if (slot[k] >= 0)
+      __hip_atomic_store(owner + slot[k], (int32_t)(threadIdx.x + k * 1024), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < FEW_ROWS / 1024; ++k) {
+    const int32_t r = threadIdx.x + k * 1024;
+    if (slot[k] >= 0 && __hip_atomic_load(owner + slot[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) < r)
+      atomicMax(owner + slot[k], r);
+  }
+}
+
 // `lpr` lanes per row; lane l of unit u has share 64 u + l of the n * lpr.
 struct RowShape {
   int lpr, grid;
@@ -358,7 +383,10 @@ FPS_API int fps_mx_set_rows(const void* x, int type, const void* idx, int idx64,
   const bool claim = idx != nullptr && n > 1;
   if (claim && owner == nullptr) return (int)hipErrorInvalidValue;
   hipStream_t st = (hipStream_t)stream;
-  if (claim) {
+  if (claim && n <= FEW_ROWS) {
+    hipLaunchKernelGGL(mx_claim_few_kernel, dim3(1), dim3(1024), 0, st, idx, idx64, (int)n, rows, owner);
+    FPS_CHECK_LAUNCH();
+  } else if (claim) {
     hipLaunchKernelGGL(mx_claim_kernel, dim3(grid_for(n, 256)), dim3(256), 0, st, idx, idx64, n, rows, owner);
     FPS_CHECK_LAUNCH();
     hipLaunchKernelGGL(mx_raise_kernel, dim3(grid_for(n, 256)), dim3(256), 0, st, idx, idx64, n, rows, owner);

@@ -36,9 +36,9 @@ constexpr int BINS = 2048;
 constexpr int THREADS = 512;    // of a finishing workgroup
 constexpr int WAVES = THREADS / 64;
 constexpr int PER = BINS / THREADS;   // bins per thread of a search
-constexpr int LIST = 2048;      // scores listed in LDS
+constexpr int LIST = 1024;      // scores listed in LDS
 constexpr int RANK = 256;       // listed scores ranked against each other; more are split by bits
-constexpr int SHORT_K = 1024;   // top-k up to this lists its candidates
+constexpr int SHORT_K = 512;    // top-k up to this lists its candidates
 constexpr int CACHED_SEGS = 128;     // segments of a row that takes one launch
 constexpr int PASS_SEGS = 64;   // segments per workgroup of the passes over long rows
 
@@ -376,7 +376,8 @@ __device__ __forceinline__ void hist_add(uint32_t* hc, unsigned long long* hm, b
   }
 }
 
-constexpr int WANTED = 4 * THREADS;  // segments looked at together
+constexpr int WANTED = 8 * THREADS;  // segments looked at together
+constexpr int KEPT = 8 * THREADS;    // segments' maxima that a long row's workgroup keeps in LDS
 
 template <bool COUNTS>
 struct Hist {
@@ -489,10 +490,13 @@ template <int T, int R>
 struct Source {
   const Args& a;
   const int b, lane, wave;
-  const float* segmax;
+  const float* in_lds;   // the maxima, or
+  const float* in_memory;
   float v[4];
-  __device__ Source(const Args& a_, int b_, const float* sm)
-      : a(a_), b(b_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), segmax(sm) {}
+  __device__ Source(const Args& a_, int b_, const float* lds, const float* memory)
+      : a(a_), b(b_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), in_lds(lds), in_memory(memory) {}
+  __device__ __forceinline__ bool kept() const { return R != ROW_LONG || a.nseg <= KEPT; }
+  __device__ __forceinline__ float segmax(int64_t s) const { return kept() ? in_lds[s] : in_memory[s]; }
   // f(segment, scores) for the segments whose largest score (not -inf) is wanted.  Their maxima
   // are looked at first, many together; the waves share out the wanted ones and load G at a time.
   template <int G = 4, typename P, typename F>
@@ -507,7 +511,7 @@ struct Source {
 #pragma unroll
         for (int j = 0; j < WANTED / THREADS; ++j) {
           const int64_t at = base + j * THREADS + threadIdx.x;
-          m[j] = at < a.nseg ? segmax[at] : -INFINITY;
+          m[j] = at < a.nseg ? segmax(at) : -INFINITY;
         }
         __syncthreads();
 #pragma unroll
@@ -634,10 +638,9 @@ __device__ __forceinline__ int take_places(const bool on[4], int* count, int pla
   return total;
 }
 
-// Put the scores for which pick(key, bin) holds into sh.list; sh.n counts them all.
+// Put the scores for which pick(score) holds into sh.list; sh.n counts them all.
 template <int T, int R, typename P, typename F>
-__device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, const Row& r, float cb, int shift,
-                                        P want, F pick) {
+__device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, const Row& r, int shift, P want, F pick) {
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
@@ -645,7 +648,7 @@ __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, 
     bool on[4];
     int place[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) on[j] = v[j] > -INFINITY && pick(key_of(v[j]), bin_of(v[j], M, cb));
+    for (int j = 0; j < 4; ++j) on[j] = v[j] > -INFINITY && pick(v[j]);
     if (take_places(on, &sh.n, place) == 0) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -937,7 +940,7 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
   const Found<double> f = find_segment<double>(
       a, b, sh, ties, wt,
       [&](int64_t s, double& m, uint32_t& c) {
-        const float x = src.segmax[s];
+        const float x = src.segmax(s);
         if (!(x >= bound) || x == -INFINITY) return false;
         m = segmass[s];
         if (have_mass) m *= w_of(x);
@@ -1014,7 +1017,7 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
       __syncthreads();
       t = sh.kmin - 1;
     } else {
-      collect<T, R>(src, sh, M, r, cb, shift, reaches(kbin), [&](uint32_t, int bin) { return bin == kbin; });
+      collect<T, R>(src, sh, M, r, shift, reaches(kbin), [&](float x) { return bin_of(x, M, cb) == kbin; });
       const int n = sh.n;
       if (n <= RANK) {
         const Slot s = rank_list(sh, n, r.k, cbefore);
@@ -1047,8 +1050,8 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
     const uint64_t above = sh.before_m;
     const uint32_t floor_key = bin == kbin ? (ties ? t : t + 1) : 0;  // what top-k left of this bin
     const uint32_t tie_cap = bin == kbin && ties ? ties : 0xffffffffu;
-    collect<T, R>(src, sh, M, r, cb, shift, reaches(bin),
-                  [&](uint32_t key, int x) { return x == bin && key >= floor_key; });
+    collect<T, R>(src, sh, M, r, shift, reaches(bin),
+                  [&](float x) { return bin_of(x, M, cb) == bin && key_of(x) >= floor_key; });
     const int n = sh.n;
     // (scores equal to top-k's threshold beyond its ties rank behind all that stay, and the mass
     // before them has reached the total: the cut drops them)
@@ -1074,16 +1077,15 @@ template <int T, int R>
 __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   __shared__ Shared sh;
   constexpr int SMALL = R == ROW_REGS ? WAVES : R == ROW_CACHED ? CACHED_SEGS : 1;
-  __shared__ float small_max[SMALL];
+  __shared__ float small_max[R == ROW_LONG ? KEPT : SMALL];
   __shared__ double small_mass[SMALL];
   __shared__ int32_t small_tie[SMALL];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Row r = row_settings(a, b);
   constexpr bool own = R != ROW_LONG;
-  const float* segmax = own ? small_max : a.segmax + (int64_t)b * a.nseg;
   double* segmass = own ? small_mass : (double*)a.segmass + (int64_t)b * a.nseg;
   int32_t* segtie = own ? small_tie : a.segtie + (int64_t)b * a.nseg;
-  Source<T, R> src(a, b, segmax);
+  Source<T, R> src(a, b, small_max, own ? nullptr : a.segmax + (int64_t)b * a.nseg);
   float m = -INFINITY;
   if constexpr (R == ROW_REGS) {
     if (wave < a.nseg) {
@@ -1108,7 +1110,13 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
         }
     }
   } else {
-    for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) m = fmaxf(m, segmax[i]);
+    const bool keep = src.kept();
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) {
+      const float x = src.in_memory[i];
+      if (keep) small_max[i] = x;
+      m = fmaxf(m, x);
+    }
   }
   const float M = block_max(m, sh.tmp);
   if (M == -INFINITY) {  // nothing is left of the row
@@ -1125,7 +1133,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     } else {
       double sum = 0, total;
       for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS)
-        if (segmax[i] > -INFINITY) sum += segmass[i] * weight(segmax[i], M, r.c);
+        if (src.segmax(i) > -INFINITY) sum += segmass[i] * weight(src.segmax(i), M, r.c);
       block_scan(sum, sh.scan_d, total);
       // N scores below (1 - p) total / N hold less than (1 - p) total: the threshold is not among
       // them, and the bins but the last span the octaves above that
@@ -1150,7 +1158,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     clear_hist(sh);
     if constexpr (R == ROW_LONG) {
       for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) {
-        const float x = segmax[i];
+        const float x = src.segmax(i);
         if (x > -INFINITY) atomicAdd(&sh.hc[bin_of(x, M, cb)], 1u);
       }
     } else {
@@ -1163,9 +1171,12 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     __syncthreads();
     find_bin<BY_COUNT>(sh, (uint32_t)r.k);
     // fewer unmasked than k: everything unmasked is a candidate
-    const int edge = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k ? BINS : sh.bin;
-    collect<T, R>(src, sh, M, r, cb, 51, [&](float x) { return bin_of(x, M, cb) <= edge; },
-                  [&](uint32_t, int bin) { return bin <= edge; });
+    // A score a little below the last of those bins (fp32 rounds M - s and its product by 2^-23 or so: a few
+    // candidates more do no harm), so that a score takes one comparison.
+    const bool all = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k || sh.bin == BINS - 1 || !(M < INFINITY);
+    const double low = (double)M - (double)(sh.bin + 1) / (double)cb * (1 + 1e-6) - fabs((double)M) * 1e-6;
+    const float cut = all ? -INFINITY : (float)low;
+    collect<T, R>(src, sh, M, r, 51, [=](float x) { return x >= cut; }, [=](float x) { return x >= cut; });
     const int n = sh.n;
     if (n <= RANK) {
       Slot s = rank_list(sh, n, r.k, 0);
@@ -1313,7 +1324,11 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
   const Row r = row_settings(a, b);
   uint64_t* segmass = a.segmass + (int64_t)b * a.nseg;
   if (st.listed > (uint32_t)a.listcap) {  // more than a list of equal or near-equal scores: the row again
-    Source<T, ROW_LONG> src(a, b, a.segmax + (int64_t)b * a.nseg);
+    __shared__ float maxima[KEPT];
+    Source<T, ROW_LONG> src(a, b, maxima, a.segmax + (int64_t)b * a.nseg);
+    if (src.kept())
+      for (int i = threadIdx.x; i < a.nseg; i += THREADS) maxima[i] = src.in_memory[i];
+    __syncthreads();
     finish_general<T, ROW_LONG>(a, b, src, sh, r, st.M, (double*)segmass, a.segtie + (int64_t)b * a.nseg);
     return;
   }
@@ -1333,8 +1348,8 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
   const AsFixed w_of{st.M, r.c, st.shift};
   uint64_t wt = w_of(score_of(t));
   if (r.cut_min && weight(score_of(t), st.M, r.c) < r.minp) { wt = 0; ties = 0; }
-  // Listed scores above t add to their segments' masses, ties are counted per segment: in LDS (the
-  // list's and the histogram's) for up to 2 LIST segments, else in the workspace.
+  // Listed scores above t add to their segments' masses, ties are counted per segment: in LDS where
+  // they fit, else in the workspace.
   const auto add = [&](auto plus_mass, auto plus_tie) {
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const Entry e = list[i];
@@ -1346,10 +1361,10 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
     }
   };
   Found<uint64_t> f;
-  if (a.nseg <= 2 * LIST) {
-    unsigned long long* more = (unsigned long long*)sh.list;
+  if (a.nseg <= KEPT) {
+    __shared__ unsigned long long more[KEPT];
     uint32_t* tied = (uint32_t*)sh.hm;
-    static_assert(2 * LIST * 4 <= BINS * 8, "a tie count per segment");
+    static_assert(KEPT * 4 <= BINS * 8, "a tie count per segment");
     __syncthreads();
     for (int s = threadIdx.x; s < a.nseg; s += THREADS) { more[s] = 0; tied[s] = 0; }
     __syncthreads();

@@ -106,7 +106,7 @@ def test_edges_of_the_range(dev, fmt):
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("fmt", ["fp4", "fp8"])
 @pytest.mark.parametrize("idx_dtype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("slots,n,dim", [(10, 1, 64), (50, 20, 33), (1000, 700, 300), (40, 500, 1100), (5000, 3000, 64)])
+@pytest.mark.parametrize("slots,n,dim", [(10, 1, 64), (50, 20, 33), (1000, 700, 300), (40, 500, 1100), (5000, 3000, 64), (3000, 9000, 64)])
 def test_indexed_write_last_row_wins_and_the_rest_stays(dev, fmt, idx_dtype, slots, n, dim):
     old, new = make(slots, dim, seed=1), make(n, dim, seed=2)
     g = torch.Generator().manual_seed(slots + n)
