@@ -180,11 +180,13 @@ __device__ __forceinline__ float load1(const void* p, int64_t i) {
 // NaN is masked; -0 and +0 are one score
 __device__ __forceinline__ float clean(float f) { return f == f ? f + 0.f : -INFINITY; }
 
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // this lane's four scores of a segment as they lie in memory; places past the row are masked
 template <int T>
 __device__ __forceinline__ void load_raw(const Args& a, int b, int64_t seg, int lane, float v[4]) {
   const int64_t i = seg * SEG + lane * 4, at = (int64_t)b * a.ld + i;
-  if (a.vec && i + 4 <= a.N) {
+  if (a.vec && (seg + 1) * SEG <= a.N) {  // (one branch for the wave)
     if (T == T_F32) {
       const float4 f = *(const float4*)((const float*)a.s + at);
       v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
@@ -315,7 +317,7 @@ template <int T>
 __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   const int b = blockIdx.y, lane = threadIdx.x & 63;
   const Row r = row_settings(a, b);
-  const int64_t seg0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * STAT_SEGS;
+  const int64_t seg0 = ((int64_t)blockIdx.x * 4 + wave_id()) * STAT_SEGS;
   if (seg0 >= a.nseg) return;
   const bool mass = r.direct() && !r.cut_min;
   // rows that cut by mass: fp32 sums, to place the histogram's bins
@@ -429,7 +431,7 @@ enum Search { BY_COUNT, BY_COUNT_WITH_MASS, BY_MASS };
 // bin reach it: the last bin that holds anything.
 template <Search S, typename H>
 __device__ __forceinline__ void find_bin(H& sh, uint32_t need, uint64_t above = 0, double target = 0, double part = -1) {
-  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+  const int i = threadIdx.x, lane = i & 63, wave = wave_id();
   uint32_t c[PER], ct = 0, cc = 0, call;
   uint64_t m[PER], mt = 0, mm = 0, mall;
 #pragma unroll
@@ -494,7 +496,7 @@ struct Source {
   const float* in_memory;
   float v[4];
   __device__ Source(const Args& a_, int b_, const float* lds, const float* memory)
-      : a(a_), b(b_), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), in_lds(lds), in_memory(memory) {}
+      : a(a_), b(b_), lane(threadIdx.x & 63), wave(wave_id()), in_lds(lds), in_memory(memory) {}
   __device__ __forceinline__ bool kept() const { return R != ROW_LONG || a.nseg <= KEPT; }
   __device__ __forceinline__ float segmax(int64_t s) const { return kept() ? in_lds[s] : in_memory[s]; }
   // f(segment, scores) for the segments whose largest score (not -inf) is wanted.  Their maxima
@@ -554,7 +556,7 @@ struct Share {
   int i, j0, j1;  // this lane's score; its part of the list
 };
 __device__ __forceinline__ Share share_list(int n) {
-  const int wave = threadIdx.x >> 6;
+  const int wave = wave_id();
   const int G = n <= 64 ? 1 : n <= 128 ? 2 : 4;
   const int parts = WAVES / G, part = wave / G, per = (n + parts - 1) / parts;
   return Share{(wave % G) * 64 + (int)(threadIdx.x & 63), min(n, part * per), min(n, (part + 1) * per)};
@@ -780,7 +782,7 @@ struct Found {
 template <typename V, typename G>
 __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& sh, uint32_t ties, V wt, G get, V* tmp_v,
                                                  Found<V>* found) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t run = (a.nseg + THREADS - 1) / THREADS;
   const int64_t s0 = min(run * threadIdx.x, a.nseg), s1 = min(s0 + run, a.nseg);
   uint32_t tie0 = 0, tall;
@@ -1080,7 +1082,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   __shared__ float small_max[R == ROW_LONG ? KEPT : SMALL];
   __shared__ double small_mass[SMALL];
   __shared__ int32_t small_tie[SMALL];
-  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = wave_id();
   const Row r = row_settings(a, b);
   constexpr bool own = R != ROW_LONG;
   double* segmass = own ? small_mass : (double*)a.segmass + (int64_t)b * a.nseg;
@@ -1206,7 +1208,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
 template <int T>
 __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
   __shared__ unsigned long long hm[BINS];
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = wave_id();
   const RowState st = a.state[b];
   if (!st.active) return;
   const Row r = row_settings(a, b);
@@ -1247,7 +1249,7 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   __shared__ Entry listed[PASS_LIST];
   __shared__ float above[WAVES][SEG];
   __shared__ int count;
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = wave_id();
   const RowState st = a.state[b];  // (target, bin, above and listed are written by this kernel, and not read)
   if (!st.active) return;
   const Row r = row_settings(a, b);
