@@ -7,13 +7,14 @@
 //   min-p  of those, the ones with w_i >= min_p    (the best one has w = 1)
 //   answer the first index i with sum_{j <= i, j kept} w_j > u * sum_{j kept} w_j
 //
-// Bound by one read of the scores, so a long row (> 32768) is read once in full where it can
+// Bound by one read of the scores, so a long row (> 16384) is read once in full where it can
 // be: the stats pass takes the largest score of every segment of 256 (and its mass, where
-// masses decide), and the finishing workgroup of a row then reads only segments whose
-// largest score can matter.  With a short top-k that is about k segments; without a cut it is
-// one.  Top-p alone needs the masses of all scores above its threshold: two more passes
-// over the row, spread over the chip (a histogram of mass, then the segments' masses above the
-// threshold's bin and a list of the scores inside it).  Shorter rows take one launch.
+// nothing is cut), and the finishing workgroup of a row then reads only segments whose
+// largest score can matter: about k of them for a short top-k, one without a cut.  Other
+// cuts need counts or masses of all scores above a threshold: passes over the row, spread
+// over the chip (a histogram, then the segments' masses above the threshold's bin and a list of
+// the scores inside it); a long top-k and then top-p take them twice.  Shorter rows take one
+// launch.  (Rows of 16384: 16 us either way without a cut; 32768: 26 us in one launch, 15 so.)
 //
 // Nothing is sorted.  Thresholds are found over bins of (max s - s) / T, and the scores of the
 // bin that holds the threshold are ranked against each other (up to 256 of them) or split
@@ -39,7 +40,7 @@ constexpr int PER = BINS / THREADS;   // bins per thread of a search
 constexpr int LIST = 1024;      // scores listed in LDS
 constexpr int RANK = 256;       // listed scores ranked against each other; more are split by bits
 constexpr int SHORT_K = 512;    // top-k up to this lists its candidates
-constexpr int CACHED_SEGS = 128;     // segments of a row that takes one launch
+constexpr int CACHED_SEGS = 64;      // segments of a row that takes one launch
 constexpr int PASS_SEGS = 64;   // segments per workgroup of the passes over long rows
 
 // a listed score: its key above the complement of its index (the larger word is the better score,
@@ -54,15 +55,21 @@ __device__ __forceinline__ Entry make_entry(uint32_t key, int32_t idx, uint64_t 
   return Entry{(uint64_t)key << 32 | (uint32_t)~idx, w};
 }
 
-// what the passes over a long row that cuts by mass alone share
+// What the passes over a long row share.  A round finds one threshold: by count (top-k), or by mass (top-p)
+// among the scores above `floor_key` and the first `ties` equal to it (what top-k left); or none (NO_CUT),
+// for the segments' masses alone.
+enum { IDLE = 0, BY_TOP_K = 1, BY_TOP_P = 2, NO_CUT = 3 };
 struct RowState {
-  int active;
-  float M, cb;     // largest score; bins per unit of score
-  int shift;
-  double target;   // p * total
-  uint64_t above;  // mass of the bins before `bin`
-  int bin;         // holds the threshold
-  uint32_t listed; // scores in it
+  int mode;
+  float M, cb;         // largest score; bins per unit of score
+  int shift;           // masses are multiples of 2^-shift
+  uint32_t floor_key, ties;
+  double target;       // count, or mass, that the threshold's bin reaches; < 0: p * all mass, which
+  double part;         // then stands here
+  uint64_t above;      // what the bins before `bin` hold of it
+  uint64_t all;        // bin == BINS: what all bins hold
+  int bin;             // the threshold's; BINS: all scores above floor_key stay
+  uint32_t listed;     // scores in it
 };
 
 struct Args {
@@ -79,7 +86,7 @@ struct Args {
   float* prob;
   // workspace (long rows)
   uint64_t* segmass; // [B, nseg] doubles (stats pass) or whole numbers (collect pass)
-  uint64_t* hmass;   // [B, BINS]     } rows that may cut by mass alone
+  uint64_t* hmass;   // [B, BINS]     } rows that may take passes
   Entry* list;       // [B, listcap]  }
   RowState* state;   // [B]           }
   float* segmax;     // [B, nseg]
@@ -94,6 +101,8 @@ struct Row {
   bool cut_p, cut_min;
   __device__ bool direct() const { return k == 0 && !cut_p; }
   __device__ bool by_mass() const { return k == 0 && cut_p; }
+  // a top-k for which the k largest scores are listed outright
+  __device__ bool short_k() const { return k > 0 && k <= SHORT_K; }
 };
 
 __device__ __forceinline__ Row row_settings(const Args& a, int b) {
@@ -1125,14 +1134,13 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     if (threadIdx.x == 0) {
       a.out[b] = -1;
       if (a.prob) a.prob[b] = 0.f;
-      if (passes) a.state[b].active = 0;
+      if (passes) a.state[b].mode = IDLE;
     }
     return;
   }
   if (R == ROW_LONG && passes) {
-    if (!r.by_mass()) {
-      if (threadIdx.x == 0) a.state[b].active = 0;
-    } else {
+    RowState st{IDLE, M, 0.f, 0, KEY_NONE, 0, -1.0, 0.0, 0, 0, 0, 0};
+    if (r.by_mass()) {
       double sum = 0, total;
       for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS)
         if (src.segmax(i) > -INFINITY) sum += segmass[i] * weight(src.segmax(i), M, r.c);
@@ -1141,24 +1149,42 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
       // them, and the bins but the last span the octaves above that
       const double least = fmax((1 - r.p) * total / (double)a.N, 0x1p-60);
       const double octaves = fmax(-log2(least), 0.0) + 0.125;
-      for (int i = threadIdx.x; i < BINS; i += THREADS) a.hmass[(int64_t)b * BINS + i] = 0;
-      if (threadIdx.x == 0)
-        a.state[b] = RowState{1, M, (float)(r.c * (BINS - 1) / octaves), shift_for(2 * total), 0, 0, 0, 0};
-      return;
+      st.mode = BY_TOP_P;
+      st.cb = (float)(r.c * (BINS - 1) / octaves);
+      st.shift = shift_for(2 * total);
+    } else if (r.k > 0 && !r.short_k()) {
+      // the bins span eight times the range of the segments' maxima, which for scores of any common
+      // distribution is beyond their bulk; a threshold in the last bin, of all below, still stands
+      float low = INFINITY;
+      for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS)
+        if (src.segmax(i) > -INFINITY) low = fminf(low, src.segmax(i));
+      low = -block_max(-low, sh.tmp);
+      const float range = 8 * (M - low);
+      st.mode = BY_TOP_K;
+      st.cb = range > 0 && range < INFINITY ? (float)(BINS - 1) / range : 32.f;
+      st.shift = shift_for((double)a.N);
+      st.target = (double)r.k;
+    } else if (r.direct() && r.cut_min) {
+      st.mode = NO_CUT;
+      st.shift = shift_for((double)a.N);
+      st.bin = BINS;
     }
+    if (threadIdx.x == 0) a.state[b] = st;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) a.hmass[(int64_t)b * BINS + i] = 0;
+    if (st.mode != IDLE) return;
   }
   if (r.direct()) {
     draw_from_row<T, R>(a, b, src, sh, r, M, KEY_NONE, 0, segmass, segtie, R == ROW_LONG && !r.cut_min);
     return;
   }
-  if (r.k > 0 && r.k <= SHORT_K && (R != ROW_LONG || r.k <= a.nseg / 2)) {
+  if (r.short_k()) {
     // A short list: the k best lie in bins up to the one in which the count of scores reaches k.  On a
-    // long row the segments' maxima are counted: that many scores, one a segment, are in
-    // those bins already, and few others (for k up to half the segments).
+    // long row the segments' maxima are counted where they are at least 2 k: that many scores, one
+    // a segment, are in those bins already, and few others.
     const float cb = (float)(r.c * 32);
     const auto any = [](float) { return true; };
     clear_hist(sh);
-    if constexpr (R == ROW_LONG) {
+    if (R == ROW_LONG && r.k <= a.nseg / 2) {
       for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) {
         const float x = src.segmax(i);
         if (x > -INFINITY) atomicAdd(&sh.hc[bin_of(x, M, cb)], 1u);
@@ -1203,18 +1229,20 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   finish_general<T, R>(a, b, src, sh, r, M, segmass, segtie);
 }
 
-// ---- long rows that cut by mass alone: mass by bin, then what lies above and in the threshold's
+// ---- a round of passes over long rows: counts or masses by bin, then what lies above the threshold's bin and in it, then the threshold
 
 template <int T>
 __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
   __shared__ unsigned long long hm[BINS];
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = wave_id();
   const RowState st = a.state[b];
-  if (!st.active) return;
+  if (st.mode == IDLE || st.mode == NO_CUT) return;
   const Row r = row_settings(a, b);
+  const bool counts = st.mode == BY_TOP_K;
+  const float floor_score = score_of(st.floor_key);
   for (int i = threadIdx.x; i < BINS; i += THREADS) hm[i] = 0;
   __syncthreads();
-  uint64_t rest = 0;  // the last bin's mass: scores that cannot hold the threshold
+  uint64_t rest = 0;  // the last bin's: scores that can hardly hold the threshold
   const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
   for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
     float x[4][4];
@@ -1227,9 +1255,10 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
       for (int i = 0; i < 4; ++i) {
         const float v = clean(x[j][i]);
         const int bin = bin_of(v, st.M, st.cb);
-        const uint64_t w = v > -INFINITY ? fixed(weight(v, st.M, r.c), st.shift) : (uint64_t)0;
-        const bool on = v > -INFINITY && bin < BINS - 1;
-        if (on) atomicAdd(&hm[bin], (unsigned long long)w);
+        const bool in = v > floor_score;
+        uint64_t w = in;
+        if (!counts) w = in ? fixed(weight(v, st.M, r.c), st.shift) : (uint64_t)0;
+        if (in && bin < BINS - 1) atomicAdd(&hm[bin], (unsigned long long)w);
         else rest += w;
       }
     }
@@ -1250,17 +1279,27 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   __shared__ float above[WAVES][SEG];
   __shared__ int count;
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = wave_id();
-  const RowState st = a.state[b];  // (target, bin, above and listed are written by this kernel, and not read)
-  if (!st.active) return;
+  const RowState st = a.state[b];  // (of which this kernel writes bin, above and listed, and reads none of them)
+  const double st_target = st.target;
+  if (st.mode == IDLE) return;
   const Row r = row_settings(a, b);
-  for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hm[i] = a.hmass[(int64_t)b * BINS + i];
-  __syncthreads();
-  find_bin<BY_MASS>(sh, 0, 0, 0, fmax(r.p, 0.0));
-  const int bin = sh.bin;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    a.state[b].target = sh.target;
-    a.state[b].bin = bin;
-    a.state[b].above = sh.before_m;
+  const float floor_score = score_of(st.floor_key);
+  // min-p drops scores from the draw, not from the total of which top-p keeps a part
+  const bool drop = r.cut_min && !(st.mode == BY_TOP_K && r.cut_p);
+  int bin = BINS;
+  if (st.mode != NO_CUT) {
+    for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hm[i] = a.hmass[(int64_t)b * BINS + i];
+    __syncthreads();
+    find_bin<BY_MASS>(sh, 0, 0, st_target, st_target < 0 ? fmax(r.p, 0.0) : -1.0);
+    bin = sh.bin;
+    // all that lies above top-k's ties is less than top-p's part: the threshold is those ties
+    if (st.mode == BY_TOP_P && st.ties && (bin < 0 || (double)(sh.before_m + sh.hm[bin]) < sh.target)) bin = BINS;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      if (st.mode == BY_TOP_P && st_target < 0) a.state[b].part = sh.target;
+      a.state[b].bin = bin;
+      a.state[b].above = sh.before_m;
+      a.state[b].all = bin == BINS ? sh.before_m + (sh.bin >= 0 ? sh.hm[sh.bin] : 0) : 0;
+    }
   }
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
@@ -1283,8 +1322,8 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[j][i] = clean(x[j][i]);
-        const int at_bin = x[j][i] > -INFINITY ? bin_of(x[j][i], st.M, st.cb) : BINS;
-        in[i] = at_bin == bin;
+        const int at_bin = x[j][i] > floor_score ? bin_of(x[j][i], st.M, st.cb) : BINS;
+        in[i] = at_bin == bin && bin < BINS;
         up[i] = at_bin < bin;
         const uint64_t mask = __ballot(up[i]);
         if (up[i]) above[wave][n + __popcll(mask & ((1ull << lane) - 1))] = x[j][i];
@@ -1293,10 +1332,17 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
       uint64_t sum = 0;
       for (int i = lane; i < n; i += 64) {
         const double w = weight(above[wave][i], st.M, r.c);
-        if (!r.cut_min || w >= r.minp) sum += fixed(w, st.shift);
+        if (!drop || w >= r.minp) sum += fixed(w, st.shift);
       }
       sum = wave_sum(sum);
       if (lane == 0) a.segmass[(int64_t)b * a.nseg + seg] = sum;
+      if (bin == BINS && st.ties) {  // the scores equal to the floor: not listed, counted here
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c += x[j][i] == floor_score;
+        c = wave_sum(c);
+        if (lane == 0) a.segtie[(int64_t)b * a.nseg + seg] = (int32_t)c;
+      }
       if (take_places(in, &count, place))
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -1315,17 +1361,20 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   for (int i = threadIdx.x; i < n; i += THREADS) put((uint32_t)(count + i), listed[i]);
 }
 
-// the threshold inside the listed bin, then the draw over whole-number masses
+// The threshold inside the listed bin; then the draw over whole-number masses, or, after top-k where top-p
+// is to follow, the state of a second round.
 template <int T>
-__global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
   __shared__ Shared sh;
   __shared__ Found<uint64_t> found;
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const RowState st = a.state[b];
-  if (!st.active) return;
+  if (st.mode == IDLE) return;
   const Row r = row_settings(a, b);
   uint64_t* segmass = a.segmass + (int64_t)b * a.nseg;
-  if (st.listed > (uint32_t)a.listcap) {  // more than a list of equal or near-equal scores: the row again
+  __syncthreads();
+  if (threadIdx.x == 0) a.state[b].mode = IDLE;
+  if (st.bin < BINS && st.listed > (uint32_t)a.listcap) {  // more than a list of equal or near-equal scores: the row again
     __shared__ float maxima[KEPT];
     Source<T, ROW_LONG> src(a, b, maxima, a.segmax + (int64_t)b * a.nseg);
     if (src.kept())
@@ -1334,20 +1383,64 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
     finish_general<T, ROW_LONG>(a, b, src, sh, r, st.M, (double*)segmass, a.segtie + (int64_t)b * a.nseg);
     return;
   }
-  const int n = (int)st.listed;
+  const int n = st.bin < BINS ? (int)st.listed : 0;
   const Entry* list = a.list + (int64_t)b * a.listcap;
-  if (n <= RANK) {
-    if ((int)threadIdx.x < n) sh.list[threadIdx.x] = list[threadIdx.x];
-    __syncthreads();
-    Slot s = rank_list(sh, n, 0, 0);
-    cut_by_mass(s, st.above, st.target);
-    list_threshold(sh, s);
-  } else {
-    split<BY_MASS>(sh, [&](auto g) { each_listed(list, n, g); }, 0, st.above, st.target, 0);
-  }
-  const uint32_t t = sh.kmin;
-  uint32_t ties = sh.ties;
   const AsFixed w_of{st.M, r.c, st.shift};
+  const double target = st.target < 0 ? st.part : st.target;
+  uint32_t t, ties;
+  if (st.bin == BINS) {  // everything above the floor, and of its ties those that top-p's part still takes
+    t = st.floor_key;
+    ties = 0;
+    if (st.mode == BY_TOP_P) {
+      const uint64_t w = w_of(score_of(t));
+      const double room = target - (double)st.all;
+      ties = w == 0 || room > (double)w * (double)st.ties ? st.ties : (uint32_t)fmax(0.0, ceil(room / (double)w));
+      if (st.all == 0 && ties == 0) ties = 1;
+      ties = min(ties, st.ties);
+    }
+  } else {
+    const bool counts = st.mode == BY_TOP_K;
+    const uint32_t need = counts ? (uint32_t)(r.k - (int64_t)st.above) : 0;
+    if (n <= RANK) {
+      if ((int)threadIdx.x < n) sh.list[threadIdx.x] = list[threadIdx.x];
+      __syncthreads();
+      Slot s = rank_list(sh, n, need, 0);
+      if (!counts) cut_by_mass(s, st.above, target);
+      list_threshold(sh, s);
+    } else if (counts) {
+      split<BY_COUNT_WITH_MASS>(sh, [&](auto g) { each_listed(list, n, g); }, need, 0, 0.0, 0);
+    } else {
+      split<BY_MASS>(sh, [&](auto g) { each_listed(list, n, g); }, 0, st.above, target, 0);
+    }
+    t = sh.kmin;
+    ties = sh.ties;
+    if (counts && r.cut_p) {
+      // what top-k leaves: the bins above, the listed scores above t, the ties
+      uint64_t mine = 0, total;
+      for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS) mine += segmass[s];
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        const Entry e = list[i];
+        if (e.key() > t) mine += e.w;
+      }
+      block_scan(mine, sh.scan_m, total);
+      total += (uint64_t)ties * w_of(score_of(t));
+      for (int i = threadIdx.x; i < BINS; i += THREADS) a.hmass[(int64_t)b * BINS + i] = 0;
+      if (threadIdx.x == 0) {
+        RowState next = st;
+        const float range = st.M - score_of(t);
+        next.mode = BY_TOP_P;
+        next.cb = range > 0 && range < INFINITY ? (float)(BINS - 2) / range : 32.f;
+        next.floor_key = t;
+        next.ties = ties;
+        next.target = fmax(r.p, 0.0) * (double)total;
+        next.above = 0;
+        next.bin = 0;
+        next.listed = 0;
+        a.state[b] = next;
+      }
+      return;
+    }
+  }
   uint64_t wt = w_of(score_of(t));
   if (r.cut_min && weight(score_of(t), st.M, r.c) < r.minp) { wt = 0; ties = 0; }
   // Listed scores above t add to their segments' masses, ties are counted per segment: in LDS where
@@ -1368,7 +1461,10 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
     uint32_t* tied = (uint32_t*)sh.hm;
     static_assert(KEPT * 4 <= BINS * 8, "a tie count per segment");
     __syncthreads();
-    for (int s = threadIdx.x; s < a.nseg; s += THREADS) { more[s] = 0; tied[s] = 0; }
+    for (int s = threadIdx.x; s < a.nseg; s += THREADS) {
+      more[s] = 0;
+      tied[s] = st.bin == BINS && ties ? (uint32_t)a.segtie[(int64_t)b * a.nseg + s] : 0u;
+    }
     __syncthreads();
     add([&](int s, uint64_t w) { atomicAdd(more + s, (unsigned long long)w); }, [&](int s) { atomicAdd(tied + s, 1u); });
     __syncthreads();
@@ -1381,8 +1477,9 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
     // agent-scope accesses meet in the L2 that this one workgroup works through; the waits put the
     // zeros before the sums and the sums before the reads
     int32_t* segtie = a.segtie + (int64_t)b * a.nseg;
-    for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS)
-      __hip_atomic_store(segtie + s, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (st.bin < BINS)
+      for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS)
+        __hip_atomic_store(segtie + s, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     add([&](int s, uint64_t w) { atomicAdd((unsigned long long*)segmass + s, (unsigned long long)w); },
@@ -1403,7 +1500,7 @@ __global__ void __launch_bounds__(THREADS) finish_mass_kernel(Args a) {
 }
 
 template <int T>
-int run(Args& a, int passes, hipStream_t st) {
+int run(Args& a, int rounds, hipStream_t st) {
   if (a.nseg <= WAVES) {
     hipLaunchKernelGGL((finish_kernel<T, ROW_REGS>), dim3(a.B), dim3(THREADS), 0, st, a, 0);
   } else if (a.nseg <= CACHED_SEGS) {
@@ -1412,15 +1509,15 @@ int run(Args& a, int passes, hipStream_t st) {
     const int per = 4 * STAT_SEGS;
     hipLaunchKernelGGL((stats_kernel<T>), dim3((unsigned)((a.nseg + per - 1) / per), a.B), dim3(256), 0, st, a);
     FPS_CHECK_LAUNCH();
-    hipLaunchKernelGGL((finish_kernel<T, ROW_LONG>), dim3(a.B), dim3(THREADS), 0, st, a, passes);
-    if (passes) {
+    hipLaunchKernelGGL((finish_kernel<T, ROW_LONG>), dim3(a.B), dim3(THREADS), 0, st, a, rounds);
+    for (int i = 0; i < rounds; ++i) {
       FPS_CHECK_LAUNCH();
       const dim3 grid((unsigned)((a.nseg + PASS_SEGS - 1) / PASS_SEGS), a.B);
       hipLaunchKernelGGL((hist_kernel<T>), grid, dim3(THREADS), 0, st, a);
       FPS_CHECK_LAUNCH();
       hipLaunchKernelGGL((collect_kernel<T>), grid, dim3(THREADS), 0, st, a);
       FPS_CHECK_LAUNCH();
-      hipLaunchKernelGGL((finish_mass_kernel<T>), dim3(a.B), dim3(THREADS), 0, st, a);
+      hipLaunchKernelGGL((finish_passes_kernel<T>), dim3(a.B), dim3(THREADS), 0, st, a);
     }
   }
   FPS_CHECK_LAUNCH();
@@ -1463,7 +1560,7 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
   a.out = out; a.prob = prob;
   a.segmass = nullptr; a.hmass = nullptr; a.list = nullptr; a.state = nullptr; a.segmax = nullptr; a.segtie = nullptr;
   a.listcap = 0;
-  int passes = 0;
+  int rounds = 0;
   if (N > kShortRow) {
     if (ws == nullptr || ((uintptr_t)ws & 15)) return (int)hipErrorInvalidValue;
     a.listcap = list_cap(N);
@@ -1474,11 +1571,13 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
     a.segmass = (uint64_t*)p; p += (int64_t)B * a.nseg * 8;
     a.segmax = (float*)p; p += (int64_t)B * a.nseg * 4;
     a.segtie = (int32_t*)p;
-    // can a row cut by mass alone?  (scalars decide here, per-row settings on the device)
+    // which rounds of passes can a row need?  (scalars decide here, per-row settings on the device)
     const bool greedy = !temperature && !(temperature0 > 0);
-    const bool k = !top_k && top_k0 > 0 && top_k0 < N;
-    passes = !greedy && !k && (top_p || top_p0 < 1);
+    const bool can_long_k = !greedy && (top_k || (top_k0 > SHORT_K && top_k0 < N));
+    const bool can_no_k = !greedy && (top_k || top_k0 <= 0 || top_k0 >= N);
+    const bool can_p = top_p || top_p0 < 1, can_min = min_p || min_p0 > 0;
+    rounds = can_long_k && can_p ? 2 : can_long_k || (can_no_k && (can_p || can_min)) ? 1 : 0;
   }
   hipStream_t st = (hipStream_t)stream;
-  return type == T_F32 ? run<T_F32>(a, passes, st) : type == T_BF16 ? run<T_BF16>(a, passes, st) : run<T_F16>(a, passes, st);
+  return type == T_F32 ? run<T_F32>(a, rounds, st) : type == T_BF16 ? run<T_BF16>(a, rounds, st) : run<T_F16>(a, rounds, st);
 }

@@ -63,9 +63,9 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
     if u.dtype != torch.float32 or tuple(u.shape) != (B,) or not u.is_contiguous():
         raise ValueError(f"sample_scores: u must be contiguous fp32 [{B}], got {u.dtype} {tuple(u.shape)}")
     _same_device("sample_scores", S, u)
-    if n > 2**31 - 1 or (B > 65535 and n > 32768):
+    if n > 2**31 - 1 or (B > 65535 and n > 16384):
         raise ValueError(f"sample_scores: {B} rows of {n} scores: rows of up to 2^31 - 1, at most 65535 rows longer than "
-                         "32768")
+                         "16384")
     t, t0 = _setting("temperature", temperature, B, S, torch.float32, 0.0, math.inf)
     k, k0 = _setting("top_k", top_k, B, S, torch.int32, 0, 2**62)
     p, p0 = _setting("top_p", top_p, B, S, torch.float32, 0.0, 1.0)
@@ -83,7 +83,7 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
         if with_prob:
             prob.copy_(q)
     elif B:
-        size = N.require().fps_sample_scores_ws_bytes(B, n) if n > 32768 else 0
+        size = N.require().fps_sample_scores_ws_bytes(B, n) if n > 16384 else 0
         ws = torch.empty(size, dtype=torch.uint8, device=S.device) if size else None
         _launch("sample_scores", S.get_device(), S.data_ptr(), _TYPE[S.dtype], B, n, S.stride(0) if B > 1 else n,
                 u.data_ptr(), N.ptr(t), t0, N.ptr(k), k0, N.ptr(p), p0, N.ptr(m), m0, out.data_ptr(), N.ptr(prob),

@@ -87,7 +87,9 @@ def scores(B, n, seed, spread=3.0, masked=0.1, dtype=torch.float32):
 SETTINGS = [dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=5), dict(top_k=40, top_p=0.9),
             dict(top_p=0.5), dict(top_p=0.95, temperature=1.5), dict(min_p=0.1), dict(top_k=700, top_p=0.99),
             dict(top_k=20, top_p=0.8, min_p=0.05, temperature=0.5), dict(top_p=0.9, min_p=0.3), dict(temperature=0.0),
-            dict(temperature=50.0, top_p=0.7), dict(temperature=0.01, top_k=30), dict(top_k=10**9), dict(top_p=0.0)]
+            dict(temperature=50.0, top_p=0.7), dict(temperature=0.01, top_k=30), dict(top_k=10**9), dict(top_p=0.0),
+            dict(top_k=9000), dict(top_k=9000, top_p=0.97, min_p=0.001), dict(top_k=15000, top_p=0.3), dict(min_p=1e-4),
+            dict(top_k=9000, min_p=0.02, temperature=2.0), dict(top_k=300, top_p=0.5, temperature=30.0)]
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -116,10 +118,12 @@ def test_settings_per_row(dev, n):
     check(S, u, dev, temperature=[1, 0, 0.5, 2, 1, 1, -1, 1, 0.1, 30, 1, 1],
           top_k=[0, 3, 10, 0, n, 4, 9, -2, 600, 0, 1, 100], top_p=[1, 0.5, 0.9, 0.8, 0.99, 0.5, 0.5, 2, 0.7, 0.6, 0.9, 0.0],
           min_p=[0, 0, 0.1, 0, 0.01, 0.5, 0, -1, 0, 0.2, 0, 5.0])
+    check(S, u, dev, top_k=[n // 2, 0, 700, n // 3, 5, 0, n // 2, 2000, 0, 900, 4000, n - 1],
+          top_p=[0.9, 0.9, 1, 0.2, 0.9, 0.3, 1, 0.999, 1, 0.7, 0.0, 0.95], min_p=[0, 0, 0, 0, 0, 0, 0.01, 0, 0.2, 0.1, 0, 0])
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("n", [8, 1000, 5000, 40000])
+@pytest.mark.parametrize("n", [8, 1000, 5000, 40000, 200000])
 def test_equal_scores_go_by_index(dev, n):
     """Every weight is 1: borders are whole numbers, exact on every side."""
     S = torch.full((6, n), 2.5)
@@ -130,8 +134,13 @@ def test_equal_scores_go_by_index(dev, n):
     assert int(i.max()) < k
     i = check(S, u, dev, near_ok=True, top_p=0.25)
     assert int(i.max()) < n // 4  # n is a multiple of 4: the border itself is cut
+    i = check(S, u, dev, near_ok=True, top_k=n - n // 4, top_p=0.5)
+    assert int(i.max()) < (n - n // 4) // 2
     check(S, u, dev, near_ok=True, top_k=k, top_p=0.5, min_p=1.0)
     S[:, ::2] = 1.0
+    # top-k takes all of the better half and some ties, top-p ends above them, among them, at them
+    for p in (0.25, 0.5, 0.75, 0.875):
+        check(S, u, dev, near_ok=True, top_k=n // 2 + n // 8, top_p=p, temperature=1e9)
     check(S, u, dev, near_ok=True, temperature=0.0)
     check(S, u, dev, near_ok=True, top_k=3)
     S[:] = 0.0
@@ -140,7 +149,7 @@ def test_equal_scores_go_by_index(dev, n):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("n", [10, 3000, 36000])
+@pytest.mark.parametrize("n", [10, 3000, 9000, 36000])
 def test_masks_infinities_and_nan(dev, n):
     S, u = scores(9, n, seed=3 * n, masked=0)
     S[0] = -INF
@@ -155,7 +164,7 @@ def test_masks_infinities_and_nan(dev, n):
     S[8] = -INF
     S[8, 2] = torch.finfo(torch.float32).min
     for kw in (dict(), dict(top_k=2), dict(top_p=0.6), dict(top_k=4, top_p=0.5, min_p=0.01), dict(temperature=0.0),
-               dict(min_p=0.5), dict(top_k=n - 1, top_p=0.9)):
+               dict(min_p=0.5), dict(top_k=n - 1, top_p=0.9), dict(top_k=n // 2, top_p=0.7), dict(top_k=n // 2)):
         check(S, u, dev, near_ok=True, **kw)
 
 
