@@ -189,6 +189,55 @@ __device__ __forceinline__ void store_scores(char* at, bool whole, int left, con
   }
 }
 
+// acc += one chunk: this lane's S blocks of cur by the queries' blocks first .. first + S - 1 in LDS
+template <int XB, bool Q4, int QT, int IT, int CS, int STRIDE, int SSTRIDE>
+__device__ __forceinline__ void multiply(const uint8_t* qrow, const uint8_t* qsrow, int first, int S,
+                                         const Chunk<XB, IT, CS>& cur, f32x16 (&acc)[IT][QT]) {
+#pragma unroll
+        for (int j = 0; j < CS; ++j) {
+          if (j < S) {
+            if constexpr (Q4) {
+              i32x8 qa[QT];
+              int qsc[QT];
+#pragma unroll
+              for (int q = 0; q < QT; ++q) {
+                const uint4 v = *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 16);
+                qa[q] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+                qsc[q] = qsrow[q * 32 * SSTRIDE + first + j];
+              }
+#pragma unroll
+              for (int t = 0; t < IT; ++t) {
+                const uint4 v = cur.b[t][j].v;
+                const i32x8 xb = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+#pragma unroll
+                for (int q = 0; q < QT; ++q)
+                  acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
+                                                                              (int)(cur.s[t] >> (8 * j)));
+              }
+            } else {
+              float f[IT];
+#pragma unroll
+              for (int t = 0; t < IT; ++t) {
+                const uint32_t s = (cur.s[t] >> (8 * j)) & 255u;
+                f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
+              }
+#pragma unroll
+              for (int s = 0; s < 4; ++s) {
+                bf16x8 xb[IT];
+#pragma unroll
+                for (int t = 0; t < IT; ++t) xb[t] = to_bf16(cur.b[t][j], s, f[t]);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                  const bf16x8 qa = __builtin_bit_cast(bf16x8, *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 64 + s * 16));
+#pragma unroll
+                  for (int t = 0; t < IT; ++t) acc[t][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, xb[t], acc[t][q], 0, 0, 0);
+                }
+              }
+            }
+          }
+        }
+}
+
 // LB: blocks of a query held in LDS
 template <int XB, bool Q4, int QT, int IT, int CS, int LB, int T>
 __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
@@ -256,49 +305,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
         }
       }
       const int S = chunk_s<CS>(a.nblk, c0), first = (once ? c0 : half * KC) + h * S;
-#pragma unroll
-      for (int j = 0; j < CS; ++j) {
-        if (j < S) {
-          if constexpr (Q4) {
-            i32x8 qa[QT];
-            int qsc[QT];
-#pragma unroll
-            for (int q = 0; q < QT; ++q) {
-              const uint4 v = *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 16);
-              qa[q] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-              qsc[q] = qsrow[q * 32 * SSTRIDE + first + j];
-            }
-#pragma unroll
-            for (int t = 0; t < IT; ++t) {
-              const uint4 v = cur.b[t][j].v;
-              const i32x8 xb = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-#pragma unroll
-              for (int q = 0; q < QT; ++q)
-                acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
-                                                                            (int)(cur.s[t] >> (8 * j)));
-            }
-          } else {
-            float f[IT];
-#pragma unroll
-            for (int t = 0; t < IT; ++t) {
-              const uint32_t s = (cur.s[t] >> (8 * j)) & 255u;
-              f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              bf16x8 xb[IT];
-#pragma unroll
-              for (int t = 0; t < IT; ++t) xb[t] = to_bf16(cur.b[t][j], s, f[t]);
-#pragma unroll
-              for (int q = 0; q < QT; ++q) {
-                const bf16x8 qa = __builtin_bit_cast(bf16x8, *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 64 + s * 16));
-#pragma unroll
-                for (int t = 0; t < IT; ++t) acc[t][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, xb[t], acc[t][q], 0, 0, 0);
-              }
-            }
-          }
-        }
-      }
+      multiply<XB, Q4, QT, IT, CS, STRIDE, SSTRIDE>(qrow, qsrow, first, S, cur, acc);
       if (CS > 1 && !once && more) {
 #pragma unroll
         for (int i = 0; i < QREGS; ++i) {
@@ -330,6 +337,89 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
         }
     }
   }
+}
+
+// Few tiles and long rows: the four waves of a workgroup take the same 64 table rows and every fourth chunk
+// each, and their sums are joined in LDS.  (The rule, with both sides measured, is where it is launched.)
+template <int XB, bool Q4, int T>
+__global__ void __launch_bounds__(THREADS, 2) mx_score_split_kernel(Args a) {
+  constexpr int QT = 1, IT = 2, CS = 2, KC = 2 * CS, LB = WAVES * KC;
+  constexpr int QBYTES = Q4 ? 16 : 64, CB = QBYTES / 16;
+  constexpr int STRIDE = LB * QBYTES + 16, SSTRIDE = LB + 4;
+  constexpr int QL = 32 * QT * STRIDE, RED = WAVES * 32 * QT * 64 * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t ql[QL > RED ? QL : RED];
+  __shared__ __attribute__((aligned(16))) uint8_t qsl[Q4 ? 32 * QT * SSTRIDE : 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int tile = xcd_remap(blockIdx.x, a.qtiles * a.itiles);
+  const int q0 = tile % a.qtiles * 32 * QT;
+  const int64_t row0 = (int64_t)(tile / a.qtiles) * (32 * IT) + (lane & 31) * IT;
+  const uint8_t* qrow = ql + (lane & 31) * STRIDE;
+  const uint8_t* qsrow = qsl + (lane & 31) * SSTRIDE;
+  f32x16 acc[IT][QT];
+#pragma unroll
+  for (int t = 0; t < IT; ++t)
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][q][r] = 0.f;
+  Chunk<XB, IT, CS> cur, nxt;
+  const int c1 = wave * KC;
+  if (c1 < a.nblk) load_chunk<XB, IT, CS>(a, row0, c1, h, cur);
+  for (int s0 = 0; s0 < a.nblk; s0 += LB) {
+    const int c0 = s0 + c1;
+    if (c0 + LB < a.nblk) load_chunk<XB, IT, CS>(a, row0, c0 + LB, h, nxt);
+    __syncthreads();
+#pragma unroll 4
+    for (int e = threadIdx.x; e < 32 * QT * LB * CB; e += THREADS) {
+      const int r = e / (LB * CB), c = e % (LB * CB);
+      *(uint4*)(ql + r * STRIDE + c * 16) = load_piece<Q4>(a, q0 + r, s0 + c / CB, c % CB);
+      if (Q4) qsl[r * SSTRIDE + c] = load_qscale(a, q0 + r, s0 + c);
+    }
+    __syncthreads();
+    if (c0 < a.nblk) {
+      const int S = chunk_s<CS>(a.nblk, c0);
+      multiply<XB, Q4, QT, IT, CS, STRIDE, SSTRIDE>(qrow, qsrow, c1 + h * S, S, cur, acc);
+    }
+    cur = nxt;
+  }
+  __syncthreads();
+  float* red = (float*)ql;
+#pragma unroll
+  for (int t = 0; t < IT; ++t)
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) red[((wave * IT + t) * QT + q) * 1024 + r * 64 + lane] = acc[t][q][r];
+  __syncthreads();
+  // wave w joins registers 4 w .. 4 w + 3: queries 8 w + (0 .. 3) + 4 h of each 32
+  constexpr int ES = T == T_F32 ? 4 : 2;
+  const int left = (int)min(a.N - row0, (int64_t)IT);
+  const bool whole = a.vec && left == IT;
+  if (left <= 0) return;
+#pragma unroll
+  for (int q = 0; q < QT; ++q)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = q0 + q * 32 + 8 * wave + i + 4 * h;
+      float v[IT];
+#pragma unroll
+      for (int t = 0; t < IT; ++t) {
+        const float* p = red + (t * QT + q) * 1024 + (4 * wave + i) * 64 + lane;
+        v[t] = (p[0] + p[IT * QT * 1024]) + (p[2 * IT * QT * 1024] + p[3 * IT * QT * 1024]);
+      }
+      if (b < a.B) store_scores<T, IT>((char*)a.out + ((int64_t)b * a.ld + row0) * ES, whole, left, v);
+    }
+}
+
+template <int XB, bool Q4>
+void launch_split(Args& a, int type, hipStream_t st) {
+  a.vec = (a.B == 1 || a.ld % 2 == 0) && ((uintptr_t)a.out & (type == T_F32 ? 7 : 3)) == 0;
+  a.qtiles = (a.B + 31) / 32;
+  a.itiles = (int)((a.N + 63) / 64);
+  const dim3 grid((unsigned)(a.qtiles * a.itiles));
+  if (type == T_F32) hipLaunchKernelGGL((mx_score_split_kernel<XB, Q4, T_F32>), grid, dim3(THREADS), 0, st, a);
+  else if (type == T_BF16) hipLaunchKernelGGL((mx_score_split_kernel<XB, Q4, T_BF16>), grid, dim3(THREADS), 0, st, a);
+  else hipLaunchKernelGGL((mx_score_split_kernel<XB, Q4, T_F16>), grid, dim3(THREADS), 0, st, a);
 }
 
 template <int XB, bool Q4, int QT, int IT, int CS, int LB, int T>
@@ -521,6 +611,16 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
   a.s_word = a.nblk % 4 == 0 && ((uintptr_t)xs & 3) == 0;
   hipStream_t st = (hipStream_t)stream;
   const bool few = B <= 32, narrow = a.nblk <= 2;
+  // Few queries, long rows and too few rows to give every CU its 256: the waves split the row instead.  (us, whole
+  // rows against split: 1000 x 4096 fp4 38.8 / 20.1, fp8 71.5 / 22.8, 30000 x 4096 fp4 44.7 / 29.8,
+  // 20000 x 1024 fp4 13.8 / 11.5; 65536 x 4096 fp4 46.4 / 42.7 but fp8 92 / 102, 130000 x 2048 fp4 29.9 / 44.9.)
+  if (few && a.nblk >= 16 && N <= 160 * 256) {
+    if (qs) launch_split<4, true>(a, out_type, st);
+    else if (xbits == 4) launch_split<4, false>(a, out_type, st);
+    else launch_split<8, false>(a, out_type, st);
+    FPS_CHECK_LAUNCH();
+    return 0;
+  }
   if (qs) {
     if (narrow) { if (few) launch<4, true, 1, 2, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
     else if (a.B > 64 && a.nblk > 16 && a.s_word) launch_wide(a, out_type, st);
