@@ -621,10 +621,17 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
     FPS_CHECK_LAUNCH();
     return 0;
   }
+  // Otherwise by the width of the rows and the number of queries.  narrow (one or two blocks a row): one block a
+  // lane, four table rows a lane so that a store of many queries' scores is 256 bytes long, two rows where
+  // there are few queries (more waves in flight: 13.7 -> 11.6 us for one query, 1M x 64).  Longer rows:
+  // chunks of 4 (fp4) or 2 (fp8) blocks a lane.  QT = 2 query tiles a wave is what the registers hold
+  // beside them (QT = 4, spilling: 417 us for 512 x 65536 x 4096 in fp4, 351 so).  Both sides in 4
+  // bits and rows long enough to amortise it: the tiled form (us, wide against QT = 2 here: 64 x 65536 x
+  // 4096 50 / 76; rows of 1000 values and 100 queries: equal).
   if (qs) {
     if (narrow) { if (few) launch<4, true, 1, 2, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
-    else if (a.B > 64 && a.nblk > 16 && a.s_word) launch_wide(a, out_type, st);
-    else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 4, 2, 2, 16>(a, out_type, st); }
+    else if (!few && a.nblk > 16 && a.s_word) launch_wide(a, out_type, st);
+    else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 2, 2, 4, 16>(a, out_type, st); }
   } else if (xbits == 4) {
     if (narrow) { if (few) launch<4, false, 1, 2, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
     else { if (few) launch<4, false, 1, 2, 4, 32>(a, out_type, st); else launch<4, false, 2, 2, 4, 16>(a, out_type, st); }
