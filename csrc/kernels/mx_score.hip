@@ -339,8 +339,9 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   }
 }
 
-// Few tiles and long rows: the four waves of a workgroup take the same 64 table rows and every fourth chunk
-// each, and their sums are joined in LDS.  (The rule, with both sides measured, is where it is launched.)
+// Few tiles and long rows: the four waves of a workgroup take the same 64 table rows and every fourth
+// chunk each, and their sums are joined in LDS.  (The rule, with both sides measured, is where it is
+// launched.)
 template <int XB, bool Q4, int T>
 __global__ void __launch_bounds__(THREADS, 2) mx_score_split_kernel(Args a) {
   constexpr int QT = 1, IT = 2, CS = 2, KC = 2 * CS, LB = WAVES * KC;
@@ -456,10 +457,12 @@ void launch(Args& a, int type, hipStream_t st) {
 typedef __attribute__((address_space(3))) uint8_t LdsByte;
 // 16 bytes a lane from base + off to LDS, lane after lane from byte `to` on.  In assembly because the
 // compiler waits for every such load of its own before the next read of LDS, whichever buffer that
-// is of; here wait_loads() does, before the barrier that hands the buffer over.  (m0, the
-// destination, is not in use by anything else in this kernel; nothing is returned in registers.)
+// is of; here wait_loads() does, before the barrier that hands the buffer over.  (m0 holds the
+// destination; a load to LDS may read it one wait state after it is written, and the compiler puts
+// none inside a block.  Nothing is returned in registers.)
 __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base)
+               : "memory", "m0");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -591,17 +594,15 @@ void launch_wide(Args& a, int type, hipStream_t st) {
   else hipLaunchKernelGGL((mx_score_wide_kernel<T_F16>), grid, dim3(WTHREADS), 0, st, a);
 }
 
-}  // namespace
+// A launch's threads must fit 32 bits: so many queries a launch (the smallest tile is 32 queries by 256
+// rows), 256 at least (with the rows that fit in memory, fewer tiles than that).
+int64_t queries_per_launch(int64_t N) {
+  const int64_t tiles = (int64_t)UINT32_MAX / WTHREADS, per = tiles / ((N + 255) / 256) * 32 / 256 * 256;
+  return min((int64_t)1 << 20, max((int64_t)256, per));
+}
 
-// out [B, N] (row stride ld, type 0 fp32 / 1 bf16 / 2 fp16) = q . x^T.  qs == nullptr: q is bf16
-// [B, D]; else q holds E2M1 blocks and qs their scales (then xbits must be 4).
-FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const void* xs, int xbits, int B, int64_t N,
-                         int D, void* out, int out_type, int64_t ld, void* stream) {
-  if (B <= 0 || N <= 0) return 0;
-  if (D <= 0 || (xbits != 4 && xbits != 8) || (qs && xbits != 4) || ld < N || out_type < 0 || out_type > 2)
-    return (int)hipErrorInvalidValue;
-  if (N > (int64_t)INT32_MAX * 32 || (int64_t)((B + 31) / 32) * ((N + 255) / 256) > INT32_MAX)
-    return (int)hipErrorInvalidValue;
+int score(const void* q, const void* qs, const void* x, const void* xs, int xbits, int B, int64_t N, int D, void* out,
+          int out_type, int64_t ld, hipStream_t st) {
   Args a;
   a.q = q; a.qs = (const uint8_t*)qs; a.x = (const uint8_t*)x; a.xs = (const uint8_t*)xs;
   a.out = out; a.ld = ld; a.N = N; a.B = B; a.D = D;
@@ -609,7 +610,6 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
   const uintptr_t qp = (uintptr_t)q | (uintptr_t)(2 * D);  // D even, a multiple of 4, of 8
   a.q_align = qp & 2 ? 2 : qp & 4 ? 4 : qp & 8 ? 8 : 16;
   a.s_word = a.nblk % 4 == 0 && ((uintptr_t)xs & 3) == 0;
-  hipStream_t st = (hipStream_t)stream;
   const bool few = B <= 32, narrow = a.nblk <= 2;
   // Few queries, long rows and too few rows to give every CU its 256: the waves split the row instead.  (us, whole
   // rows against split: 1000 x 4096 fp4 38.8 / 20.1, fp8 71.5 / 22.8, 30000 x 4096 fp4 44.7 / 29.8,
@@ -627,10 +627,11 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
   // chunks of 4 (fp4) or 2 (fp8) blocks a lane.  QT = 2 query tiles a wave is what the registers hold
   // beside them (QT = 4, spilling: 417 us for 512 x 65536 x 4096 in fp4, 351 so).  Both sides in 4
   // bits and rows long enough to amortise it: the tiled form (us, wide against QT = 2 here: 64 x 65536 x
-  // 4096 50 / 76; rows of 1000 values and 100 queries: equal).
+  // 4096 50 / 76; rows of 1000 values and 100 queries: equal); its scales are read in words, and its
+  // offsets within a tile's 256 rows are 32-bit ones.
   if (qs) {
     if (narrow) { if (few) launch<4, true, 1, 2, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
-    else if (!few && a.nblk > 16 && a.s_word) launch_wide(a, out_type, st);
+    else if (!few && a.nblk > 16 && a.nblk < (1 << 20) && a.s_word && ((uintptr_t)qs & 3) == 0) launch_wide(a, out_type, st);
     else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 2, 2, 4, 16>(a, out_type, st); }
   } else if (xbits == 4) {
     if (narrow) { if (few) launch<4, false, 1, 2, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
@@ -640,5 +641,27 @@ FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const voi
     else { if (few) launch<8, false, 1, 2, 2, 32>(a, out_type, st); else launch<8, false, 2, 2, 2, 16>(a, out_type, st); }
   }
   FPS_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // namespace
+
+// out [B, N] (row stride ld, type 0 fp32 / 1 bf16 / 2 fp16) = q . x^T.  qs == nullptr: q is bf16
+// [B, D]; else q holds E2M1 blocks and qs their scales (then xbits must be 4).
+FPS_API int fps_mx_score(const void* q, const void* qs, const void* x, const void* xs, int xbits, int B, int64_t N,
+                         int D, void* out, int out_type, int64_t ld, void* stream) {
+  if (B <= 0 || N <= 0) return 0;
+  if (D <= 0 || D > INT32_MAX - MX_BLOCK || (xbits != 4 && xbits != 8) || (qs && xbits != 4) || ld < N || out_type < 0 ||
+      out_type > 2)
+    return (int)hipErrorInvalidValue;
+  if (N > (int64_t)INT32_MAX * 32) return (int)hipErrorInvalidValue;
+  const int64_t per = queries_per_launch(N);
+  const int64_t nblk = (D + MX_BLOCK - 1) / MX_BLOCK, q_bytes = qs ? nblk * 16 : (int64_t)D * 2;
+  for (int64_t b = 0; b < B; b += per) {
+    const int rc = score((const char*)q + b * q_bytes, qs ? (const char*)qs + b * nblk : nullptr, x, xs, xbits,
+                         (int)min(per, B - b), N, D, (char*)out + b * ld * (out_type == T_F32 ? 4 : 2), out_type, ld,
+                         (hipStream_t)stream);
+    if (rc) return rc;
+  }
   return 0;
 }

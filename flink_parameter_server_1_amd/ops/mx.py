@@ -10,8 +10,9 @@ power of two (an E8M0 byte ``s``, value ``2^(s - 127)``, 255 = NaN):
 The shared exponent is the largest magnitude's less the element format's largest
 (``floor(log2 max|x|) - 2`` or ``- 8``), elements are rounded to nearest even and saturated.
 A block that holds an infinity or a NaN reads back as NaN.  Every read of an element is
-exact in fp32 (and in bf16), so the only rounding is the write's: half an element step,
-``eps / 2`` of the element type relative to a value that does not saturate.
+exact in fp32 (and in bf16 down to its smallest normal number), so the only rounding is the
+write's: half an element step, ``eps / 2`` of the element type relative to a value that does
+not saturate.
 
 Dispatch is by the table's device as for every op: the gfx950 kernels on a GPU, the plain
 PyTorch twin (``ops.reference``) on the CPU.  Nothing here is differentiated: tables are
@@ -230,7 +231,7 @@ def mx_score(Q, X: MXTable, out: Optional[torch.Tensor] = None, out_dtype=torch.
         return out
     if not out.is_cuda:
         q = R.mx_decode(Q.data, Q.scale, Q.bits, dim) if mx else Q.float()
-        out.copy_(q @ R.mx_decode(X.data, X.scale, X.bits, dim).t())
+        out.copy_(q.detach() @ R.mx_decode(X.data, X.scale, X.bits, dim).t())
         return out
     ld = out.stride(0) if B > 1 else X.rows
     _launch("mx_score", out.get_device(), Q.data.data_ptr() if mx else Q.data_ptr(), Q.scale.data_ptr() if mx else None,

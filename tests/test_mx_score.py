@@ -128,6 +128,34 @@ def test_refusals(dev):
             f()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("B", [9, 70])
+def test_scales_at_any_address(dev, form, B):
+    """Tables wrapped over buffers whose scale bytes start off four bytes."""
+    Q, X = operands(B, 300, 1024, form, dev, seed=21)
+
+    def moved(t):
+        buf = torch.zeros(t.scale.numel() + 1, dtype=torch.uint8, device=dev)
+        buf[1:] = t.scale.flatten()
+        return ops.MXTable.wrap(t.data, buf[1:].view(t.scale.shape), t.dim, t.fmt)
+
+    check(ops.mx_score(Q, moved(X)), Q, X)
+    if form[0] == "fp4":
+        check(ops.mx_score(moved(Q), X), Q, X)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_more_queries_than_a_launch_takes(form):
+    B = (1 << 20) + 77
+    Q, X = operands(B, 70, 40, form, "cuda", seed=22)
+    S = ops.mx_score(Q, X)
+    for a, b in ((0, 300), ((1 << 20) - 100, B)):
+        part = Q[a:b].contiguous() if form[0] == "bf16" else ops.MXTable.wrap(Q.data[a:b], Q.scale[a:b], 40)
+        check(S[a:b], part, X)
+
+
 @pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A score matrix of more than 2^32 bytes and 2^31 entries, a table of more than 2^31 bytes."""
