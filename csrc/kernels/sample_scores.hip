@@ -55,9 +55,9 @@ __device__ __forceinline__ Entry make_entry(uint32_t key, int32_t idx, uint64_t 
   return Entry{(uint64_t)key << 32 | (uint32_t)~idx, w};
 }
 
-// What the passes over a long row share.  A round finds one threshold: by count (top-k), or by mass (top-p)
-// among the scores above `floor_key` and the first `ties` equal to it (what top-k left); or none (NO_CUT),
-// for the segments' masses alone.
+// What the passes over a long row share.  A round finds one threshold: by count (top-k), or by mass
+// (top-p) among the scores above `floor_key` and the first `ties` equal to it (what top-k left); or none
+// (NO_CUT), for the segments' masses alone.
 enum { IDLE = 0, BY_TOP_K = 1, BY_TOP_P = 2, NO_CUT = 3 };
 struct RowState {
   int mode;
@@ -111,7 +111,7 @@ __device__ __forceinline__ Row row_settings(const Args& a, int b) {
   r.k = a.top_k ? (int64_t)a.top_k[b] : a.top_k0;
   r.p = a.top_p ? (double)a.top_p[b] : a.top_p0;
   r.minp = a.min_p ? (double)a.min_p[b] : a.min_p0;
-  r.c = 1.4426950408889634 / T;
+  r.c = fmin(1.4426950408889634 / T, 1e300);  // finite: 0 * c is 0 at the best score
   if (!(T > 0)) {  // greedy: the best alone
     r.c = 1.4426950408889634;
     r.k = 1;
@@ -1199,9 +1199,9 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     }
     __syncthreads();
     find_bin<BY_COUNT>(sh, (uint32_t)r.k);
-    // fewer unmasked than k: everything unmasked is a candidate
-    // A score a little below the last of those bins (fp32 rounds M - s and its product by 2^-23 or so: a few
-    // candidates more do no harm), so that a score takes one comparison.
+    // Candidates are the scores above one a little below the last of those bins, so that each takes one
+    // comparison (fp32 rounds M - s and its product by 2^-23 or so: a few candidates more do no harm).
+    // Fewer unmasked than k: everything unmasked.
     const bool all = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k || sh.bin == BINS - 1 || !(M < INFINITY);
     const double low = (double)M - (double)(sh.bin + 1) / (double)cb * (1 + 1e-6) - fabs((double)M) * 1e-6;
     const float cut = all ? -INFINITY : (float)low;
@@ -1230,7 +1230,8 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   finish_general<T, R>(a, b, src, sh, r, M, segmass, segtie);
 }
 
-// ---- a round of passes over long rows: counts or masses by bin, then what lies above the threshold's bin and in it, then the threshold
+// ---- a round of passes over long rows: counts or masses by bin, then what lies above the threshold's
+// bin and in it, then the threshold
 
 template <int T>
 __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
@@ -1362,8 +1363,8 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   for (int i = threadIdx.x; i < n; i += THREADS) put((uint32_t)(count + i), listed[i]);
 }
 
-// The threshold inside the listed bin; then the draw over whole-number masses, or, after top-k where top-p
-// is to follow, the state of a second round.
+// The threshold inside the listed bin; then the draw over whole-number masses, or, after top-k where
+// top-p is to follow, the state of a second round.
 template <int T>
 __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
   __shared__ Shared sh;
@@ -1526,6 +1527,7 @@ int run(Args& a, int rounds, hipStream_t st) {
 }
 
 constexpr int64_t kShortRow = (int64_t)CACHED_SEGS * SEG;  // rows up to this take no workspace
+constexpr int LAUNCH_ROWS = 1 << 22;  // of those, so many at most a launch (its threads must fit 32 bits)
 
 int list_cap(int64_t N) { return (int)(N / 8 < 16384 ? N / 8 : 16384); }
 
@@ -1580,5 +1582,22 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
     rounds = can_long_k && can_p ? 2 : can_long_k || (can_no_k && (can_p || can_min)) ? 1 : 0;
   }
   hipStream_t st = (hipStream_t)stream;
-  return type == T_F32 ? run<T_F32>(a, rounds, st) : type == T_BF16 ? run<T_BF16>(a, rounds, st) : run<T_F16>(a, rounds, st);
+  const auto launch = [&] {
+    return type == T_F32 ? run<T_F32>(a, rounds, st) : type == T_BF16 ? run<T_BF16>(a, rounds, st) : run<T_F16>(a, rounds, st);
+  };
+  if (B <= LAUNCH_ROWS) return launch();
+  for (int64_t b = 0; b < B; b += LAUNCH_ROWS) {
+    a.B = (int)(B - b < LAUNCH_ROWS ? B - b : LAUNCH_ROWS);
+    a.s = (const char*)s + b * ld * (type == T_F32 ? 4 : 2);
+    a.u = u + b;
+    a.temperature = temperature ? temperature + b : nullptr;
+    a.top_k = top_k ? top_k + b : nullptr;
+    a.top_p = top_p ? top_p + b : nullptr;
+    a.min_p = min_p ? min_p + b : nullptr;
+    a.out = out + b;
+    a.prob = prob ? prob + b : nullptr;
+    const int rc = launch();
+    if (rc) return rc;
+  }
+  return 0;
 }

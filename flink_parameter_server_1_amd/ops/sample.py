@@ -77,7 +77,7 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
         if with_prob:
             prob.zero_()
     elif B and not S.is_cuda:
-        i, q = R.sample_scores(S, u, t0 if t is None else t, k0 if k is None else k, p0 if p is None else p,
+        i, q = R.sample_scores(S.detach(), u, t0 if t is None else t, k0 if k is None else k, p0 if p is None else p,
                                m0 if m is None else m)
         out.copy_(i)
         if with_prob:
