@@ -75,7 +75,7 @@ struct RowState {
 struct Args {
   const void* s;
   int64_t ld, N, nseg;
-  int B, vec;
+  int B;
   const float* u;
   // per row, or nullptr and the same for all rows
   const float* temperature; double temperature0;
@@ -134,8 +134,7 @@ __device__ __forceinline__ float score_of(uint32_t k) {
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // key_of(-inf)
 
 // p f + c with the coefficient in scalar registers (the compiler's form copies each coefficient
-// into vector registers first: the weights of a pass over 16.7M scores took 32 us against
-// 27)
+// into vector registers first: 5 us of a pass over 16.7M scores that takes 27 so)
 __device__ __forceinline__ double horner(double p, double f, double c) {
   double r;
   asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(p), "v"(f), "s"(c));
@@ -144,13 +143,14 @@ __device__ __forceinline__ double horner(double p, double f, double c) {
 
 // 2^((s - M) c): interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 8 (relative
 // error 1.1e-12: two answers differ where u * total falls that near to a step), times the
-// power of two.  n = round(t) is read from the low bits of t + 1.5 * 2^52.
+// power of two, which vanishes by itself at the clamp.  (Built from the bits of t + 1.5 * 2^52, with a
+// comparison for what is too small, a pass over 16.7M scores took 28.5 us against 26.)
 __device__ __forceinline__ double weight(float s, float M, double c) {
   if (M == INFINITY) return s == M ? 1.0 : 0.0;  // (one branch for a whole row)
   const double t0 = ((double)s - (double)M) * c;  // exactly 0 at the best score
-  const double t = fmax(t0, -1020.0);
-  const double u = t + 6755399441055744.0;
-  const double f = t - (u - 6755399441055744.0);
+  const double t = fmax(t0, -2000.0);  // (a NaN too: a masked score at an endless temperature)
+  const double n = __builtin_rint(t);
+  const double f = t - n;
   double p = 0x1.63d1363a7ecb6p-20;
   p = horner(p, f, 0x1.00dc4a534054dp-16);
   p = horner(p, f, 0x1.4308ac85a6c21p-13);
@@ -160,8 +160,7 @@ __device__ __forceinline__ double weight(float s, float M, double c) {
   p = horner(p, f, 0x1.ebfbdff823cedp-3);
   p = horner(p, f, 0x1.62e42fef84cf0p-1);
   p = horner(p, f, 0x1.0000000000000p+0);
-  const double w = __longlong_as_double(__double_as_longlong(p) + ((__double_as_longlong(u) << 52)));
-  return t0 > -1020.0 ? w : 0.0;
+  return __builtin_ldexp(p, (int)n);
 }
 
 // w in [0, 1] as a whole multiple of 2^-shift, shift <= 51 (rounded to nearest even)
@@ -175,51 +174,86 @@ __device__ __forceinline__ int shift_for(double total) {
   return min(51, 61 - (int)((__double_as_longlong(total) >> 52) - 1023));
 }
 
+// (the median of three with a NaN is the smallest of the others, and a NaN is made by s = M alone, with an
+// infinite M or cb, or by all scores alike, with cb = 0)
 __device__ __forceinline__ int bin_of(float s, float M, float cb) {
-  const float x = fminf((M - s) * cb, (float)(BINS - 1));
-  return s == M ? 0 : (int)x;
+  return (int)__builtin_amdgcn_fmed3f((M - s) * cb, 0.f, (float)(BINS - 1));
 }
 
-template <int T>
-__device__ __forceinline__ float load1(const void* p, int64_t i) {
-  if (T == T_F32) return ((const float*)p)[i];
-  const uint16_t b = ((const uint16_t*)p)[i];
-  return T == T_BF16 ? bf16_to_f32(b) : __half2float(__ushort_as_half(b));
-}
+// loads of four scores: a row may start at any score
+typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(2)));
 
 // NaN is masked; -0 and +0 are one score
-__device__ __forceinline__ float clean(float f) { return f == f ? f + 0.f : -INFINITY; }
+__device__ __forceinline__ float clean(float f) { return fmaxf(f + 0.f, -INFINITY); }
 
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// this lane's four scores of a segment as they lie in memory; places past the row are masked
-template <int T>
-__device__ __forceinline__ void load_raw(const Args& a, int b, int64_t seg, int lane, float v[4]) {
-  const int64_t i = seg * SEG + lane * 4, at = (int64_t)b * a.ld + i;
-  if (a.vec && (seg + 1) * SEG <= a.N) {  // (one branch for the wave)
-    if (T == T_F32) {
-      const float4 f = *(const float4*)((const float*)a.s + at);
-      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else {
-      const uint2 u = *(const uint2*)((const uint16_t*)a.s + at);
-      const uint32_t w[2] = {u.x, u.y};
+// This lane's four scores of a segment as they lie in memory; places past the row are masked.  They are
+// unpacked where they are used, and a wave takes one branch for a group of segments: converted at once,
+// or with a branch for each, a load would be waited for before the next is sent (16.7M bf16 scores:
+// stats pass 12 us against STATS, histogram 24 against HIST).
+template <int T> struct Raw { u32x2 w; };
+template <> struct Raw<T_F32> { f32x4 f; };
+
+template <int T, int G>
+__device__ __forceinline__ void load_segs(const Args& a, int b, int lane, const int64_t (&seg)[G], Raw<T> (&r)[G]) {
+  bool whole = true;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint16_t lo = (uint16_t)w[j], hi = (uint16_t)(w[j] >> 16);
-        v[2 * j] = T == T_BF16 ? bf16_to_f32(lo) : __half2float(__ushort_as_half(lo));
-        v[2 * j + 1] = T == T_BF16 ? bf16_to_f32(hi) : __half2float(__ushort_as_half(hi));
-      }
+  for (int g = 0; g < G; ++g) whole = whole && (seg[g] + 1) * SEG <= a.N;
+  const int64_t row = (int64_t)b * a.ld + lane * 4;
+  if (whole) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if constexpr (T == T_F32) r[g].f = *(const f32x4*)((const float*)a.s + row + seg[g] * SEG);
+      else r[g].w = *(const u32x2*)((const uint16_t*)a.s + row + seg[g] * SEG);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = i + j < a.N ? load1<T>(a.s, at + j) : -INFINITY;
+    for (int g = 0; g < G; ++g) {
+      const int64_t i = seg[g] * SEG + lane * 4;
+      if constexpr (T == T_F32) {
+        const float* p = (const float*)a.s + row + seg[g] * SEG;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[g].f[j] = i + j < a.N ? p[j] : -INFINITY;
+      } else {
+        const uint16_t* p = (const uint16_t*)a.s + row + seg[g] * SEG;
+        const uint32_t none = T == T_BF16 ? 0xff80u : 0xfc00u;  // -inf
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = i + j < a.N ? p[j] : none;
+        r[g].w = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+      }
+    }
+  }
+}
+// G segments of a row, `step` apart (those behind the row's last: the last again)
+template <int T, int G>
+__device__ __forceinline__ void load_segs(const Args& a, int b, int lane, int64_t first, int step, Raw<T> (&r)[G]) {
+  int64_t seg[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) seg[g] = min(first + g * step, a.nseg - 1);
+  load_segs<T, G>(a, b, lane, seg, r);
+}
+template <int T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float v[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (T == T_F32) {
+      v[j] = r.f[j];
+    } else {
+      const uint16_t h = (uint16_t)(r.w[j >> 1] >> (16 * (j & 1)));
+      v[j] = T == T_BF16 ? bf16_to_f32(h) : __half2float(__ushort_as_half(h));
+    }
+    v[j] = clean(v[j]);
   }
 }
 template <int T>
 __device__ __forceinline__ void load_seg(const Args& a, int b, int64_t seg, int lane, float v[4]) {
-  load_raw<T>(a, b, seg, lane, v);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = clean(v[j]);
+  const int64_t at[1] = {seg};
+  Raw<T> raw[1];
+  load_segs<T, 1>(a, b, lane, at, raw);
+  unpack<T>(raw[0], v);
 }
 __device__ __forceinline__ float max4(const float v[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
 
@@ -229,7 +263,7 @@ __device__ __forceinline__ float max4(const float v[4]) { return fmaxf(fmaxf(v[0
 // between lanes: a step costs a few cycles where a shuffle through LDS costs ~100.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t lanes_below(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, ROWS == 0xf);
 }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint64_t lanes_below(uint64_t v) {
@@ -264,22 +298,28 @@ __device__ __forceinline__ float lane_value(float v, int l) { return __uint_as_f
 __device__ __forceinline__ double lane_value(double v, int l) {
   return __longlong_as_double((int64_t)lane_value((uint64_t)__double_as_longlong(v), l));
 }
+// The total, which only the last lane has to come by: the steps between rows go to all rows, the moves
+// need no cleared register before them, and 32-bit ones are operands of the sums.  The order is the scan's.
 template <typename V>
-__device__ __forceinline__ V wave_sum(V v) { return lane_value(wave_scan(v), 63); }
-
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float max_below(float v) {
-  const int none = (int)0xff800000u;  // -inf
-  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(none, __float_as_int(v), CTRL, ROWS, 0xf, false)));
+__device__ __forceinline__ V wave_sum(V v) {
+  v += lanes_below<0x111, 0xf>(v);
+  v += lanes_below<0x112, 0xf>(v);
+  v += lanes_below<0x114, 0xf>(v);
+  v += lanes_below<0x118, 0xf>(v);
+  v += lanes_below<0x142, 0xf>(v);
+  v += lanes_below<0x143, 0xf>(v);
+  return lane_value(v, 63);
 }
-__device__ __forceinline__ float wave_max(float v) {
-  v = max_below<0x111, 0xf>(v);
-  v = max_below<0x112, 0xf>(v);
-  v = max_below<0x114, 0xf>(v);
-  v = max_below<0x118, 0xf>(v);
-  v = max_below<0x142, 0xa>(v);
-  v = max_below<0x143, 0xc>(v);
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+// (over keys: where no lane is below, 0 takes part, the smallest of them)
+__device__ __forceinline__ float wave_max(float f) {
+  uint32_t v = key_of(f);
+  v = max(v, lanes_below<0x111, 0xf>(v));
+  v = max(v, lanes_below<0x112, 0xf>(v));
+  v = max(v, lanes_below<0x114, 0xf>(v));
+  v = max(v, lanes_below<0x118, 0xf>(v));
+  v = max(v, lanes_below<0x142, 0xf>(v));
+  v = max(v, lanes_below<0x143, 0xf>(v));
+  return score_of(lane_value(v, 63));
 }
 
 template <int CTRL, int ROWS>
@@ -332,30 +372,34 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   const bool mass = r.direct() && !r.cut_min;
   // rows that cut by mass: fp32 sums, to place the histogram's bins
   const bool rough = r.by_mass();
-  const float cf = (float)r.c;
-  float v[STAT_SEGS][4];
-#pragma unroll
-  for (int j = 0; j < STAT_SEGS; ++j) load_raw<T>(a, b, min(seg0 + j, a.nseg - 1), lane, v[j]);
+  const float cf = fminf(fmaxf((float)r.c, 0x1p-100f), 0x1p100f);  // (no NaN from 0 * inf)
+  Raw<T> raw[STAT_SEGS];
+  load_segs<T, STAT_SEGS>(a, b, lane, seg0, 1, raw);
   float ms = -INFINITY;
   double ws = 0;
 #pragma unroll
   for (int j = 0; j < STAT_SEGS; ++j) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[j][i] = clean(v[j][i]);
-    const float m = wave_max(max4(v[j]));
+    float v[4];
+    unpack<T>(raw[j], v);
+    const float m = wave_max(max4(v));
     if (lane == j) ms = m;
     if (mass) {
       double w = 0;
       if (m > -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w += weight(v[j][i], m, r.c);
+        for (int i = 0; i < 4; ++i) w += weight(v[i], m, r.c);
         w = wave_sum(w);
       }
       if (lane == j) ws = w;
     } else if (rough) {
-      float w = 0;
+      float w = 0;  // (nothing reads that of a segment without scores)
+      if (m < INFINITY) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w += v[j][i] == m ? 1.f : v[j][i] > -INFINITY ? __builtin_amdgcn_exp2f((v[j][i] - m) * cf) : 0.f;
+        for (int i = 0; i < 4; ++i) w += __builtin_amdgcn_exp2f((v[i] - m) * cf);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w += v[i] == m ? 1.f : 0.f;
+      }
       w = wave_sum(w);
       if (lane == j) ws = w;
     }
@@ -540,19 +584,17 @@ struct Source {
         __syncthreads();
         const int n = sh.nsegs;
         for (int q = wave * G; q < n; q += G * WAVES) {
-          float x[G][4];
+          Raw<T> x[G];
           int64_t seg[G];
 #pragma unroll
-          for (int j = 0; j < G; ++j) {
-            seg[j] = base + __builtin_amdgcn_readfirstlane((int)sh.segs[min(q + j, n - 1)]);
-            load_raw<T>(a, b, seg[j], lane, x[j]);
-          }
+          for (int j = 0; j < G; ++j) seg[j] = base + __builtin_amdgcn_readfirstlane((int)sh.segs[min(q + j, n - 1)]);
+          load_segs<T, G>(a, b, lane, seg, x);
 #pragma unroll
           for (int j = 0; j < G; ++j)
             if (q + j < n) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
-              f(seg[j], x[j]);
+              float y[4];
+              unpack<T>(x[j], y);
+              f(seg[j], y);
             }
         }
       }
@@ -1107,16 +1149,14 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     }
   } else if constexpr (R == ROW_CACHED) {
     for (int64_t seg0 = wave; seg0 < a.nseg; seg0 += 4 * WAVES) {
-      float x[4][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (seg0 + j * WAVES < a.nseg) load_raw<T>(a, b, seg0 + j * WAVES, lane, x[j]);
+      Raw<T> raw[4];
+      load_segs<T, 4>(a, b, lane, seg0, WAVES, raw);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (seg0 + j * WAVES < a.nseg) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
-          const float y = wave_max(max4(x[j]));
+          float x[4];
+          unpack<T>(raw[j], x);
+          const float y = wave_max(max4(x));
           if (lane == 0) small_max[seg0 + j * WAVES] = y;
           m = fmaxf(m, y);
         }
@@ -1247,15 +1287,16 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
   uint64_t rest = 0;  // the last bin's: scores that can hardly hold the threshold
   const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
   for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
-    float x[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) load_raw<T>(a, b, min(seg0 + j * WAVES, a.nseg - 1), lane, x[j]);
+    Raw<T> raw[4];
+    load_segs<T, 4>(a, b, lane, seg0, WAVES, raw);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (seg0 + j * WAVES >= s1) continue;
+      float x[4];
+      unpack<T>(raw[j], x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float v = clean(x[j][i]);
+        const float v = x[i];
         const int bin = bin_of(v, st.M, st.cb);
         const bool in = v > floor_score;
         uint64_t w = in;
@@ -1286,6 +1327,9 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   if (st.mode == IDLE) return;
   const Row r = row_settings(a, b);
   const float floor_score = score_of(st.floor_key);
+  const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
+  Raw<T> raw[4];
+  load_segs<T, 4>(a, b, lane, (int64_t)blockIdx.x * PASS_SEGS + wave, WAVES, raw);  // on their way during the search
   // min-p drops scores from the draw, not from the total of which top-p keeps a part
   const bool drop = r.cut_min && !(st.mode == BY_TOP_K && r.cut_p);
   int bin = BINS;
@@ -1309,26 +1353,24 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
     e.w = fixed(weight(score_of(e.key()), st.M, r.c), st.shift);
     if (at < (uint32_t)a.listcap) a.list[(int64_t)b * a.listcap + at] = e;
   };
-  const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
   for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
-    float x[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) load_raw<T>(a, b, min(seg0 + j * WAVES, a.nseg - 1), lane, x[j]);
+    if (seg0 >= (int64_t)blockIdx.x * PASS_SEGS + 4 * WAVES) load_segs<T, 4>(a, b, lane, seg0, WAVES, raw);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t seg = seg0 + j * WAVES;
       if (seg >= s1) continue;
+      float x[4];
+      unpack<T>(raw[j], x);
       // scores above the threshold's bin are moved together, so that a wave computes 64 weights at once
       bool up[4], in[4];
       int place[4], n = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[j][i] = clean(x[j][i]);
-        const int at_bin = x[j][i] > floor_score ? bin_of(x[j][i], st.M, st.cb) : BINS;
+        const int at_bin = x[i] > floor_score ? bin_of(x[i], st.M, st.cb) : BINS;
         in[i] = at_bin == bin && bin < BINS;
         up[i] = at_bin < bin;
         const uint64_t mask = __ballot(up[i]);
-        if (up[i]) above[wave][n + __popcll(mask & ((1ull << lane) - 1))] = x[j][i];
+        if (up[i]) above[wave][n + __popcll(mask & ((1ull << lane) - 1))] = x[i];
         n += __popcll(mask);
       }
       uint64_t sum = 0;
@@ -1341,15 +1383,15 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
       if (bin == BINS && st.ties) {  // the scores equal to the floor: not listed, counted here
         uint32_t c = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c += x[j][i] == floor_score;
+        for (int i = 0; i < 4; ++i) c += x[i] == floor_score;
         c = wave_sum(c);
         if (lane == 0) a.segtie[(int64_t)b * a.nseg + seg] = (int32_t)c;
       }
-      if (take_places(in, &count, place))
+      if (__ballot(in[0] | in[1] | in[2] | in[3]) && take_places(in, &count, place))
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (in[i]) {
-            const Entry e = make_entry(key_of(x[j][i]), (int32_t)(seg * SEG + lane * 4 + i), 0);
+            const Entry e = make_entry(key_of(x[i]), (int32_t)(seg * SEG + lane * 4 + i), 0);
             if (place[i] < PASS_LIST) listed[place[i]] = e;
             else put(atomicAdd(&a.state[b].listed, 1u), e);  // more than this workgroup lists
           }
@@ -1554,7 +1596,6 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
     return (int)hipErrorInvalidValue;
   Args a;
   a.s = s; a.ld = ld; a.N = N; a.nseg = (N + SEG - 1) / SEG; a.B = B;
-  a.vec = (B == 1 || ld % 4 == 0) && ((uintptr_t)s & (type == T_F32 ? 15 : 7)) == 0;
   a.u = u;
   a.temperature = temperature; a.temperature0 = temperature0;
   a.top_k = top_k; a.top_k0 = top_k0;
