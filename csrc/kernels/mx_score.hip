@@ -69,11 +69,19 @@ __device__ __forceinline__ bf16x8 to_bf16(const Block<8>& b, int s, float f) {
   return bf16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-// a lane's blocks of one chunk, for its IT rows, with their scale bytes
+// A lane's blocks of one chunk, for its IT rows, with their scale bytes as they were loaded, CS in a load
+// (byte by byte and put together, each would be waited for before the next block's load is sent:
+// 37 x 100003 x 300 in fp8 21.5 us against 17).  `late`: how many of them lie before the chunk's first.
+template <int CS> struct Scales { typedef uint32_t Word; typedef uint32_t Any __attribute__((aligned(1))); };
+template <> struct Scales<2> { typedef uint16_t Word; typedef uint16_t Any __attribute__((aligned(1))); };
+template <> struct Scales<1> { typedef uint8_t Word; typedef uint8_t Any; };
 template <int XB, int IT, int CS>
 struct Chunk {
   Block<XB> b[IT][CS];
-  uint32_t s[IT];  // byte j: block j's scale
+  typename Scales<CS>::Word s[IT];  // (widened at use: a load widened at once would be waited for)
+  int late;
+  // byte j: block j's scale, 0 for a block that is not there (zeros times 2^-127)
+  __device__ __forceinline__ uint32_t scales(int t) const { return late >= CS ? 0u : (uint32_t)s[t] >> (8 * late); }
 };
 
 struct Args {
@@ -85,7 +93,6 @@ struct Args {
   int64_t ld, N;
   int B, D, nblk;
   int vec;               // every lane's IT scores start on their own size
-  int q_align;           // bytes on which every 8th value of every bf16 query starts (at most 16)
   int s_word;            // nblk % 4 == 0: scales in loads of four
   int qtiles, itiles;
 };
@@ -96,15 +103,21 @@ __device__ __forceinline__ int chunk_s(int nblk, int c0) { return min(CS, (nblk 
 
 template <int XB, int IT, int CS>
 __device__ __forceinline__ void load_chunk(const Args& a, int64_t row0, int c0, int h, Chunk<XB, IT, CS>& ch) {
+  static_assert(CS == 1 || CS == 2 || CS == 4, "scale bytes in one load");
   const int S = chunk_s<CS>(a.nblk, c0), first = c0 + h * S;
+  const int from = max(min(first, a.nblk - CS), 0);
+  ch.late = first - from;
 #pragma unroll
   for (int t = 0; t < IT; ++t) {
     const int64_t row = min(row0 + t, a.N - 1);  // rows past the end: loaded again, not stored
     const uint8_t* p = a.x + (row * a.nblk + first) * (MX_BLOCK * XB / 8);
-    const uint8_t* sp = a.xs + row * a.nblk + first;
-    uint32_t s = 0x7f7f7f7fu;  // a block that is not there: zeros times one
-    const bool word = CS == 4 && S == 4 && a.s_word;
-    if (word) s = *(const uint32_t*)sp;  // nblk % 4 == 0: first + 4 <= nblk
+    const uint8_t* sp = a.xs + row * a.nblk + from;
+    if (CS <= 2 || a.nblk >= CS) {  // (CS <= 2: nblk >= CS in every launch)
+      ch.s[t] = *(const typename Scales<CS>::Any*)sp;
+    } else {
+      ch.s[t] = 0;
+      for (int j = 0; j < a.nblk; ++j) ch.s[t] |= sp[j] << (8 * j);
+    }
 #pragma unroll
     for (int j = 0; j < CS; ++j) {
       Block<XB>& b = ch.b[t][j];
@@ -113,40 +126,48 @@ __device__ __forceinline__ void load_chunk(const Args& a, int64_t row0, int c0, 
       if (j < S && first + j < a.nblk) {
         b.v = *(const uint4*)(p + j * (MX_BLOCK * XB / 8));
         if constexpr (XB == 8) b.w = *(const uint4*)(p + j * 32 + 16);
-        if (!word) s = (s & ~(255u << (8 * j))) | ((uint32_t)sp[j] << (8 * j));
       }
     }
-    ch.s[t] = s;
   }
 }
 
-// eight bf16 of a query from value d on; values >= D are zero
-__device__ __forceinline__ uint4 load_query8(const Args& a, int q, int d) {
-  const uint16_t* p = (const uint16_t*)a.q + (int64_t)q * a.D + d;
-  if (d + 8 <= a.D) {
-    if (a.q_align == 16) return *(const uint4*)p;
-    if (a.q_align == 8) {
-      const uint2 lo = *(const uint2*)p, hi = *(const uint2*)(p + 4);
-      return make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
-    if (a.q_align == 4) {
-      const uint32_t* w = (const uint32_t*)p;
-      return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (d + j < a.D) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
+// Waits for all loads, where the compiler sees it: registers loaded before a loop and again in it would
+// else be waited for at their first use there, every time, with all that was sent since.
+__device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
-// 16 bytes of a query: piece c of block blk (bf16: 4 pieces a block, E2M1: 1)
-template <bool Q4>
+// 16 bytes of a query: piece c of block blk (bf16: 4 pieces a block, E2M1: 1).  A row of bf16 values may
+// start and end anywhere: the piece over its end is loaded as the row's last 8 values, and settle()
+// moves them to their places and zeros behind them (apart, so that loads do not wait for each other).
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <bool Q4, bool NARROW>
 __device__ __forceinline__ uint4 load_piece(const Args& a, int q, int blk, int c) {
-  if (q >= a.B || blk >= a.nblk) return make_uint4(0, 0, 0, 0);
-  if (Q4) return *(const uint4*)((const uint8_t*)a.q + ((int64_t)q * a.nblk + blk) * 16);
-  return load_query8(a, q, blk * 32 + c * 8);
+  if (Q4) {
+    if (q >= a.B || blk >= a.nblk) return make_uint4(0, 0, 0, 0);
+    return *(const uint4*)((const uint8_t*)a.q + ((int64_t)q * a.nblk + blk) * 16);
+  }
+  const int d = blk * 32 + c * 8;
+  if (q >= a.B || d >= a.D) return make_uint4(0, 0, 0, 0);
+  const uint16_t* p = (const uint16_t*)a.q + (int64_t)q * a.D;
+  if (NARROW && a.D < 8) {
+    uint64_t w[2] = {0, 0};
+#pragma unroll 1
+    for (int j = a.D - 1; j >= 0; --j) {
+      w[1] = w[1] << 16 | w[0] >> 48;
+      w[0] = w[0] << 16 | p[j];
+    }
+    return make_uint4((uint32_t)w[0], (uint32_t)(w[0] >> 32), (uint32_t)w[1], (uint32_t)(w[1] >> 32));
+  }
+  const u32x4_any v = *(const u32x4_any*)(p + min(d, a.D - 8));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+template <bool Q4>
+__device__ __forceinline__ uint4 settle(const Args& a, int blk, int c, uint4 v) {
+  if (Q4 || (a.D & 7) == 0 || a.D < 8) return v;
+  const int n = max(blk * 32 + c * 8 - (a.D - 8), 0);  // values too early (8 and more: the piece is zeros)
+  if (n & 4) v = make_uint4(v.z, v.w, 0, 0);
+  if (n & 2) v = make_uint4(v.y, v.z, v.w, 0);
+  if (n & 1) v = make_uint4(v.x >> 16 | v.y << 16, v.y >> 16 | v.z << 16, v.z >> 16 | v.w << 16, v.w >> 16);
+  return v;
 }
 __device__ __forceinline__ uint8_t load_qscale(const Args& a, int q, int blk) {
   return q < a.B && blk < a.nblk ? a.qs[(int64_t)q * a.nblk + blk] : (uint8_t)127;
@@ -193,6 +214,9 @@ __device__ __forceinline__ void store_scores(char* at, bool whole, int left, con
 template <int XB, bool Q4, int QT, int IT, int CS, int STRIDE, int SSTRIDE>
 __device__ __forceinline__ void multiply(const uint8_t* qrow, const uint8_t* qsrow, int first, int S,
                                          const Chunk<XB, IT, CS>& cur, f32x16 (&acc)[IT][QT]) {
+  uint32_t sc[IT];
+#pragma unroll
+  for (int t = 0; t < IT; ++t) sc[t] = cur.scales(t);
 #pragma unroll
         for (int j = 0; j < CS; ++j) {
           if (j < S) {
@@ -212,13 +236,13 @@ __device__ __forceinline__ void multiply(const uint8_t* qrow, const uint8_t* qsr
 #pragma unroll
                 for (int q = 0; q < QT; ++q)
                   acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
-                                                                              (int)(cur.s[t] >> (8 * j)));
+                                                                              (int)(sc[t] >> (8 * j)));
               }
             } else {
               float f[IT];
 #pragma unroll
               for (int t = 0; t < IT; ++t) {
-                const uint32_t s = (cur.s[t] >> (8 * j)) & 255u;
+                const uint32_t s = (sc[t] >> (8 * j)) & 255u;
                 f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
               }
 #pragma unroll
@@ -236,6 +260,32 @@ __device__ __forceinline__ void multiply(const uint8_t* qrow, const uint8_t* qsr
             }
           }
         }
+}
+
+// 16-byte pieces 0 .. pieces - 1 of 32 QT queries from block blk0 on to LDS, U in flight a thread
+template <bool Q4, bool NARROW, int QT, int STRIDE, int SSTRIDE, int U>
+__device__ __forceinline__ void stage_queries(const Args& a, int q0, int blk0, int pieces, uint8_t* ql, uint8_t* qsl) {
+  constexpr int CB = Q4 ? 1 : 4;
+  for (int e0 = threadIdx.x; e0 < 32 * QT * pieces; e0 += U * THREADS) {
+    uint4 v[U];
+    uint8_t s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * THREADS, r = e / pieces, c = e - r * pieces;
+      if (e < 32 * QT * pieces) {
+        v[u] = load_piece<Q4, NARROW>(a, q0 + r, blk0 + c / CB, c % CB);
+        if (Q4) s[u] = load_qscale(a, q0 + r, blk0 + c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * THREADS, r = e / pieces, c = e - r * pieces;
+      if (e < 32 * QT * pieces) {
+        *(uint4*)(ql + r * STRIDE + c * 16) = settle<Q4>(a, blk0 + c / CB, c % CB, v[u]);
+        if (Q4) qsl[r * SSTRIDE + c] = s[u];
+      }
+    }
+  }
 }
 
 // LB: blocks of a query held in LDS
@@ -267,12 +317,9 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   if (it >= a.itiles) return;
   const int q0 = qt * 32 * QT;
   {  // all of the queries, or their first chunk
-    const int nb = once ? (a.nblk + KC - 1) / KC * KC : KC, pieces = min(nb, LB) * CB;
-    for (int e = threadIdx.x; e < 32 * QT * pieces; e += THREADS) {
-      const int r = e / pieces, c = e - r * pieces;
-      *(uint4*)(ql + r * STRIDE + c * 16) = load_piece<Q4>(a, q0 + r, c / CB, c % CB);
-      if (Q4) qsl[r * SSTRIDE + c] = load_qscale(a, q0 + r, c);
-    }
+    const int nb = once ? (a.nblk + KC - 1) / KC * KC : KC;
+    constexpr int U = 32 * QT * LB * CB / THREADS;
+    stage_queries<Q4, CS == 1, QT, STRIDE, SSTRIDE, U < 1 ? 1 : U < 6 ? U : 6>(a, q0, 0, min(nb, LB) * CB, ql, qsl);
     __syncthreads();
   }
   const uint8_t* qrow = ql + (lane & 31) * STRIDE;
@@ -280,6 +327,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   const auto row_of_tile = [&](int i) { return (int64_t)i * (WAVES * 32 * IT) + wave * (32 * IT) + (lane & 31) * IT; };
   Chunk<XB, IT, CS> cur, nxt;
   load_chunk<XB, IT, CS>(a, row_of_tile(it), 0, h, cur);
+  settle_loads();
   int half = 0;  // not once: the half of LDS that holds the present chunk's queries
   for (; it < a.itiles; it += step) {
     const int64_t row0 = row_of_tile(it);
@@ -292,15 +340,15 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
         for (int r = 0; r < 16; ++r) acc[t][q][r] = 0.f;
     for (int c0 = 0; c0 < a.nblk; c0 += KC) {
       const bool more = c0 + KC < a.nblk;
-      if (more) load_chunk<XB, IT, CS>(a, row0, c0 + KC, h, nxt);
-      else if (it + step < a.itiles) load_chunk<XB, IT, CS>(a, row_of_tile(it + step), 0, h, nxt);
+      if (more || it + step < a.itiles)
+        load_chunk<XB, IT, CS>(a, more ? row0 : row_of_tile(it + step), more ? c0 + KC : 0, h, nxt);
       uint4 qn[QREGS];
       uint8_t qsn[QREGS];
       if (CS > 1 && !once && more) {
 #pragma unroll
         for (int i = 0; i < QREGS; ++i) {
           const int e = threadIdx.x + i * THREADS, r = e / (KC * CB), c = e % (KC * CB);
-          qn[i] = load_piece<Q4>(a, q0 + r, c0 + KC + c / CB, c % CB);
+          qn[i] = load_piece<Q4, false>(a, q0 + r, c0 + KC + c / CB, c % CB);
           if (Q4) qsn[i] = load_qscale(a, q0 + r, c0 + KC + c);
         }
       }
@@ -310,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < QREGS; ++i) {
           const int e = threadIdx.x + i * THREADS, r = e / (KC * CB), c = e % (KC * CB);
-          *(uint4*)(ql + r * STRIDE + (half ^ 1) * (KC * QBYTES) + c * 16) = qn[i];
+          *(uint4*)(ql + r * STRIDE + (half ^ 1) * (KC * QBYTES) + c * 16) = settle<Q4>(a, c0 + KC + c / CB, c % CB, qn[i]);
           if (Q4) qsl[r * SSTRIDE + (half ^ 1) * KC + c] = qsn[i];
         }
         half ^= 1;
@@ -366,16 +414,12 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_split_kernel(Args a) {
   Chunk<XB, IT, CS> cur, nxt;
   const int c1 = wave * KC;
   if (c1 < a.nblk) load_chunk<XB, IT, CS>(a, row0, c1, h, cur);
+  settle_loads();
   for (int s0 = 0; s0 < a.nblk; s0 += LB) {
     const int c0 = s0 + c1;
     if (c0 + LB < a.nblk) load_chunk<XB, IT, CS>(a, row0, c0 + LB, h, nxt);
     __syncthreads();
-#pragma unroll 4
-    for (int e = threadIdx.x; e < 32 * QT * LB * CB; e += THREADS) {
-      const int r = e / (LB * CB), c = e % (LB * CB);
-      *(uint4*)(ql + r * STRIDE + c * 16) = load_piece<Q4>(a, q0 + r, s0 + c / CB, c % CB);
-      if (Q4) qsl[r * SSTRIDE + c] = load_qscale(a, q0 + r, s0 + c);
-    }
+    stage_queries<Q4, false, QT, STRIDE, SSTRIDE, 4>(a, q0, s0, LB * CB, ql, qsl);
     __syncthreads();
     if (c0 < a.nblk) {
       const int S = chunk_s<CS>(a.nblk, c0);
@@ -607,8 +651,6 @@ int score(const void* q, const void* qs, const void* x, const void* xs, int xbit
   a.q = q; a.qs = (const uint8_t*)qs; a.x = (const uint8_t*)x; a.xs = (const uint8_t*)xs;
   a.out = out; a.ld = ld; a.N = N; a.B = B; a.D = D;
   a.nblk = (D + MX_BLOCK - 1) / MX_BLOCK;
-  const uintptr_t qp = (uintptr_t)q | (uintptr_t)(2 * D);  // D even, a multiple of 4, of 8
-  a.q_align = qp & 2 ? 2 : qp & 4 ? 4 : qp & 8 ? 8 : 16;
   a.s_word = a.nblk % 4 == 0 && ((uintptr_t)xs & 3) == 0;
   const bool few = B <= 32, narrow = a.nblk <= 2;
   // Few queries, long rows and too few rows to give every CU its 256: the waves split the row instead.  (us, whole

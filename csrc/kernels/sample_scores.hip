@@ -191,8 +191,8 @@ __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane
 
 // This lane's four scores of a segment as they lie in memory; places past the row are masked.  They are
 // unpacked where they are used, and a wave takes one branch for a group of segments: converted at once,
-// or with a branch for each, a load would be waited for before the next is sent (16.7M bf16 scores:
-// stats pass 12 us against STATS, histogram 24 against HIST).
+// or with a branch for each, a load would be waited for before the next is sent (softmax over 16M fp32
+// scores: stats pass 24 us against 21).
 template <int T> struct Raw { u32x2 w; };
 template <> struct Raw<T_F32> { f32x4 f; };
 
