@@ -31,4 +31,8 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
   return e == 255 ? 255u : (uint32_t)max(e - emax, 0);
 }
 
+// Waits for all loads, where the compiler sees it: a register that a branch may or may not have loaded is
+// else waited for at each later use, with all that was sent since.
+__device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
 }  // namespace fps

@@ -160,6 +160,27 @@ __device__ __forceinline__ Walk walk_from(const RowShape& s, int64_t unit) {
   return Walk{row, (int)(share - row * s.lpr)};
 }
 
+// The indices of UNROLL places as they lie in memory (places past the end: the last index), and the slots they
+// name.  Apart, so that the loads leave together: widened at once, each 32-bit index would be waited for.
+struct RawIndex { int32_t lo, hi; };
+__device__ __forceinline__ void load_indices(const void* idx, int idx64, int64_t n, const Place (&w)[UNROLL],
+                                             RawIndex (&raw)[UNROLL]) {
+  if (idx == nullptr) return;
+  if (idx64) {
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) raw[k] = ((const RawIndex*)idx)[min(w[k].row, n - 1)];
+  } else {
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) raw[k].lo = ((const int32_t*)idx)[min(w[k].row, n - 1)];
+  }
+}
+// -1 where there is none
+__device__ __forceinline__ int64_t slot_of(const void* idx, int idx64, const Place& w, const RawIndex& raw, int64_t rows) {
+  int64_t slot = w.row;
+  if (idx != nullptr) slot = idx64 ? (int64_t)((uint64_t)(uint32_t)raw.hi << 32 | (uint32_t)raw.lo) : (int64_t)raw.lo;
+  return w.on && slot < rows ? slot : -1;
+}
+
 template <int BITS>
 __device__ __forceinline__ void quantise(float v[VPL], uint32_t& s, uint2& q) {
   uint32_t m = 0;
@@ -199,6 +220,7 @@ __global__ void __launch_bounds__(256) mx_set_rows_kernel(const void* __restrict
   Walk walk = walk_from(shape, first_unit());
   for (int64_t u0 = first_unit(); u0 < shape.units; u0 += (int64_t)gridDim.x * 4 * UNROLL) {
     Place w[UNROLL];
+    RawIndex raw[UNROLL];
     int64_t slot[UNROLL];
     float v[UNROLL][VPL];
     Walk unit = walk;
@@ -207,20 +229,25 @@ __global__ void __launch_bounds__(256) mx_set_rows_kernel(const void* __restrict
     for (int k = 0; k < UNROLL; ++k) {
       w[k] = unit.place(shape, n);
       unit.move(shape.unit_rows, shape.unit_rem, shape.lpr);
-      slot[k] = -1;
-      if (w[k].on) {
-        slot[k] = row_of(idx, idx64, w[k].row);
-        load8<T, VEC>(x, w[k].row, D, w[k].g * VPL, v[k]);
-      }
     }
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k)
+      if (w[k].on) load8<T, VEC>(x, w[k].row, D, w[k].g * VPL, v[k]);
+    load_indices(idx, idx64, n, w, raw);
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) slot[k] = slot_of(idx, idx64, w[k], raw[k], rows);
     if (CLAIM) {
+      settle_loads();
+      int32_t own[UNROLL];
+#pragma unroll
+      for (int k = 0; k < UNROLL; ++k) own[k] = owner[max(slot[k], (int64_t)0)];
 #pragma unroll
       for (int k = 0; k < UNROLL; ++k)
-        if (slot[k] >= 0 && slot[k] < rows && owner[slot[k]] != (int32_t)w[k].row) slot[k] = -1;
+        if (own[k] != (int32_t)w[k].row) slot[k] = -1;
     }
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      if (slot[k] < 0 || slot[k] >= rows) continue;
+      if (slot[k] < 0) continue;
       uint32_t s;
       uint2 q;
       quantise<BITS>(v[k], s, q);
@@ -302,6 +329,7 @@ __global__ void __launch_bounds__(256) mx_gather_rows_kernel(const uint8_t* __re
   Walk walk = walk_from(shape, first_unit());
   for (int64_t u0 = first_unit(); u0 < shape.units; u0 += (int64_t)gridDim.x * 4 * UNROLL) {
     Place w[UNROLL];
+    RawIndex raw[UNROLL];
     int64_t slot[UNROLL];
     uint2 q[UNROLL];
     uint32_t s[UNROLL];
@@ -312,18 +340,21 @@ __global__ void __launch_bounds__(256) mx_gather_rows_kernel(const uint8_t* __re
       w[k] = unit.place(shape, n);
       unit.move(shape.unit_rows, shape.unit_rem, shape.lpr);
       w[k].on = w[k].on && w[k].g * V < D;
-      slot[k] = -1;
-      if (w[k].on) slot[k] = row_of(idx, idx64, w[k].row);
     }
+    load_indices(idx, idx64, n, w, raw);
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) slot[k] = slot_of(idx, idx64, w[k], raw[k], rows);
+    settle_loads();
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       q[k] = make_uint2(0, 0);
       s[k] = 127;
-      if (slot[k] >= 0 && slot[k] < rows) {
+      if (slot[k] >= 0) {
         q[k] = load_packed<BITS, V>(data + slot[k] * row_bytes + (int64_t)w[k].g * (V * BITS / 8));
         s[k] = scale[slot[k] * nblk + w[k].g / PER];
       }
     }
+    settle_loads();  // here, and not again between the stores, each of which would be waited for
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       float v[V];

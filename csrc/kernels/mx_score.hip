@@ -105,19 +105,14 @@ template <int XB, int IT, int CS>
 __device__ __forceinline__ void load_chunk(const Args& a, int64_t row0, int c0, int h, Chunk<XB, IT, CS>& ch) {
   static_assert(CS == 1 || CS == 2 || CS == 4, "scale bytes in one load");
   const int S = chunk_s<CS>(a.nblk, c0), first = c0 + h * S;
-  const int from = max(min(first, a.nblk - CS), 0);
+  const int from = min(first, a.nblk - CS);  // (nblk >= CS in every launch)
   ch.late = first - from;
 #pragma unroll
   for (int t = 0; t < IT; ++t) {
     const int64_t row = min(row0 + t, a.N - 1);  // rows past the end: loaded again, not stored
     const uint8_t* p = a.x + (row * a.nblk + first) * (MX_BLOCK * XB / 8);
     const uint8_t* sp = a.xs + row * a.nblk + from;
-    if (CS <= 2 || a.nblk >= CS) {  // (CS <= 2: nblk >= CS in every launch)
-      ch.s[t] = *(const typename Scales<CS>::Any*)sp;
-    } else {
-      ch.s[t] = 0;
-      for (int j = 0; j < a.nblk; ++j) ch.s[t] |= sp[j] << (8 * j);
-    }
+    ch.s[t] = *(const typename Scales<CS>::Any*)sp;
 #pragma unroll
     for (int j = 0; j < CS; ++j) {
       Block<XB>& b = ch.b[t][j];
@@ -130,10 +125,6 @@ __device__ __forceinline__ void load_chunk(const Args& a, int64_t row0, int c0, 
     }
   }
 }
-
-// Waits for all loads, where the compiler sees it: registers loaded before a loop and again in it would
-// else be waited for at their first use there, every time, with all that was sent since.
-__device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 // 16 bytes of a query: piece c of block blk (bf16: 4 pieces a block, E2M1: 1).  A row of bf16 values may
 // start and end anywhere: the piece over its end is loaded as the row's last 8 values, and settle()
@@ -327,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   const auto row_of_tile = [&](int i) { return (int64_t)i * (WAVES * 32 * IT) + wave * (32 * IT) + (lane & 31) * IT; };
   Chunk<XB, IT, CS> cur, nxt;
   load_chunk<XB, IT, CS>(a, row_of_tile(it), 0, h, cur);
-  settle_loads();
+  settle_loads();  // (else cur's first use in the loop waits, every time, for nxt as well)
   int half = 0;  // not once: the half of LDS that holds the present chunk's queries
   for (; it < a.itiles; it += step) {
     const int64_t row0 = row_of_tile(it);
@@ -414,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_split_kernel(Args a) {
   Chunk<XB, IT, CS> cur, nxt;
   const int c1 = wave * KC;
   if (c1 < a.nblk) load_chunk<XB, IT, CS>(a, row0, c1, h, cur);
-  settle_loads();
+  settle_loads();  // (else cur's first use in the loop waits, every time, for nxt as well)
   for (int s0 = 0; s0 < a.nblk; s0 += LB) {
     const int c0 = s0 + c1;
     if (c0 + LB < a.nblk) load_chunk<XB, IT, CS>(a, row0, c0 + LB, h, nxt);
@@ -487,6 +478,31 @@ void launch(Args& a, int type, hipStream_t st) {
   if (type == T_F32) launch_as<XB, Q4, QT, IT, CS, LB, T_F32>(a, st);
   else if (type == T_BF16) launch_as<XB, Q4, QT, IT, CS, LB, T_BF16>(a, st);
   else launch_as<XB, Q4, QT, IT, CS, LB, T_F16>(a, st);
+}
+
+// By the width of the rows and the number of queries (us; fp4 table, bf16 queries where not said).
+// One or two blocks a row: a block a lane; so many rows a lane that a store of many queries' scores is 256
+// bytes long (2 against 4 rows: 300 x 200000 x 64 fp32 scores 40.3 / 44.1, 256 x 1M x 64 bf16 ones 120.6 /
+// 115.6), two for few queries (more waves in flight: one query x 1M x 64 11.6 against 13.7).  Longer
+// rows: chunks of 2 blocks a lane, of 4 for fp4 where that fills chunks (2 against 4: 256 x 100003 x
+// 300 36.9 / 41.2, 1 x 1M x 128 17.7 / 19.6, but 64 x 65536 x 4096 62.6 / 60.1, 8 x 65536 x 4096 42.0 /
+// 37.2; fp4 queries, 37 x 300000 x 512 31.4 / 26.1; fp8 table with 4 blocks, 37 x 100003 x 300 23.2 / 16.5).
+// QT = 2 query tiles a wave is what the registers hold beside them (QT = 4, spilling: 512 x 65536 x 4096 417
+// against 351).
+template <int XB, bool Q4>
+void launch_rows(Args& a, bool few, int type, hipStream_t st) {
+  if (a.nblk <= 2) {
+    if (few) launch<XB, Q4, 1, 2, 1, 2>(a, type, st);
+    else if (type == T_F32) launch_as<XB, Q4, 2, 2, 1, 2, T_F32>(a, st);
+    else if (type == T_BF16) launch_as<XB, Q4, 2, 4, 1, 2, T_BF16>(a, st);
+    else launch_as<XB, Q4, 2, 4, 1, 2, T_F16>(a, st);
+  } else if (few) {
+    if (XB == 8 || a.nblk <= 4) launch<XB, Q4, 1, 2, 2, 32>(a, type, st);
+    else if constexpr (XB == 4) launch<XB, Q4, 1, 2, 4, 32>(a, type, st);
+  } else {
+    if (XB == 8 || a.nblk <= (Q4 ? 12 : 32)) launch<XB, Q4, 2, 2, 2, 16>(a, type, st);
+    else if constexpr (XB == 4) launch<XB, Q4, 2, 2, 4, 16>(a, type, st);
+  }
 }
 
 // Both sides in 4 bits, many queries, long rows: bound by the matrix instructions, so both operands
@@ -652,35 +668,27 @@ int score(const void* q, const void* qs, const void* x, const void* xs, int xbit
   a.out = out; a.ld = ld; a.N = N; a.B = B; a.D = D;
   a.nblk = (D + MX_BLOCK - 1) / MX_BLOCK;
   a.s_word = a.nblk % 4 == 0 && ((uintptr_t)xs & 3) == 0;
-  const bool few = B <= 32, narrow = a.nblk <= 2;
+  const bool few = B <= 32;
   // Few queries, long rows and too few rows to give every CU its 256: the waves split the row instead.  (us, whole
-  // rows against split: 1000 x 4096 fp4 38.8 / 20.1, fp8 71.5 / 22.8, 30000 x 4096 fp4 44.7 / 29.8,
-  // 20000 x 1024 fp4 13.8 / 11.5; 65536 x 4096 fp4 46.4 / 42.7 but fp8 92 / 102, 130000 x 2048 fp4 29.9 / 44.9.)
+  // rows against split: 1000 x 4096 fp4 30.7 / 16.1, fp8 48.3 / 20.2, 30000 x 4096 fp4 34.4 / 20.6,
+  // 20000 x 1024 fp4 11.3 / 7.9; 8 queries x 65536 x 4096 fp4 37.0 / 43.1, fp8 72.5 / 63.9, 20 x 65536 x 2048 fp8
+  // 31.7 / 34.3, 130000 x 2048 fp4 28.4 / 37.9.)
   if (few && a.nblk >= 16 && N <= 160 * 256) {
     if (qs) launch_split<4, true>(a, out_type, st);
     else if (xbits == 4) launch_split<4, false>(a, out_type, st);
     else launch_split<8, false>(a, out_type, st);
-    FPS_CHECK_LAUNCH();
-    return 0;
-  }
-  // Otherwise by the width of the rows and the number of queries.  narrow (one or two blocks a row): one block a
-  // lane, four table rows a lane so that a store of many queries' scores is 256 bytes long, two rows where
-  // there are few queries (more waves in flight: 13.7 -> 11.6 us for one query, 1M x 64).  Longer rows:
-  // chunks of 4 (fp4) or 2 (fp8) blocks a lane.  QT = 2 query tiles a wave is what the registers hold
-  // beside them (QT = 4, spilling: 417 us for 512 x 65536 x 4096 in fp4, 351 so).  Both sides in 4
-  // bits and rows long enough to amortise it: the tiled form (us, wide against QT = 2 here: 64 x 65536 x
-  // 4096 50 / 76; rows of 1000 values and 100 queries: equal); its scales are read in words, and its
-  // offsets within a tile's 256 rows are 32-bit ones.
-  if (qs) {
-    if (narrow) { if (few) launch<4, true, 1, 2, 1, 2>(a, out_type, st); else launch<4, true, 2, 4, 1, 2>(a, out_type, st); }
-    else if (!few && a.nblk > 16 && a.nblk < (1 << 20) && a.s_word && ((uintptr_t)qs & 3) == 0) launch_wide(a, out_type, st);
-    else { if (few) launch<4, true, 1, 2, 4, 32>(a, out_type, st); else launch<4, true, 2, 2, 4, 16>(a, out_type, st); }
+  } else if (qs && !few && a.nblk > 16 && a.nblk < (1 << 20) && a.s_word && ((uintptr_t)qs & 3) == 0) {
+    // Both sides in 4 bits and rows long enough to amortise it: the tiled form (us, against the other: 512 x
+    // 20000 x 1024 20.3 / 28.0, 64 x 65536 x 4096 44 / 45; few rows leave it few workgroups: 33 x 7 x
+    // 4096 29.5 / 22.8).  Its scales are read in words, and its offsets within a tile's 256 rows are 32-bit
+    // ones.
+    launch_wide(a, out_type, st);
+  } else if (qs) {
+    launch_rows<4, true>(a, few, out_type, st);
   } else if (xbits == 4) {
-    if (narrow) { if (few) launch<4, false, 1, 2, 1, 2>(a, out_type, st); else launch<4, false, 2, 4, 1, 2>(a, out_type, st); }
-    else { if (few) launch<4, false, 1, 2, 4, 32>(a, out_type, st); else launch<4, false, 2, 2, 4, 16>(a, out_type, st); }
+    launch_rows<4, false>(a, few, out_type, st);
   } else {
-    if (narrow) { if (few) launch<8, false, 1, 2, 1, 2>(a, out_type, st); else launch<8, false, 2, 4, 1, 2>(a, out_type, st); }
-    else { if (few) launch<8, false, 1, 2, 2, 32>(a, out_type, st); else launch<8, false, 2, 2, 2, 16>(a, out_type, st); }
+    launch_rows<8, false>(a, few, out_type, st);
   }
   FPS_CHECK_LAUNCH();
   return 0;
