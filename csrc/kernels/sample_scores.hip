@@ -255,6 +255,13 @@ __device__ __forceinline__ void load_seg(const Args& a, int b, int64_t seg, int 
   load_segs<T, 1>(a, b, lane, at, raw);
   unpack<T>(raw[0], v);
 }
+template <int T>
+__device__ __forceinline__ float load_score(const Args& a, int b, int64_t i) {
+  const int64_t at = (int64_t)b * a.ld + i;
+  if (T == T_F32) return clean(((const float*)a.s)[at]);
+  const uint16_t h = ((const uint16_t*)a.s)[at];
+  return clean(T == T_BF16 ? bf16_to_f32(h) : __half2float(__ushort_as_half(h)));
+}
 __device__ __forceinline__ float max4(const float v[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
 
 // ---- wave and workgroup sums ---------------------------------------------------------------
@@ -355,10 +362,8 @@ __device__ __forceinline__ float block_max(float v, float* tmp) {
   __syncthreads();
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
   __syncthreads();
-  const int nw = blockDim.x >> 6;
-  float m = tmp[0];
-  for (int i = 1; i < nw; ++i) m = fmaxf(m, tmp[i]);
-  return m;
+  const int nw = blockDim.x >> 6, lane = threadIdx.x & 63;
+  return wave_max(lane < nw ? tmp[lane] : -INFINITY);
 }
 
 // ---- long rows, pass 1: the largest score of every segment, its mass where masses decide ----
@@ -454,7 +459,7 @@ struct Shared : Hist<true> {
   uint32_t rank[RANK];
   unsigned long long before[RANK];
   uint16_t segs[WANTED];
-  int nsegs, n;
+  int nsegs, seg_base, n;
   float tmp[WAVES];
   double scan_d[WAVES];
   uint32_t kmin, ties;
@@ -553,16 +558,28 @@ struct Source {
       : a(a_), b(b_), lane(threadIdx.x & 63), wave(wave_id()), in_lds(lds), in_memory(memory) {}
   __device__ __forceinline__ bool kept() const { return R != ROW_LONG || a.nseg <= KEPT; }
   __device__ __forceinline__ float segmax(int64_t s) const { return kept() ? in_lds[s] : in_memory[s]; }
-  // f(segment, scores) for the segments whose largest score (not -inf) is wanted.  Their maxima
-  // are looked at first, many together; the waves share out the wanted ones and load G at a time.
-  template <int G = 4, typename P, typename F>
+  // inside each_batch's f: the segment at a place
+  __device__ __forceinline__ int32_t segment(const Shared& sh, int place) const { return sh.seg_base + sh.segs[place]; }
+  // f(segment, scores) for the segments whose largest score (not -inf) is wanted.
+  template <typename P, typename F>
   __device__ __forceinline__ void each(Shared& sh, P want, F f) {
+    each_batch<4>(sh, want, [&](const int64_t* seg, const float (*x)[4], int count, int) {
+#pragma unroll
+      for (int j = 0; j < (R == ROW_REGS ? 1 : 4); ++j)
+        if (j < count) f(seg[j], x[j]);
+    });
+  }
+  // f(segments, scores, how many, place of the first): up to G of them.  The segments' maxima are looked
+  // at first, many together; the waves share out the wanted ones and load G at a time.
+  template <int G, typename P, typename F>
+  __device__ __forceinline__ void each_batch(Shared& sh, P want, F f) {
     if constexpr (R == ROW_REGS) {
-      if (wave < a.nseg) f((int64_t)wave, v);
+      const int64_t seg[1] = {wave};
+      if (wave < a.nseg) f(seg, &v, 1, 0);
     } else {
       for (int64_t base = 0; base < a.nseg; base += WANTED) {
         __syncthreads();
-        if (threadIdx.x == 0) sh.nsegs = 0;
+        if (threadIdx.x == 0) { sh.nsegs = 0; sh.seg_base = (int)base; }
         float m[WANTED / THREADS];
 #pragma unroll
         for (int j = 0; j < WANTED / THREADS; ++j) {
@@ -570,15 +587,20 @@ struct Source {
           m[j] = at < a.nseg ? segmax(at) : -INFINITY;
         }
         __syncthreads();
+        uint64_t mask[WANTED / THREADS];
+        int total = 0, at = 0;
 #pragma unroll
         for (int j = 0; j < WANTED / THREADS; ++j) {
-          const bool on = m[j] > -INFINITY && want(m[j]);
-          const uint64_t mask = __ballot(on);
-          if (mask) {
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&sh.nsegs, (int)__popcll(mask));
-            at = __builtin_amdgcn_readfirstlane(at);
-            if (on) sh.segs[at + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(j * THREADS + threadIdx.x);
+          mask[j] = __ballot(m[j] > -INFINITY && want(m[j]));
+          total += __popcll(mask[j]);
+        }
+        if (total) {
+          if (lane == 0) at = atomicAdd(&sh.nsegs, total);
+          at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+          for (int j = 0; j < WANTED / THREADS; ++j) {
+            if (mask[j] >> lane & 1) sh.segs[at + __popcll(mask[j] & ((1ull << lane) - 1))] = (uint16_t)(j * THREADS + threadIdx.x);
+            at += __popcll(mask[j]);
           }
         }
         __syncthreads();
@@ -589,13 +611,10 @@ struct Source {
 #pragma unroll
           for (int j = 0; j < G; ++j) seg[j] = base + __builtin_amdgcn_readfirstlane((int)sh.segs[min(q + j, n - 1)]);
           load_segs<T, G>(a, b, lane, seg, x);
+          float y[G][4];
 #pragma unroll
-          for (int j = 0; j < G; ++j)
-            if (q + j < n) {
-              float y[4];
-              unpack<T>(x[j], y);
-              f(seg[j], y);
-            }
+          for (int j = 0; j < G; ++j) unpack<T>(x[j], y[j]);
+          f(seg, y, min(n - q, G), q);
         }
       }
     }
@@ -698,16 +717,54 @@ __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, 
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  src.template each<8>(sh, want, [&](int64_t seg, const float* v) {
-    bool on[4];
-    int place[4];
+  if constexpr (R == ROW_REGS) {
+    src.each(sh, want, [&](int64_t seg, const float* v) {
+      bool on[4];
+      int place[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) on[j] = v[j] > -INFINITY && pick(v[j]);
-    if (take_places(on, &sh.n, place) == 0) return;
+      for (int j = 0; j < 4; ++j) on[j] = v[j] > -INFINITY && pick(v[j]);
+      if (take_places(on, &sh.n, place) == 0) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (on[j] && place[j] < LIST) sh.list[place[j]].at = make_entry(key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), 0).at;
-  });
+      for (int j = 0; j < 4; ++j)
+        if (on[j] && place[j] < LIST) sh.list[place[j]].at = make_entry(key_of(v[j]), (int32_t)(seg * SEG + src.lane * 4 + j), 0).at;
+    });
+  } else {
+    // 16 segments together: a bit per score, then the lanes take out their bits, one each in a turn, and load those
+    // scores again.  (Few of the scores are picked, and instructions that run once cost their fetch:
+    // with every place worked out in line this took 4.6 us of a row's 21, so 1.7.)
+    src.template each_batch<16>(sh, want, [&](const int64_t* seg, const float (*v)[4], int count, int q) {
+      uint32_t bits[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits[j >> 3] += bits[j >> 3] + (uint32_t)(v[j][i] > -INFINITY && pick(v[j][i]));
+      const int gone = 16 - count;  // (the last segment stands in for those behind it)
+      bits[1] &= gone >= 8 ? 0u : ~0u << 4 * gone;
+      bits[0] &= gone > 8 ? ~0u << 4 * (gone - 8) : ~0u;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t left = h ? bits[1] : bits[0];
+#pragma unroll 1
+        for (uint64_t mask; (mask = __ballot(left != 0)) != 0;) {
+          int at = 0;
+          if (src.lane == 0) at = atomicAdd(&sh.n, (int)__popcll(mask));
+          at = __builtin_amdgcn_readfirstlane(at);
+          if (at > LIST) {  // the list is not used: count the rest
+            const uint32_t rest = wave_sum((uint32_t)__popc(left)) - (uint32_t)__popcll(mask);
+            if (src.lane == 0 && rest) atomicAdd(&sh.n, (int)rest);
+            break;
+          }
+          if (left) {
+            const int k = __clz(left);
+            left &= ~(0x80000000u >> k);
+            const int32_t i = src.segment(sh, q + 8 * h + (k >> 2)) * SEG + src.lane * 4 + (k & 3);
+            const int place = at + __popcll(mask & ((1ull << src.lane) - 1));
+            if (place < LIST) sh.list[place].at = make_entry(key_of(load_score<T>(src.a, src.b, i)), i, 0).at;
+          }
+        }
+      }
+    });
+  }
   __syncthreads();
   if (sh.n <= LIST)
     for (int i = threadIdx.x; i < sh.n; i += THREADS) sh.list[i].w = fixed(weight(score_of(sh.list[i].key()), M, r.c), shift);
@@ -1226,7 +1283,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     const auto any = [](float) { return true; };
     clear_hist(sh);
     if (R == ROW_LONG && r.k <= a.nseg / 2) {
-      for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS) {
+      for (int i = threadIdx.x; i < a.nseg; i += THREADS) {
         const float x = src.segmax(i);
         if (x > -INFINITY) atomicAdd(&sh.hc[bin_of(x, M, cb)], 1u);
       }
