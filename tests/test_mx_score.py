@@ -130,6 +130,27 @@ def test_refusals(dev):
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("B", [3, 70])
+@pytest.mark.parametrize("dim", [2, 3, 7, 8, 9, 15, 31, 41, 71, 97, 103, 129, 165, 263, 389, 515, 1029])
+def test_rows_that_end_anywhere(dev, form, B, dim):
+    """Widths around the 8 values of a load, the block and the chunks of 2 and 4 blocks; the last row and
+    query end their buffers."""
+    Q, X = operands(B, 130, dim, form, dev, seed=dim)
+    check(ops.mx_score(Q, X), Q, X)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,N,dim", [(3, 41000, 515), (70, 150000, 64), (33, 140000, 96)])
+def test_many_table_tiles(dev, form, dtype, B, N, dim):
+    """Workgroups that walk several tiles, with the next one's rows on their way."""
+    Q, X = operands(B, N, dim, form, dev, seed=N + B, spread=0.5)
+    check(ops.mx_score(Q, X, out_dtype=dtype), Q, X)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("B", [9, 70])
 def test_scales_at_any_address(dev, form, B):
     """Tables wrapped over buffers whose scale bytes start off four bytes."""
