@@ -139,13 +139,13 @@ def test_rows_that_end_anywhere(dev, form, B, dim):
     check(ops.mx_score(Q, X), Q, X)
 
 
-@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.gpu
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,N,dim", [(3, 41000, 515), (70, 150000, 64), (33, 140000, 96)])
-def test_many_table_tiles(dev, form, dtype, B, N, dim):
+def test_many_table_tiles(form, dtype, B, N, dim):
     """Workgroups that walk several tiles, with the next one's rows on their way."""
-    Q, X = operands(B, N, dim, form, dev, seed=N + B, spread=0.5)
+    Q, X = operands(B, N, dim, form, "cuda", seed=N + B, spread=0.5)
     check(ops.mx_score(Q, X, out_dtype=dtype), Q, X)
 
 
