@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   static_assert(CS == 1 || LB >= 2 * KC, "two chunks of queries");
   __shared__ __attribute__((aligned(16))) uint8_t ql[32 * QT * STRIDE];
   __shared__ __attribute__((aligned(16))) uint8_t qsl[Q4 ? 32 * QT * SSTRIDE : 16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const bool once = CS == 1 || a.nblk <= LB;
   // once: one query tile, every stride-th table tile (the workgroups of one table tile are on one XCD);
   // else one tile
@@ -307,6 +307,9 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   }
   if (it >= a.itiles) return;
   const int q0 = qt * 32 * QT;
+  const auto row_of_tile = [&](int i) { return (int64_t)i * (WAVES * 32 * IT) + wave * (32 * IT) + (lane & 31) * IT; };
+  Chunk<XB, IT, CS> cur, nxt;
+  load_chunk<XB, IT, CS>(a, row_of_tile(it), 0, h, cur);  // on its way while the queries are staged
   {  // all of the queries, or their first chunk
     const int nb = once ? (a.nblk + KC - 1) / KC * KC : KC;
     constexpr int U = 32 * QT * LB * CB / THREADS;
@@ -315,9 +318,6 @@ __global__ void __launch_bounds__(THREADS, 2) mx_score_kernel(Args a) {
   }
   const uint8_t* qrow = ql + (lane & 31) * STRIDE;
   const uint8_t* qsrow = qsl + (lane & 31) * SSTRIDE;
-  const auto row_of_tile = [&](int i) { return (int64_t)i * (WAVES * 32 * IT) + wave * (32 * IT) + (lane & 31) * IT; };
-  Chunk<XB, IT, CS> cur, nxt;
-  load_chunk<XB, IT, CS>(a, row_of_tile(it), 0, h, cur);
   settle_loads();  // (else cur's first use in the loop waits, every time, for nxt as well)
   int half = 0;  // not once: the half of LDS that holds the present chunk's queries
   for (; it < a.itiles; it += step) {
@@ -538,7 +538,7 @@ struct WideLds {
 template <int T>
 __global__ void __launch_bounds__(WTHREADS, 2) mx_score_wide_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) WideLds lds;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
   const int tile = xcd_remap(blockIdx.x, a.qtiles * a.itiles);
   const int q0 = tile % a.qtiles * WT;
   const int64_t i0 = (int64_t)(tile / a.qtiles) * WT;
@@ -626,21 +626,33 @@ __global__ void __launch_bounds__(WTHREADS, 2) mx_score_wide_kernel(Args a) {
     __syncthreads();
     buf ^= 1;
   }
+  // Eight queries at a time, for which one branch decides: those past the last are jumped over, and where all
+  // is there the stores follow each other.  (512 x 20000 x 1024: 17.7 us against 20.3 with conditions for each
+  // store; the other kernel's short calls lose by the two copies of the code: 100 x 20000 x 300 8.0 / 6.9.)
   constexpr int ES = T == T_F32 ? 4 : 2;
   const int64_t row0 = i0 + wi + 2 * l;
-  const int left = (int)min(a.N - row0, (int64_t)2), rows = a.B - q0 - wq - 4 * h;
-  const bool whole = a.vec && left == 2;
+  const int left = (int)min(a.N - row0, (int64_t)2);
+  const bool whole = a.vec && left == 2, full = a.vec && i0 + wi + 64 <= a.N;
   char* o = (char*)a.out + ((int64_t)(q0 + wq + 4 * h) * a.ld + row0) * ES;
   const int64_t down = a.ld * ES;
-  if (left > 0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+  for (int g = 0; g < 16; ++g) {
+    const int first = q0 + wq + 8 * g;
+    if (first >= a.B) return;
+    float v[4][2];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float v[2] = {acc[0][q][r], acc[1][q][r]};
-        if (q * 32 + (r & 3) + 8 * (r >> 2) < rows) store_scores<T, 2>(o, whole, left, v);
-        o += (r & 3) == 3 ? 5 * down : down;
-      }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) v[i][t] = acc[t][g >> 2][4 * (g & 3) + i];
+    if (full && first + 8 <= a.B) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store_scores<T, 2>(o + i * down, true, 2, v[i]);
+    } else if (left > 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (first + 4 * h + i < a.B) store_scores<T, 2>(o + i * down, whole, left, v[i]);
+    }
+    o += 8 * down;
   }
 }
 
@@ -679,7 +691,7 @@ int score(const void* q, const void* qs, const void* x, const void* xs, int xbit
     else launch_split<8, false>(a, out_type, st);
   } else if (qs && !few && a.nblk > 16 && a.nblk < (1 << 20) && a.s_word && ((uintptr_t)qs & 3) == 0) {
     // Both sides in 4 bits and rows long enough to amortise it: the tiled form (us, against the other: 512 x
-    // 20000 x 1024 20.3 / 28.0, 64 x 65536 x 4096 44 / 45; few rows leave it few workgroups: 33 x 7 x
+    // 20000 x 1024 17.4 / 28.0, 64 x 65536 x 4096 39 / 45; few rows leave it few workgroups: 33 x 7 x
     // 4096 29.5 / 22.8).  Its scales are read in words, and its offsets within a tile's 256 rows are 32-bit
     // ones.
     launch_wide(a, out_type, st);
