@@ -860,6 +860,13 @@ __device__ __forceinline__ void draw_from_list(const Args& a, int b, Shared& sh,
   }
 }
 
+__device__ __forceinline__ void no_answer(const Args& a, int b) {
+  if (threadIdx.x == 0) {
+    a.out[b] = -1;
+    if (a.prob) a.prob[b] = 0.f;
+  }
+}
+
 // ---- a draw over a row's segments, given what stays: keys above t and the first `ties` equal to t
 
 // a kept score's mass, in the unit of the segments' masses
@@ -879,7 +886,7 @@ struct AsFixed {
 
 template <typename V>
 struct Found {
-  int64_t seg;
+  int64_t seg;     // -1: no segment has mass
   V before;        // mass of the segments before it
   uint32_t ties;   // ties in the segments before it
   double total, target;
@@ -919,6 +926,7 @@ __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& s
     sum += m;
   }
   const V in_wave = wave_scan(sum);
+  if (threadIdx.x == 0) found->seg = -1;
   __syncthreads();
   if (lane == 63) tmp_v[wave] = in_wave;
   __syncthreads();
@@ -1059,6 +1067,10 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
         return true;
       },
       sh.scan_d, &found);
+  if (f.seg < 0) {
+    no_answer(a, b);
+    return;
+  }
   if (src.wave == (R == ROW_REGS ? (int)f.seg : 0)) {
     float v[4];
     if constexpr (R == ROW_REGS) {
@@ -1229,11 +1241,8 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   }
   const float M = block_max(m, sh.tmp);
   if (M == -INFINITY) {  // nothing is left of the row
-    if (threadIdx.x == 0) {
-      a.out[b] = -1;
-      if (a.prob) a.prob[b] = 0.f;
-      if (passes) a.state[b].mode = IDLE;
-    }
+    no_answer(a, b);
+    if (threadIdx.x == 0 && passes) a.state[b].mode = IDLE;
     return;
   }
   if (R == ROW_LONG && passes) {
@@ -1408,16 +1417,20 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
       a.state[b].all = bin == BINS ? sh.before_m + (sh.bin >= 0 ? sh.hm[sh.bin] : 0) : 0;
     }
   }
-  // what is surely below min-p (the weights themselves decide next to it)
-  float up_floor = floor_score;
+  // The least score that may count: the next above the floor, and none that is surely below min-p (the weights
+  // themselves decide next to it).  That bound is at most M, whatever underflows in it, and rounding to fp32 moves it
+  // past no score at or above it: compared with >=, it drops neither the best score nor any other that stays.  (A NaN,
+  // where M is infinite, drops nothing; above a floor of +inf there is nothing, and a NaN to compare with.)
+  uint32_t up_key = st.floor_key + 1;
   if (drop) {
     const double lim = (double)st.M + ((double)__builtin_amdgcn_logf((float)r.minp) * (1 + 1e-5) - 1e-5) / r.c;
-    up_floor = fmaxf(floor_score, (float)(lim - fabs(lim) * 1e-6));  // (a NaN, where M is infinite, drops nothing)
+    up_key = max(up_key, key_of(fmaxf((float)(lim - fabs(lim) * 1e-6), -INFINITY)));
   }
+  const float up_floor = score_of(up_key);
   // segments without a score that counts (of peaked scores nearly all: 256 x 128000, min-p 0.05 87 us without this)
   bool counts = largest > -INFINITY;
   if (bin < BINS) counts = counts && largest > floor_score && bin_of(largest, st.M, st.cb) <= bin;
-  else counts = counts && (largest > up_floor || (st.ties && largest >= floor_score));
+  else counts = counts && (largest >= up_floor || (st.ties && largest >= floor_score));
   const uint32_t wanted = (uint32_t)__ballot(counts);
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
@@ -1446,7 +1459,7 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
       for (int i = 0; i < 4; ++i) {
         const int at_bin = bin_of(x[i], st.M, st.cb);
         in[i] = at_bin == bin && x[i] > floor_score;
-        up[i] = at_bin < bin && x[i] > up_floor;
+        up[i] = at_bin < bin && x[i] >= up_floor;
         const uint64_t mask = __ballot(up[i]);
         if (up[i]) above[wave][n + __popcll(mask & ((1ull << lane) - 1))] = x[i];
         n += __popcll(mask);
@@ -1613,6 +1626,10 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
       c = (uint32_t)__hip_atomic_load(segtie + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       return true;
     }, sh.scan_m, &found);
+  }
+  if (f.seg < 0) {
+    no_answer(a, b);
+    return;
   }
   if (threadIdx.x < 64) {
     float v[4];

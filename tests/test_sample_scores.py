@@ -341,3 +341,23 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for j in range(2):
         assert all(torch.equal(x, want[j]) for x in got[j])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("n", [100, 3000, 9000, 40000])
+def test_min_p_next_to_a_best_score_of_zero(dev, n):
+    """Rows whose best score is zero or subnormal, at temperatures at which the least weight that min-p keeps lies
+    no fp32 step below the best one: the best one stays, and it is what remains."""
+    S, u = scores(6, n, seed=7 * n)
+    S[0] = 0.0
+    S[1].clamp_(max=0.0)                      # many best scores
+    S[2] = -S[2].abs() - 0.5
+    S[2, n // 3] = 0.0                        # one
+    S[3] = -INF
+    S[3, n - 2] = 0.0
+    S[4] = 1e-40
+    S[5] = S[5].clamp(max=0.0) - 1e-40
+    for T in (1e-310, 5e-324, 1e-46, [2.0**-149] * 6):
+        for q in (0.9, 0.05, 1.0, [0.5] * 6):
+            for kw in (dict(), dict(top_k=n // 2 + 1), dict(top_k=n // 2 + 1, top_p=0.7), dict(top_p=0.7), dict(top_k=3)):
+                check(S, u, dev, near_ok=True, temperature=T, min_p=q, **kw)
