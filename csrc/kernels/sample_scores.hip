@@ -19,9 +19,10 @@
 // Nothing is sorted.  Thresholds are found over bins of (max s - s) / T, and the scores of the
 // bin that holds the threshold are ranked against each other (up to 256 of them) or split
 // by the bits of the scores.  Weights are computed in 64 bits: an answer depends on
-// which side of u * total a sum of up to N weights falls.  Where masses meet in atomics they
-// are whole multiples of 2^-shift, so their order does not matter; the other sums are in a
-// fixed order.
+// which side of u * total a sum of up to N weights falls.  Where masses meet in atomics (the
+// histograms, which find thresholds, and the scores listed from a threshold's bin) they are
+// whole multiples of a unit taken from the row's own total or the bin's weights, so their order
+// does not matter; the other sums, the draw's above all, are 64-bit ones in a fixed order.
 #include <hip/hip_fp16.h>
 
 #include "common.h"
@@ -38,6 +39,7 @@ constexpr int THREADS = 512;    // of a finishing workgroup
 constexpr int WAVES = THREADS / 64;
 constexpr int PER = BINS / THREADS;   // bins per thread of a search
 constexpr int LIST = 1024;      // scores listed in LDS
+constexpr int LIST_SHIFT = 51;  // unit 2^-51: all their masses together stay below 2^62
 constexpr int RANK = 256;       // listed scores ranked against each other; more are split by bits
 constexpr int SHORT_K = 512;    // top-k up to this lists its candidates
 constexpr int CACHED_SEGS = 64;      // segments of a row that takes one launch
@@ -85,12 +87,13 @@ struct Args {
   int32_t* out;
   float* prob;
   // workspace (long rows)
-  uint64_t* segmass; // [B, nseg] doubles (stats pass) or whole numbers (collect pass)
+  double* segmass;   // [B, nseg]
   uint64_t* hmass;   // [B, BINS]     } rows that may take passes
   Entry* list;       // [B, listcap]  }
   RowState* state;   // [B]           }
   float* segmax;     // [B, nseg]
   int32_t* segtie;   // [B, nseg]
+  uint64_t* listed;  // [B, nseg], of rows whose segments do not fit in LDS
   int listcap;
 };
 
@@ -141,12 +144,15 @@ __device__ __forceinline__ double horner(double p, double f, double c) {
   return r;
 }
 
-// 2^((s - M) c): interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 8 (relative
-// error 1.1e-12: two answers differ where u * total falls that near to a step), times the
-// power of two, which vanishes by itself at the clamp.  (Built from the bits of t + 1.5 * 2^52, with a
-// comparison for what is too small, a pass over 16.7M scores took 28.5 us against 26.)
-__device__ __forceinline__ double weight(float s, float M, double c) {
-  if (M == INFINITY) return s == M ? 1.0 : 0.0;  // (one branch for a whole row)
+// 2^((s - M) c) = p 2^n: interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2], degree 8 (relative
+// error 1.1e-12: two answers differ where u * total falls that near to a step), and the power of two.
+// (Built from the bits of t + 1.5 * 2^52, with a comparison for what is too small, a pass over 16.7M scores
+// took 28.5 us against 26.)
+struct Power {
+  double p;  // in [0.7, 1.42]; 1 at the best score
+  int n;     // -2000 at least, where weights and masses vanish
+};
+__device__ __forceinline__ Power power(float s, float M, double c) {
   const double t0 = ((double)s - (double)M) * c;  // exactly 0 at the best score
   const double t = fmax(t0, -2000.0);  // (a NaN too: a masked score at an endless temperature)
   const double n = __builtin_rint(t);
@@ -160,18 +166,34 @@ __device__ __forceinline__ double weight(float s, float M, double c) {
   p = horner(p, f, 0x1.ebfbdff823cedp-3);
   p = horner(p, f, 0x1.62e42fef84cf0p-1);
   p = horner(p, f, 0x1.0000000000000p+0);
-  return __builtin_ldexp(p, (int)n);
+  return Power{p, (int)n};
+}
+__device__ __forceinline__ double weight(float s, float M, double c) {
+  if (M == INFINITY) return s == M ? 1.0 : 0.0;  // (one branch for a whole row)
+  const Power w = power(s, M, c);
+  return __builtin_ldexp(w.p, w.n);
 }
 
-// w in [0, 1] as a whole multiple of 2^-shift, shift <= 51 (rounded to nearest even)
-__device__ __forceinline__ uint64_t fixed(double w, int shift) {
-  const double magic = 4503599627370496.0;  // 2^52
-  const double d = __builtin_fma(w, (double)(1ull << shift), magic);
-  return (uint64_t)__double_as_longlong(d) & 0x000fffffffffffffull;
+// A weight as a whole multiple of 2^-shift: the significand with its leading one in bit 62, moved down.
+// `place` (0 .. 255, a score's place in its segment; without it the rest below the unit is cut off) spreads
+// the rounding: place / 256 of a unit is added first, so that of equal scores all over a segment so many
+// are rounded up that their sum is right to one unit, and others' errors have no common sign.
+// weight * 2^shift may reach 2^60.
+__device__ __forceinline__ uint64_t mass(float s, float M, double c, int shift, uint32_t place = 0) {
+  if (M == INFINITY) return s == M ? 1ull << shift : 0ull;
+  const Power w = power(s, M, c);
+  const uint64_t bits = (uint64_t)__double_as_longlong(w.p);
+  uint64_t m = (bits << 10 & 0x3fffffffffffffffull) | 1ull << 62;
+  const int down = 63 - shift - w.n - (int)(bits >> 52 & 1);  // (p in [1, 2) or [1/2, 1))
+  m += ((uint64_t)place << 56) >> (64 - min(down, 63));
+  return down > 63 ? 0 : m >> down;
 }
-// a total of weights up to `total` must not pass 2^62
+// The unit for a row whose weights sum up to `total` at most (and 1 at least): all masses together stay
+// below 2^62, and what rounding takes from N scores is about 2^-69 N of a total that is known to a factor
+// of two.  (By the length of the row, as if every weight were 1, a best score over a flat tail loses the
+// tail: each of a million scores cut at 2^-42.)
 __device__ __forceinline__ int shift_for(double total) {
-  return min(51, 61 - (int)((__double_as_longlong(total) >> 52) - 1023));
+  return min(60, 61 - (int)((__double_as_longlong(total) >> 52) - 1023));
 }
 
 // (the median of three with a NaN is the smallest of the others, and a NaN is made by s = M alone, with an
@@ -374,8 +396,8 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   const Row r = row_settings(a, b);
   const int64_t seg0 = ((int64_t)blockIdx.x * 4 + wave_id()) * STAT_SEGS;
   if (seg0 >= a.nseg) return;
-  const bool mass = r.direct() && !r.cut_min;
-  // rows that cut by mass: fp32 sums, to place the histogram's bins
+  const bool exact = r.direct() && !r.cut_min;
+  // rows that cut by mass: fp32 sums, for the unit of their masses and to place the histogram's bins
   const bool rough = r.by_mass();
   const float cf = fminf(fmaxf((float)r.c, 0x1p-100f), 0x1p100f);  // (no NaN from 0 * inf)
   Raw<T> raw[STAT_SEGS];
@@ -388,7 +410,7 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
     unpack<T>(raw[j], v);
     const float m = wave_max(max4(v));
     if (lane == j) ms = m;
-    if (mass) {
+    if (exact) {
       double w = 0;
       if (m > -INFINITY) {
 #pragma unroll
@@ -412,7 +434,7 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   if (lane < STAT_SEGS && seg0 + lane < a.nseg) {
     const int64_t at = (int64_t)b * a.nseg + seg0 + lane;
     a.segmax[at] = ms;
-    if (mass || rough) a.segmass[at] = (uint64_t)__double_as_longlong(ws);
+    if (exact || rough) a.segmass[at] = ws;
   }
 }
 
@@ -767,7 +789,7 @@ __device__ __forceinline__ void collect(Source<T, R>& src, Shared& sh, float M, 
   }
   __syncthreads();
   if (sh.n <= LIST)
-    for (int i = threadIdx.x; i < sh.n; i += THREADS) sh.list[i].w = fixed(weight(score_of(sh.list[i].key()), M, r.c), shift);
+    for (int i = threadIdx.x; i < sh.n; i += THREADS) sh.list[i].w = mass(score_of(sh.list[i].key()), M, r.c, shift);
   __syncthreads();
 }
 
@@ -796,10 +818,9 @@ __device__ __forceinline__ void split(Shared& sh, E each, uint32_t need, uint64_
   }
   const uint32_t cnt = sh.hc[sh.bin];
   uint32_t ties = need;
-  if (S == BY_MASS) {  // tie number j stays while above + j w < target
-    const uint64_t w = cnt ? sh.hm[sh.bin] / cnt : 0;
-    const double room = target - (double)above_m;
-    ties = w == 0 || room > (double)w * (double)cnt ? cnt : (uint32_t)fmax(0.0, ceil(room / (double)w));
+  if (S == BY_MASS) {  // tie number j stays while above + j w < target, w = all / cnt
+    const double all = (double)sh.hm[sh.bin], room = target - (double)above_m;
+    ties = room > all ? cnt : all > 0 ? (uint32_t)fmax(0.0, ceil(room * ((double)cnt / all))) : 0;
     if (above_m == 0 && ties == 0) ties = 1;
   }
   __syncthreads();
@@ -869,35 +890,19 @@ __device__ __forceinline__ void no_answer(const Args& a, int b) {
 
 // ---- a draw over a row's segments, given what stays: keys above t and the first `ties` equal to t
 
-// a kept score's mass, in the unit of the segments' masses
-struct AsDouble {
-  typedef double V;
-  float M;
-  double c;
-  __device__ double operator()(float s) const { return weight(s, M, c); }
-};
-struct AsFixed {
-  typedef uint64_t V;
-  float M;
-  double c;
-  int shift;
-  __device__ uint64_t operator()(float s) const { return fixed(weight(s, M, c), shift); }
-};
-
-template <typename V>
 struct Found {
   int64_t seg;     // -1: no segment has mass
-  V before;        // mass of the segments before it
+  double before;   // mass of the segments before it
   uint32_t ties;   // ties in the segments before it
   double total, target;
 };
 
 // The segment in which u * total falls: every lane sums a run of segments, the lane whose run holds
 // the target has its wave walk it.  get(seg, mass, ties): a segment's mass of keys above t and its
-// count of ties (false: nothing of it stays).
-template <typename V, typename G>
-__device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& sh, uint32_t ties, V wt, G get, V* tmp_v,
-                                                 Found<V>* found) {
+// count of ties (false: nothing of it stays); wt: a tie's weight.
+template <typename G>
+__device__ __forceinline__ Found find_segment(const Args& a, int b, Shared& sh, uint32_t ties, double wt, G get, Found* found) {
+  double* tmp_v = sh.scan_d;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t run = (a.nseg + THREADS - 1) / THREADS;
   const int64_t s0 = min(run * threadIdx.x, a.nseg), s1 = min(s0 + run, a.nseg);
@@ -906,41 +911,41 @@ __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& s
     uint32_t c = 0;
 #pragma unroll 4
     for (int64_t s = s0; s < s1; ++s) {
-      V m;
+      double m;
       uint32_t x = 0;
       if (get(s, m, x)) c += x;
     }
     tie0 = block_scan(c, sh.scan_c, tall) - c;
   }
-  V sum = 0;
+  double sum = 0;
   uint32_t tie = tie0;
 #pragma unroll 8
   for (int64_t s = s0; s < s1; ++s) {
-    V m = 0;
+    double m = 0;
     uint32_t x = 0;
     if (!get(s, m, x)) { m = 0; x = 0; }
     if (ties) {
-      m += (V)(tie < ties ? min(ties - tie, x) : 0u) * wt;
+      m += (tie < ties ? min(ties - tie, x) : 0u) * wt;
       tie += x;
     }
     sum += m;
   }
-  const V in_wave = wave_scan(sum);
+  const double in_wave = wave_scan(sum);
   if (threadIdx.x == 0) found->seg = -1;
   __syncthreads();
   if (lane == 63) tmp_v[wave] = in_wave;
   __syncthreads();
-  V all = 0;
-  for (int w = 0; w < WAVES; ++w) all += tmp_v[w];
-  const double total = (double)all, target = (double)a.u[b] * total;
+  double total = 0;
+  for (int w = 0; w < WAVES; ++w) total += tmp_v[w];
+  const double target = (double)a.u[b] * total;
   int pick = -1, last = -1;
-  V cum = 0, pick_before = 0, last_before = 0;
+  double cum = 0, pick_before = 0, last_before = 0;
   for (int w = 0; w < WAVES; ++w) {
-    const V m = tmp_v[w];
+    const double m = tmp_v[w];
     if (m > 0) {
       last = w;
       last_before = cum;
-      if (pick < 0 && (double)(cum + m) > target) { pick = w; pick_before = cum; }
+      if (pick < 0 && cum + m > target) { pick = w; pick_before = cum; }
     }
     cum += m;
   }
@@ -949,21 +954,21 @@ __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& s
   if (wave == (over ? last : pick)) {
     // the first of 64 values, in order after `before`, that has mass and passes the target (or the last
     // with mass): lane -1 if none has mass
-    const auto choose = [&](V m, V before, bool& hit) {
-      const V upto = before + wave_scan(m);
-      const uint64_t has = __ballot(m > 0), hits = over ? 0 : __ballot(m > 0 && (double)upto > target);
+    const auto choose = [&](double m, double before, bool& hit) {
+      const double upto = before + wave_scan(m);
+      const uint64_t has = __ballot(m > 0), hits = over ? 0 : __ballot(m > 0 && upto > target);
       hit = hits != 0;
       return hits ? __ffsll((unsigned long long)hits) - 1 : has ? 63 - __clzll(has) : -1;
     };
     bool hit;
-    V before = over ? last_before : pick_before;
+    double before = over ? last_before : pick_before;
     const int l = choose(sum, before, hit);
     before += lane_value(in_wave, l) - lane_value(sum, l);
     tie = lane_value(tie0, l);
     const int64_t first = run * (wave * 64 + l), end = min(first + run, a.nseg);
-    Found<V> f{-1, before, 0, total, over ? INFINITY : target};
+    Found f{-1, before, 0, total, over ? INFINITY : target};
     for (int64_t s = first; s < end; s += 64) {
-      V m = 0;
+      double m = 0;
       uint32_t x = 0;
       if (s + lane >= end || !get(s + lane, m, x)) { m = 0; x = 0; }
       uint32_t tb = tie;
@@ -971,10 +976,10 @@ __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& s
         const uint32_t scan = wave_scan(x);
         tb = tie + scan - x;
         tie += lane_value(scan, 63);
-        m += (V)(tb < ties ? min(ties - tb, x) : 0u) * wt;
+        m += (tb < ties ? min(ties - tb, x) : 0u) * wt;
       }
       const int at = choose(m, before, hit);
-      const V upto = wave_scan(m);
+      const double upto = wave_scan(m);
       if (at >= 0) {
         f.seg = s + at;
         f.before = before + (lane_value(upto, at) - lane_value(m, at));
@@ -990,31 +995,30 @@ __device__ __forceinline__ Found<V> find_segment(const Args& a, int b, Shared& s
 }
 
 // One wave: the first kept score of the segment at which the mass passes the target (or its last).
-template <typename W, typename V = typename W::V>
-__device__ __forceinline__ void pick_in_segment(const Args& a, int b, const Found<V>& f, const float v[4], const Row& r,
-                                                W wt_of, uint32_t t, uint32_t ties) {
+__device__ __forceinline__ void pick_in_segment(const Args& a, int b, const Found& f, const float v[4], const Row& r, float M,
+                                                uint32_t t, uint32_t ties) {
   const int lane = threadIdx.x & 63;
   uint32_t c = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) c += v[j] > -INFINITY && key_of(v[j]) == t;
   uint32_t tie = f.ties + wave_scan(c) - c;
-  V w[4], m = 0;
+  double w[4], m = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t key = key_of(v[j]);
-    bool kept = v[j] > -INFINITY && (key > t || (key == t && tie < ties));
+    const bool kept = v[j] > -INFINITY && (key > t || (key == t && tie < ties));
     tie += v[j] > -INFINITY && key == t;
-    if (kept && r.cut_min) kept = weight(v[j], wt_of.M, r.c) >= r.minp;
-    w[j] = kept ? wt_of(v[j]) : V(0);
+    w[j] = kept ? weight(v[j], M, r.c) : 0.0;
+    if (r.cut_min && w[j] < r.minp) w[j] = 0;
     m += w[j];
   }
-  V cum = f.before + (wave_scan(m) - m);
+  double cum = f.before + (wave_scan(m) - m);
   int hit = -1, end = -1;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     cum += w[j];
     if (w[j] > 0) {
-      if (hit < 0 && (double)cum > f.target) hit = j;
+      if (hit < 0 && cum > f.target) hit = j;
       end = j;
     }
   }
@@ -1023,19 +1027,18 @@ __device__ __forceinline__ void pick_in_segment(const Args& a, int b, const Foun
   if (lane == win) {
     const int j = hits ? hit : end;
     a.out[b] = (int32_t)(f.seg * SEG + lane * 4 + j);
-    if (a.prob) a.prob[b] = (float)((double)(j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]) / f.total);
+    if (a.prob) a.prob[b] = (float)((j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]) / f.total);
   }
 }
 
 template <int T, int R>
 __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>& src, Shared& sh, const Row& r, float M,
                                               uint32_t t, uint32_t ties, double* segmass, int32_t* segtie, bool have_mass) {
-  __shared__ Found<double> found;
+  __shared__ Found found;
   const float bound = score_of(max(t, KEY_NONE));
-  const AsDouble w_of{M, r.c};
   double wt = 0;
   if (ties) {
-    wt = w_of(bound);
+    wt = weight(bound, M, r.c);
     if (r.cut_min && wt < r.minp) { wt = 0; ties = 0; }
   }
   if (!have_mass)
@@ -1046,7 +1049,7 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
       for (int j = 0; j < 4; ++j) {
         const uint32_t key = key_of(v[j]);
         if (v[j] > -INFINITY && key > t) {
-          const double w = w_of(v[j]);
+          const double w = weight(v[j], M, r.c);
           m += !r.cut_min || w >= r.minp ? w : 0.0;
         }
         c += v[j] > -INFINITY && key == t;
@@ -1056,17 +1059,17 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
       if (src.lane == 0) { segmass[seg] = m; segtie[seg] = (int32_t)c; }
     });
   __syncthreads();
-  const Found<double> f = find_segment<double>(
+  const Found f = find_segment(
       a, b, sh, ties, wt,
       [&](int64_t s, double& m, uint32_t& c) {
         const float x = src.segmax(s);
         if (!(x >= bound) || x == -INFINITY) return false;
         m = segmass[s];
-        if (have_mass) m *= w_of(x);
+        if (have_mass) m *= weight(x, M, r.c);
         else c = (uint32_t)segtie[s];
         return true;
       },
-      sh.scan_d, &found);
+      &found);
   if (f.seg < 0) {
     no_answer(a, b);
     return;
@@ -1079,23 +1082,31 @@ __device__ __forceinline__ void draw_from_row(const Args& a, int b, Source<T, R>
     } else {
       load_seg<T>(a, b, f.seg, src.lane, v);
     }
-    pick_in_segment(a, b, f, v, r, w_of, t, ties);
+    pick_in_segment(a, b, f, v, r, M, t, ties);
   }
+}
+
+// the unit of a row's masses from its segments' largest scores, each taken for the whole segment
+template <int T, int R>
+__device__ __forceinline__ int shift_from_maxima(const Args& a, const Source<T, R>& src, const Row& r, float M) {
+  double sum = 0;
+  for (int64_t s = src.lane; s < a.nseg; s += 64) sum += weight(src.segmax(s), M, r.c);
+  return shift_for(SEG * wave_sum(sum));
 }
 
 // A row from its scores alone (rows of one launch; long rows with a long top-k, or whose lists ran
 // over): histogram, threshold of top-k, threshold of top-p, draw.
 template <int T, int R>
 __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R>& src, Shared& sh, const Row& r, float M,
-                                               double* segmass, int32_t* segtie) {
+                                               int shift, double* segmass, int32_t* segtie) {
   const float cb = (float)(r.c * 32);  // 32 bins to an octave of weight
-  const int shift = shift_for((double)a.N);
+  const uint32_t place = src.lane * 4;
   const auto any = [](float) { return true; };
   clear_hist(sh);
   src.each(sh, any, [&](int64_t, const float* v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint64_t w = r.cut_p ? fixed(weight(v[j], M, r.c), shift) : 0;
+      const uint64_t w = r.cut_p ? mass(v[j], M, r.c, shift, place + j) : 0;
       hist_add<true, true>(sh.hc, sh.hm, v[j] > -INFINITY, bin_of(v[j], M, cb), w);
     }
   });
@@ -1106,7 +1117,8 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
       src.each(sh, [=](float m) { return bin_of(m, M, cb) <= bin; }, [&](int64_t, const float* v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          g(v[j] > -INFINITY && bin_of(v[j], M, cb) == bin, key_of(v[j]), fixed(weight(v[j], M, r.c), shift));
+          g(v[j] > -INFINITY && bin_of(v[j], M, cb) == bin, key_of(v[j]),
+            mass(v[j], M, r.c, shift, place + j));
       });
     };
   };
@@ -1150,7 +1162,7 @@ __device__ __forceinline__ void finish_general(const Args& a, int b, Source<T, R
         const uint32_t need = (uint32_t)(r.k - cbefore);
         if (n <= LIST) split<BY_COUNT_WITH_MASS>(sh, [&](auto g) { each_listed(sh.list, n, g); }, need, kbefore, 0.0, 0);
         else split<BY_COUNT_WITH_MASS>(sh, of_bin(kbin), need, kbefore, 0.0, 0);
-        total = sh.before_m + (uint64_t)sh.ties * fixed(weight(score_of(sh.kmin), M, r.c), shift);
+        total = sh.before_m + (uint64_t)(sh.ties * __builtin_ldexp(weight(score_of(sh.kmin), M, r.c), shift));
       }
       t = sh.kmin;
       ties = sh.ties;
@@ -1206,7 +1218,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = wave_id();
   const Row r = row_settings(a, b);
   constexpr bool own = R != ROW_LONG;
-  double* segmass = own ? small_mass : (double*)a.segmass + (int64_t)b * a.nseg;
+  double* segmass = own ? small_mass : a.segmass + (int64_t)b * a.nseg;
   int32_t* segtie = own ? small_tie : a.segtie + (int64_t)b * a.nseg;
   Source<T, R> src(a, b, small_max, own ? nullptr : a.segmax + (int64_t)b * a.nseg);
   float m = -INFINITY;
@@ -1252,13 +1264,13 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
       for (int64_t i = threadIdx.x; i < a.nseg; i += THREADS)
         if (src.segmax(i) > -INFINITY) sum += segmass[i] * weight(src.segmax(i), M, r.c);
       block_scan(sum, sh.scan_d, total);
+      st.shift = shift_for(2 * total);
       // N scores below (1 - p) total / N hold less than (1 - p) total: the threshold is not among
       // them, and the bins but the last span the octaves above that
       const double least = fmax((1 - r.p) * total / (double)a.N, 0x1p-60);
       const double octaves = fmax(-log2(least), 0.0) + 0.125;
       st.mode = BY_TOP_P;
       st.cb = (float)(r.c * (BINS - 1) / octaves);
-      st.shift = shift_for(2 * total);
     } else if (r.k > 0 && !r.short_k()) {
       // the bins span eight times the range of the segments' maxima, which for scores of any common
       // distribution is beyond their bulk; a threshold in the last bin, of all below, still stands
@@ -1269,11 +1281,9 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
       const float range = 8 * (M - low);
       st.mode = BY_TOP_K;
       st.cb = range > 0 && range < INFINITY ? (float)(BINS - 1) / range : 32.f;
-      st.shift = shift_for((double)a.N);
       st.target = (double)r.k;
     } else if (r.direct() && r.cut_min) {
       st.mode = NO_CUT;
-      st.shift = shift_for((double)a.N);
       st.bin = BINS;
     }
     if (threadIdx.x == 0) a.state[b] = st;
@@ -1311,7 +1321,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
     const bool all = sh.before_c + sh.hc[sh.bin] < (uint32_t)r.k || sh.bin == BINS - 1 || !(M < INFINITY);
     const double low = (double)M - (double)(sh.bin + 1) / (double)cb * (1 + 1e-6) - fabs((double)M) * 1e-6;
     const float cut = all ? -INFINITY : (float)low;
-    collect<T, R>(src, sh, M, r, 51, [=](float x) { return x >= cut; }, [=](float x) { return x >= cut; });
+    collect<T, R>(src, sh, M, r, LIST_SHIFT, [=](float x) { return x >= cut; }, [=](float x) { return x >= cut; });
     const int n = sh.n;
     if (n <= RANK) {
       Slot s = rank_list(sh, n, r.k, 0);
@@ -1324,7 +1334,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
       split<BY_COUNT_WITH_MASS>(sh, listed, (uint32_t)r.k, 0, 0.0, 0);
       uint32_t t = sh.kmin, ties = sh.ties;
       if (r.cut_p) {
-        const uint64_t total = sh.before_m + (uint64_t)ties * fixed(weight(score_of(t), M, r.c), 51);
+        const uint64_t total = sh.before_m + (uint64_t)ties * mass(score_of(t), M, r.c, LIST_SHIFT);
         split<BY_MASS>(sh, listed, 0, 0, r.p * (double)total, t);
         ties = sh.kmin == t ? min(ties, sh.ties) : sh.ties;
         t = sh.kmin;
@@ -1333,7 +1343,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(Args a, int passes) {
       return;
     }
   }
-  finish_general<T, R>(a, b, src, sh, r, M, segmass, segtie);
+  finish_general<T, R>(a, b, src, sh, r, M, shift_from_maxima<T, R>(a, src, r, M), segmass, segtie);
 }
 
 // ---- a round of passes over long rows: counts or masses by bin, then what lies above the threshold's
@@ -1350,6 +1360,7 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
   const float floor_score = score_of(st.floor_key);
   for (int i = threadIdx.x; i < BINS; i += THREADS) hm[i] = 0;
   __syncthreads();
+  const uint32_t place = lane * 4;
   uint64_t rest = 0;  // the last bin's: scores that can hardly hold the threshold
   const int64_t s1 = min((int64_t)(blockIdx.x + 1) * PASS_SEGS, a.nseg);
   for (int64_t seg0 = (int64_t)blockIdx.x * PASS_SEGS + wave; seg0 < s1; seg0 += 4 * WAVES) {
@@ -1366,7 +1377,7 @@ __global__ void __launch_bounds__(THREADS) hist_kernel(Args a) {
         const int bin = bin_of(v, st.M, st.cb);
         const bool in = v > floor_score;
         uint64_t w = in;
-        if (!counts) w = in ? fixed(weight(v, st.M, r.c), st.shift) : (uint64_t)0;
+        if (!counts) w = in ? mass(v, st.M, r.c, st.shift, place + i) : (uint64_t)0;
         if (in && bin < BINS - 1) atomicAdd(&hm[bin], (unsigned long long)w);
         else rest += w;
       }
@@ -1435,7 +1446,7 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
   const auto put = [&](uint32_t at, Entry e) {
-    e.w = fixed(weight(score_of(e.key()), st.M, r.c), st.shift);
+    if (st.mode == BY_TOP_P) e.w = mass(score_of(e.key()), st.M, r.c, st.shift);  // (counts need none)
     if (at < (uint32_t)a.listcap) a.list[(int64_t)b * a.listcap + at] = e;
   };
   for (int g = 0; g < PASS_SEGS / WAVES; g += 4) {
@@ -1464,10 +1475,10 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
         if (up[i]) above[wave][n + __popcll(mask & ((1ull << lane) - 1))] = x[i];
         n += __popcll(mask);
       }
-      uint64_t sum = 0;
+      double sum = 0;
       for (int i = lane; i < n; i += 64) {
         const double w = weight(above[wave][i], st.M, r.c);
-        if (!drop || w >= r.minp) sum += fixed(w, st.shift);
+        if (!drop || w >= r.minp) sum += w;
       }
       sum = wave_sum(sum);
       if (lane == 0) a.segmass[(int64_t)b * a.nseg + seg] = sum;
@@ -1496,17 +1507,24 @@ __global__ void __launch_bounds__(THREADS) collect_kernel(Args a) {
   for (int i = threadIdx.x; i < n; i += THREADS) put((uint32_t)(count + i), listed[i]);
 }
 
-// The threshold inside the listed bin; then the draw over whole-number masses, or, after top-k where
-// top-p is to follow, the state of a second round.
+// The unit 2^-shift for sums of listed scores' weights, by the bound that their bin sets: (M - s) cb is at least its number,
+// but for the rounding of the two.  A listcap of masses of up to 2^46 stays below 2^62.
+__device__ __forceinline__ int listed_shift(const RowState& st, const Row& r) {
+  const double gap = st.bin ? fmin((double)st.bin / (double)st.cb, 3.4e38) : 0.0;  // (M - s may have passed fp32's range)
+  return 46 + (int)fmin(fmax(gap * (1 - 1e-6) * r.c, 0.0), 900.0);
+}
+
+// The threshold inside the listed bin; then the draw, or, after top-k where top-p is to follow, the state of a
+// second round.
 template <int T>
 __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
   __shared__ Shared sh;
-  __shared__ Found<uint64_t> found;
+  __shared__ Found found;
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const RowState st = a.state[b];
   if (st.mode == IDLE) return;
   const Row r = row_settings(a, b);
-  uint64_t* segmass = a.segmass + (int64_t)b * a.nseg;
+  double* segmass = a.segmass + (int64_t)b * a.nseg;
   __syncthreads();
   if (threadIdx.x == 0) a.state[b].mode = IDLE;
   if (st.bin < BINS && st.listed > (uint32_t)a.listcap) {  // more than a list of equal or near-equal scores: the row again
@@ -1515,21 +1533,22 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
     if (src.kept())
       for (int i = threadIdx.x; i < a.nseg; i += THREADS) maxima[i] = src.in_memory[i];
     __syncthreads();
-    finish_general<T, ROW_LONG>(a, b, src, sh, r, st.M, (double*)segmass, a.segtie + (int64_t)b * a.nseg);
+    const int shift = r.by_mass() ? st.shift : shift_from_maxima<T, ROW_LONG>(a, src, r, st.M);
+    finish_general<T, ROW_LONG>(a, b, src, sh, r, st.M, shift, segmass, a.segtie + (int64_t)b * a.nseg);
     return;
   }
   const int n = st.bin < BINS ? (int)st.listed : 0;
   const Entry* list = a.list + (int64_t)b * a.listcap;
-  const AsFixed w_of{st.M, r.c, st.shift};
+  const int lshift = listed_shift(st, r);
   const double target = st.target < 0 ? st.part : st.target;
   uint32_t t, ties;
   if (st.bin == BINS) {  // everything above the floor, and of its ties those that top-p's part still takes
     t = st.floor_key;
     ties = 0;
     if (st.mode == BY_TOP_P) {
-      const uint64_t w = w_of(score_of(t));
+      const double w = __builtin_ldexp(weight(score_of(t), st.M, r.c), st.shift);
       const double room = target - (double)st.all;
-      ties = w == 0 || room > (double)w * (double)st.ties ? st.ties : (uint32_t)fmax(0.0, ceil(room / (double)w));
+      ties = w == 0 || room > w * (double)st.ties ? st.ties : (uint32_t)fmax(0.0, ceil(room / w));
       if (st.all == 0 && ties == 0) ties = 1;
       ties = min(ties, st.ties);
     }
@@ -1551,14 +1570,16 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
     ties = sh.ties;
     if (counts && r.cut_p) {
       // what top-k leaves: the bins above, the listed scores above t, the ties
-      uint64_t mine = 0, total;
+      double mine = 0, total;
       for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS) mine += segmass[s];
+      uint64_t in_bin = 0, all_in_bin;
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const Entry e = list[i];
-        if (e.key() > t) mine += e.w;
+        if (e.key() > t) in_bin += mass(score_of(e.key()), st.M, r.c, lshift);
       }
-      block_scan(mine, sh.scan_m, total);
-      total += (uint64_t)ties * w_of(score_of(t));
+      block_scan(mine, sh.scan_d, total);
+      block_scan(in_bin, sh.scan_m, all_in_bin);
+      total += __builtin_ldexp((double)all_in_bin, -lshift) + ties * weight(score_of(t), st.M, r.c);
       for (int i = threadIdx.x; i < BINS; i += THREADS) a.hmass[(int64_t)b * BINS + i] = 0;
       if (threadIdx.x == 0) {
         RowState next = st;
@@ -1567,7 +1588,8 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
         next.cb = range > 0 && range < INFINITY ? (float)(BINS - 2) / range : 32.f;
         next.floor_key = t;
         next.ties = ties;
-        next.target = fmax(r.p, 0.0) * (double)total;
+        next.shift = shift_for(2 * total);
+        next.target = __builtin_ldexp(fmax(r.p, 0.0) * total, next.shift);
         next.above = 0;
         next.bin = 0;
         next.listed = 0;
@@ -1576,21 +1598,22 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
       return;
     }
   }
-  uint64_t wt = w_of(score_of(t));
-  if (r.cut_min && weight(score_of(t), st.M, r.c) < r.minp) { wt = 0; ties = 0; }
-  // Listed scores above t add to their segments' masses, ties are counted per segment: in LDS where
-  // they fit, else in the workspace.
+  double wt = weight(score_of(t), st.M, r.c);
+  if (r.cut_min && wt < r.minp) { wt = 0; ties = 0; }
+  // Listed scores above t add to their segments' masses (as whole numbers: their order does not matter), ties are
+  // counted per segment: in LDS where they fit, else in the workspace.
   const auto add = [&](auto plus_mass, auto plus_tie) {
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const Entry e = list[i];
       if (e.key() > t) {
-        if (!r.cut_min || weight(score_of(e.key()), st.M, r.c) >= r.minp) plus_mass(e.idx() / SEG, e.w);
+        const float x = score_of(e.key());
+        if (!r.cut_min || weight(x, st.M, r.c) >= r.minp) plus_mass(e.idx() / SEG, mass(x, st.M, r.c, lshift));
       } else if (e.key() == t && ties) {
         plus_tie(e.idx() / SEG);
       }
     }
   };
-  Found<uint64_t> f;
+  Found f;
   if (a.nseg <= KEPT) {
     __shared__ unsigned long long more[KEPT];
     uint32_t* tied = (uint32_t*)sh.hm;
@@ -1603,29 +1626,33 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
     __syncthreads();
     add([&](int s, uint64_t w) { atomicAdd(more + s, (unsigned long long)w); }, [&](int s) { atomicAdd(tied + s, 1u); });
     __syncthreads();
-    f = find_segment<uint64_t>(a, b, sh, ties, wt, [&](int64_t s, uint64_t& m, uint32_t& c) {
-      m = segmass[s] + more[s];
+    f = find_segment(a, b, sh, ties, wt, [&](int64_t s, double& m, uint32_t& c) {
+      m = segmass[s] + __builtin_ldexp((double)more[s], -lshift);
       c = tied[s];
       return true;
-    }, sh.scan_m, &found);
+    }, &found);
   } else {
     // agent-scope accesses meet in the L2 that this one workgroup works through; the waits put the
     // zeros before the sums and the sums before the reads
     int32_t* segtie = a.segtie + (int64_t)b * a.nseg;
+    uint64_t* more = a.listed + (int64_t)b * a.nseg;
     if (st.bin < BINS)
-      for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS)
+      for (int64_t s = threadIdx.x; s < a.nseg; s += THREADS) {
         __hip_atomic_store(segtie + s, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(more + s, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    add([&](int s, uint64_t w) { atomicAdd((unsigned long long*)segmass + s, (unsigned long long)w); },
+    add([&](int s, uint64_t w) { atomicAdd((unsigned long long*)more + s, (unsigned long long)w); },
         [&](int s) { atomicAdd(segtie + s, 1); });
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    f = find_segment<uint64_t>(a, b, sh, ties, wt, [&](int64_t s, uint64_t& m, uint32_t& c) {
-      m = __hip_atomic_load(segmass + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    f = find_segment(a, b, sh, ties, wt, [&](int64_t s, double& m, uint32_t& c) {
+      m = segmass[s];
+      if (st.bin < BINS) m += __builtin_ldexp((double)__hip_atomic_load(more + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), -lshift);
       c = (uint32_t)__hip_atomic_load(segtie + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       return true;
-    }, sh.scan_m, &found);
+    }, &found);
   }
   if (f.seg < 0) {
     no_answer(a, b);
@@ -1634,7 +1661,7 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
   if (threadIdx.x < 64) {
     float v[4];
     load_seg<T>(a, b, f.seg, lane, v);
-    pick_in_segment(a, b, f, v, r, w_of, t, ties);
+    pick_in_segment(a, b, f, v, r, st.M, t, ties);
   }
 }
 
@@ -1676,7 +1703,7 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 FPS_API int64_t fps_sample_scores_ws_bytes(int64_t B, int64_t N) {
   if (B <= 0 || N <= kShortRow) return 0;
   const int64_t nseg = (N + SEG - 1) / SEG;
-  return B * (list_cap(N) * (int64_t)sizeof(Entry)) + round16(B * sizeof(RowState)) + B * BINS * 8 + B * nseg * 16 + 16;
+  return B * (list_cap(N) * (int64_t)sizeof(Entry)) + round16(B * sizeof(RowState)) + B * BINS * 8 + B * nseg * (nseg > KEPT ? 24 : 16) + 16;
 }
 
 // s [B, N] (row stride ld, type 0 fp32 / 1 bf16 / 2 fp16); u [B]; temperature / top_k / top_p /
@@ -1697,7 +1724,7 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
   a.top_p = top_p; a.top_p0 = top_p0;
   a.min_p = min_p; a.min_p0 = min_p0;
   a.out = out; a.prob = prob;
-  a.segmass = nullptr; a.hmass = nullptr; a.list = nullptr; a.state = nullptr; a.segmax = nullptr; a.segtie = nullptr;
+  a.segmass = nullptr; a.hmass = nullptr; a.list = nullptr; a.state = nullptr; a.segmax = nullptr; a.segtie = nullptr; a.listed = nullptr;
   a.listcap = 0;
   int rounds = 0;
   if (N > kShortRow) {
@@ -1707,7 +1734,8 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
     a.list = (Entry*)p; p += (int64_t)B * a.listcap * sizeof(Entry);
     a.state = (RowState*)p; p += round16(B * sizeof(RowState));
     a.hmass = (uint64_t*)p; p += (int64_t)B * BINS * 8;
-    a.segmass = (uint64_t*)p; p += (int64_t)B * a.nseg * 8;
+    a.segmass = (double*)p; p += (int64_t)B * a.nseg * 8;
+    if (a.nseg > KEPT) { a.listed = (uint64_t*)p; p += (int64_t)B * a.nseg * 8; }
     a.segmax = (float*)p; p += (int64_t)B * a.nseg * 4;
     a.segtie = (int32_t*)p;
     // which rounds of passes can a row need?  (scalars decide here, per-row settings on the device)

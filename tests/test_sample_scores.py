@@ -6,6 +6,9 @@ oracle says how near it came, both sides' sums are good to about 1e-12); such a 
 would say nothing about which side is right.  Where the steps are exact in both (equal
 scores), the borders themselves are tested.
 """
+import math
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -361,3 +364,90 @@ def test_min_p_next_to_a_best_score_of_zero(dev, n):
         for q in (0.9, 0.05, 1.0, [0.5] * 6):
             for kw in (dict(), dict(top_k=n // 2 + 1), dict(top_k=n // 2 + 1, top_p=0.7), dict(top_p=0.7), dict(top_k=3)):
                 check(S, u, dev, near_ok=True, temperature=T, min_p=q, **kw)
+
+
+def flat_tail(n, B, tail_mass, seed):
+    """Rows of one best score over equal ones, which hold `tail_mass` of its weight together."""
+    g = torch.Generator().manual_seed(seed)
+    S = torch.full((B, n), float(np.log(tail_mass / (n - 1))))
+    S[torch.arange(B), torch.randint(0, n, (B,), generator=g)] = 0.0
+    S[0] = S[0, 1]
+    S[0, 0] = 0.0
+    return S
+
+
+def tail_row(n, best, w, u, top_k=0, top_p=1.0, min_p=0.0):
+    """(index, probability, distance to a step in steps) in whole and rational numbers: ``n - 1`` scores of weight ``w`` (all
+    above ``min_p``) around one of weight 1.  (A running sum loses it: n roundings at 2^-64 are a tenth of a step.)"""
+    w, u, kept = Fraction(w), Fraction(u), (top_k or n) - 1
+    off = Fraction(1, 2)
+    if top_p < 1:
+        border = (Fraction(top_p) * (1 + kept * w) - 1) / w  # tie number j stays while j < border
+        off = min(off, abs(border - round(border)))
+        kept = min(kept, max(0, math.ceil(border)))
+    total = 1 + kept * w
+    target, before = u * total, min(best, kept)
+    if target < before * w or target >= before * w + 1:
+        x = target / w if target < before * w else (target - 1) / w
+        m = min(math.floor(x), kept - 1)
+        return m + (m >= best), float(w / total), float(min(off, abs(x - round(x))))
+    return best, float(1 / total), float(min(off, (target - before * w) / w, (before * w + 1 - target) / w))
+
+
+def check_tail(n, dev, tail_mass, B=4):
+    """The draws that fall into the tail.  A step there is far below 1e-10 of the total, and still one index: the sums
+    have to be right to a hundredth of it."""
+    S = flat_tail(n, B, tail_mass, seed=n)
+    k = n - n // 10
+    w = float(np.exp(np.float64(S[0, 1])))
+    p, pk = ((1 + (int(0.6 * kept) + 0.5) * w) / (1 + (kept - 1) * w) for kept in (n, k))  # half way between two steps
+    for kw in (dict(), dict(top_k=k), dict(min_p=1e-30), dict(top_p=p), dict(top_k=k, top_p=pk), dict(top_k=k, min_p=1e-30),
+               dict(top_k=400, min_p=1e-30), dict(top_k=k, top_p=pk, min_p=1e-30)):
+        tried = 0
+        for part in (0.13, 0.29, 0.37, 0.49, 0.52, 0.58):
+            u = torch.full((B,), float(1 - part * tail_mass / (1 + tail_mass)))
+            idx, prob = ops.sample_scores(S.to(dev), u.to(dev), with_prob=True, **kw)
+            for b in range(B):
+                want, pr, near = tail_row(n, int(S[b].argmax()), w, float(u[b]), **kw)
+                if near < 0.01:
+                    continue  # next to a step
+                tried += 1
+                assert int(idx[b]) == want, (b, int(idx[b]), want, near, kw)
+                assert abs(float(prob[b]) - pr) <= 2.0**-23 * pr, (b, float(prob[b]), pr, kw)
+        assert tried >= 1
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("n", [1000, 9000, 16000, 40000, 70001])
+@pytest.mark.parametrize("tail_mass", [0.3, 2.0**-14, 2.0**-19])
+def test_a_best_score_over_a_flat_tail(dev, n, tail_mass):
+    check_tail(n, dev, tail_mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1_000_000, 1_200_003])
+@pytest.mark.parametrize("tail_mass", [0.3, 1.4e-5, 2.0**-21])
+def test_a_best_score_over_a_long_flat_tail(n, tail_mass):
+    check_tail(n, "cuda", tail_mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,p_best", [(25, 0.99977), (28, 0.985)])
+def test_the_tail_of_very_long_rows(bits, p_best):
+    """One best score, the others together 1 - p_best: their number times a weight far below 2^-31."""
+    n = 1 << bits
+    tail = torch.tensor(np.log((1 / p_best - 1) / n)).bfloat16()
+    S = torch.empty(1, n, dtype=torch.bfloat16, device="cuda")
+    S[:] = tail
+    S[0, 0] = 0
+    w = float(np.exp(np.float64(tail.float())))
+    for kw, kept in ((dict(top_k=n // 2), n // 2), (dict(min_p=1e-12), n), (dict(), n),
+                     (dict(top_k=n // 2, min_p=1e-12), n // 2)):
+        total = 1 + (kept - 1) * w
+        i, p = ops.sample_scores(S, torch.tensor([0.5], device="cuda"), with_prob=True, **kw)
+        assert int(i[0]) == 0 and abs(float(p[0]) - 1 / total) <= 2.0**-23
+        u = float(torch.tensor(1 - 0.3 * (total - 1) / total).float())
+        i, p = ops.sample_scores(S, torch.tensor([u], device="cuda"), with_prob=True, **kw)
+        # weights are good to 1.1e-12 each, sums to 2^-61 for each segment of 256
+        assert abs(int(i[0]) - ((u * total - 1) / w + 1)) <= 1.5
+        assert abs(float(p[0]) * total / w - 1) <= 2.0**-23
