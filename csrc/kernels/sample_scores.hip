@@ -839,45 +839,50 @@ __device__ __forceinline__ void each_listed(const Entry* list, int n, G g) {
   }
 }
 
-// Draw from the kept entries of the list (n <= RANK), in index order.
+// Draw from the kept entries of the list (n <= RANK), in index order: their weights put in that order and summed.
 __device__ __forceinline__ void draw_from_list(const Args& a, int b, Shared& sh, int n, Slot s, const Row& r, float M) {
-  const int i = threadIdx.x;
-  Entry mine{0, 0};
-  if (i < n) mine = sh.list[i];
-  if (s.kept && r.cut_min) s.kept = weight(score_of(mine.key()), M, r.c) >= r.minp;
-  if (!s.kept) mine.w = 0;
-  if (i < RANK) sh.before[i] = 0;
-  if (i == 0) { sh.kmin = 0xffffffffu; sh.ties = 0xffffffffu; }
-  uint64_t all;
-  block_scan(mine.w, sh.scan_m, all);  // (its barriers also close the reads of the list)
-  if (i < n) sh.list[i].w = mine.w;
+  const int i = threadIdx.x, lane = i & 63, wave = wave_id();
+  uint32_t at = 0;
+  double mine = 0;
+  if (i < n) {
+    at = (uint32_t)sh.list[i].idx();
+    mine = s.kept ? weight(score_of(sh.list[i].key()), M, r.c) : 0.0;
+    if (r.cut_min && mine < r.minp) mine = 0;
+  }
+  if (i < RANK) sh.rank[i] = 0;
   __syncthreads();
-  const double total = (double)all, target = (double)a.u[b] * total;
   const Share w = share_list(n);
-  uint32_t idx = 0;
+  uint32_t idx = 0, place = 0;
   if (w.i < n) idx = (uint32_t)sh.list[w.i].idx();
-  uint64_t cum = 0;
 #pragma unroll 4
-  for (int j = w.j0; j < w.j1; ++j) {
-    const Entry o = sh.list[j];
-    cum += (uint32_t)o.idx() <= idx ? o.w : (uint64_t)0;
-  }
-  if (w.i < n) atomicAdd(&sh.before[w.i], (unsigned long long)cum);
+  for (int j = w.j0; j < w.j1; ++j) place += (uint32_t)sh.list[j].idx() < idx;
+  if (w.i < n) atomicAdd(&sh.rank[w.i], place);
   __syncthreads();
-  // the lowest index past the target; else the highest kept one
-  const uint32_t at = (uint32_t)mine.idx();
-  const bool live = i < n && mine.w;
-  const uint32_t low = wave_min(live && (double)sh.before[i < RANK ? i : 0] > target ? at : 0xffffffffu);
-  const uint32_t high = wave_min(live ? ~at : 0xffffffffu);
-  if ((i & 63) == 0) {
-    atomicMin(&sh.kmin, low);
-    atomicMin(&sh.ties, high);
+  double* weights = (double*)sh.before;
+  uint32_t* indices = sh.hc;
+  static_assert(BINS >= RANK, "the histogram is done with");
+  if (i < n) {
+    weights[sh.rank[i]] = mine;
+    indices[sh.rank[i]] = at;
   }
   __syncthreads();
-  const uint32_t pick = sh.kmin != 0xffffffffu ? sh.kmin : ~sh.ties;
-  if (live && at == pick) {
-    a.out[b] = (int32_t)pick;
-    if (a.prob) a.prob[b] = (float)((double)mine.w / total);
+  const double x = i < n ? weights[i] : 0.0;
+  double total;
+  const double cum = block_scan(x, sh.scan_d, total);
+  const double target = (double)a.u[b] * total;
+  // the lowest index past the target; else the highest with weight
+  const int hit = first_of(x > 0 && cum > target ? i : -1), last = last_of(x > 0 ? i : -1);
+  if (lane == 0) { sh.wave_hit[wave] = hit; sh.wave_any[wave] = last; }
+  __syncthreads();
+  int pick = -1, end = -1;
+#pragma unroll
+  for (int v = 0; v < WAVES; ++v) {
+    if (pick < 0) pick = sh.wave_hit[v];
+    end = max(end, sh.wave_any[v]);
+  }
+  if (i == (pick >= 0 ? pick : end)) {
+    a.out[b] = (int32_t)indices[i];
+    if (a.prob) a.prob[b] = (float)(x / total);
   }
 }
 
@@ -1606,8 +1611,10 @@ __global__ void __launch_bounds__(THREADS) finish_passes_kernel(Args a) {
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const Entry e = list[i];
       if (e.key() > t) {
+        // (a weight below the unit counts as one: a kept score can be the first or the last of its row)
         const float x = score_of(e.key());
-        if (!r.cut_min || weight(x, st.M, r.c) >= r.minp) plus_mass(e.idx() / SEG, mass(x, st.M, r.c, lshift));
+        const double w = weight(x, st.M, r.c);
+        if (w > 0 && (!r.cut_min || w >= r.minp)) plus_mass(e.idx() / SEG, max(mass(x, st.M, r.c, lshift), (uint64_t)1));
       } else if (e.key() == t && ties) {
         plus_tie(e.idx() / SEG);
       }

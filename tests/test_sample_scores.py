@@ -451,3 +451,27 @@ def test_the_tail_of_very_long_rows(bits, p_best):
         # weights are good to 1.1e-12 each, sums to 2^-61 for each segment of 256
         assert abs(int(i[0]) - ((u * total - 1) / w + 1)) <= 1.5
         assert abs(float(p[0]) * total / w - 1) <= 2.0**-23
+
+
+def check_ends(n, dev):
+    """u at and outside the ends of its range: the first and the last kept score, however small their weights are."""
+    g = torch.Generator().manual_seed(n)
+    u = torch.tensor([0.0, -1.0, 1.0, float("nan"), 1 - 2.0**-24, 2.0])
+    S = -30 - 50 * torch.rand(6, n, generator=g)
+    S[torch.arange(6), torch.randint(n // 4, n // 2, (6,), generator=g)] = 0.0
+    for kw in (dict(), dict(top_k=2), dict(top_k=40), dict(top_k=200), dict(top_k=n // 2), dict(top_k=n - 1),
+               dict(min_p=1e-30), dict(top_k=40, min_p=1e-25), dict(top_k=n // 2, min_p=1e-25)):
+        check(S, u, dev, near_ok=True, **kw)
+    S += 3.0  # nor does the best score's own value matter
+    check(S, u, dev, near_ok=True, top_k=n // 2)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("n", [50, 300, 2000, 9000, 40000])
+def test_ends_of_rows_of_tiny_weights(dev, n):
+    check_ends(n, dev)
+
+
+@pytest.mark.gpu
+def test_ends_of_long_rows_of_tiny_weights():
+    check_ends(1_200_003, "cuda")
