@@ -399,7 +399,10 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
   const bool exact = r.direct() && !r.cut_min;
   // rows that cut by mass: fp32 sums, for the unit of their masses and to place the histogram's bins
   const bool rough = r.by_mass();
-  const float cf = fminf(fmaxf((float)r.c, 0x1p-100f), 0x1p100f);  // (no NaN from 0 * inf)
+  // A sum may be too large (it costs the masses bits), never too small (they would pass 64 bits): a temperature at
+  // which scores that differ by more than fp32's range may still have weight gives every score 1.
+  const bool flat = r.c < 0x1p-100;
+  const float cf = fminf((float)r.c, 0x1p100f);
   Raw<T> raw[STAT_SEGS];
   load_segs<T, STAT_SEGS>(a, b, lane, seg0, 1, raw);
   float ms = -INFINITY;
@@ -420,12 +423,13 @@ __global__ void __launch_bounds__(256) stats_kernel(Args a) {
       if (lane == j) ws = w;
     } else if (rough) {
       float w = 0;  // (nothing reads that of a segment without scores)
-      if (m < INFINITY) {
+      if (m < INFINITY && !flat) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) w += __builtin_amdgcn_exp2f((v[i] - m) * cf);
       } else {
+        const float least = m < INFINITY ? -__FLT_MAX__ : m;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w += v[i] == m ? 1.f : 0.f;
+        for (int i = 0; i < 4; ++i) w += v[i] >= least ? 1.f : 0.f;
       }
       w = wave_sum(w);
       if (lane == j) ws = w;

@@ -475,3 +475,18 @@ def test_ends_of_rows_of_tiny_weights(dev, n):
 @pytest.mark.gpu
 def test_ends_of_long_rows_of_tiny_weights():
     check_ends(1_200_003, "cuda")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("n", [3000, 40000])
+def test_scores_apart_by_more_than_the_type_holds(dev, n):
+    """Differences past fp32's range that a temperature past it makes small again."""
+    S, u = scores(4, n, seed=n + 1, masked=0.1)
+    S = S.clamp(-8, 8) * 4e37
+    S[1] = -3e38
+    S[1, ::256] = 3e38  # one score of each 256
+    S[2] = torch.finfo(torch.float32).min
+    S[2, ::300] = 1.0
+    for T in (1e39, 3e38, 1e300, [3e38] * 4):
+        for kw in (dict(), dict(top_p=0.61), dict(top_k=n // 2, top_p=0.61), dict(min_p=0.2), dict(top_p=0.61, min_p=0.2)):
+            check(S, u, dev, near_ok=True, temperature=T, **kw)
