@@ -410,9 +410,9 @@ void gather_rows(bool vec, const RowShape& s, hipStream_t st, const uint8_t* dat
 FPS_API int fps_mx_set_rows(const void* x, int type, const void* idx, int idx64, int64_t n, int D, int64_t rows,
                             void* data, void* scale, int bits, int32_t* owner, void* stream) {
   if (n <= 0 || rows <= 0) return 0;
-  if (D <= 0 || (bits != 4 && bits != 8) || type < 0 || type > 2 || n > INT32_MAX) return (int)hipErrorInvalidValue;
+  if (D <= 0 || D > INT32_MAX - MX_BLOCK || (bits != 4 && bits != 8) || type < 0 || type > 2) return (int)hipErrorInvalidValue;
   const bool claim = idx != nullptr && n > 1;
-  if (claim && owner == nullptr) return (int)hipErrorInvalidValue;
+  if (claim && (owner == nullptr || n > INT32_MAX)) return (int)hipErrorInvalidValue;  // (claims are 32-bit)
   hipStream_t st = (hipStream_t)stream;
   if (claim && n <= FEW_ROWS) {
     hipLaunchKernelGGL(mx_claim_few_kernel, dim3(1), dim3(1024), 0, st, idx, idx64, (int)n, rows, owner);
@@ -440,7 +440,7 @@ FPS_API int fps_mx_set_rows(const void* x, int type, const void* idx, int idx64,
 FPS_API int fps_mx_gather_rows(const void* data, const void* scale, int64_t rows, int D, int bits, const void* idx,
                                int idx64, int64_t n, void* out, int type, void* stream) {
   if (n <= 0) return 0;
-  if (D <= 0 || (bits != 4 && bits != 8) || type < 0 || type > 2) return (int)hipErrorInvalidValue;
+  if (D <= 0 || D > INT32_MAX - MX_BLOCK || (bits != 4 && bits != 8) || type < 0 || type > 2) return (int)hipErrorInvalidValue;
   hipStream_t st = (hipStream_t)stream;
   const RowShape s = row_shape(n, D, type == T_F32 ? MX_BLOCK / 4 : MX_BLOCK / 8);
   const bool vec = wide(out, D, type);

@@ -32,6 +32,7 @@ MX_BLOCK = 32
 #: bits per element of a table format
 MX_FORMATS = {"fp4": 4, "fp8": 8}
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT_MAX = 2**31 - 1  # (of the kernels' 32-bit sizes)
 
 
 _pkg = sys.modules[__package__]  # (for the debug switch; an import inside the calls costs a microsecond)
@@ -73,7 +74,7 @@ class MXTable:
     def _layout(rows: int, dim: int, fmt: str):
         if fmt not in MX_FORMATS:
             raise ValueError(f"MXTable: format must be one of {tuple(MX_FORMATS)}, not {fmt!r}")
-        if dim < 1 or rows < 0:
+        if dim < 1 or rows < 0 or dim > _INT_MAX - MX_BLOCK:
             raise ValueError(f"MXTable: {rows} rows of {dim} values")
         return MX_FORMATS[fmt], (dim + MX_BLOCK - 1) // MX_BLOCK
 
@@ -158,6 +159,8 @@ def mx_set_rows(table: MXTable, idx: Optional[torch.Tensor], rows: torch.Tensor)
         idx = _index("mx_set_rows", table, idx)
         if idx.numel() != n:
             raise ValueError(f"mx_set_rows: {idx.numel()} indices for {n} rows")
+        if n > _INT_MAX:
+            raise ValueError(f"mx_set_rows: {n} indexed rows in one write, at most 2^31 - 1")
     if not rows.is_cuda:
         R.mx_set_rows(table.data, table.scale, table.bits, idx, rows)
         return table
@@ -218,6 +221,8 @@ def mx_score(Q, X: MXTable, out: Optional[torch.Tensor] = None, out_dtype=torch.
         B, dim = Q.shape
     if dim != X.dim:
         raise ValueError(f"mx_score: queries of {dim} values, table rows of {X.dim}")
+    if B > _INT_MAX:
+        raise ValueError(f"mx_score: {B} queries in one call, at most 2^31 - 1")
     if out is None:
         if out_dtype not in _TYPE:
             raise ValueError(f"mx_score: out_dtype must be fp32, bf16 or fp16, not {out_dtype}")

@@ -14,7 +14,7 @@ import torch
 
 from . import _native as N
 from . import reference as R
-from .mx import _TYPE, _launch, _same_device
+from .mx import _INT_MAX, _TYPE, _launch, _same_device
 
 Setting = Union[float, int, torch.Tensor]
 
@@ -63,8 +63,8 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
     if u.dtype != torch.float32 or tuple(u.shape) != (B,) or not u.is_contiguous():
         raise ValueError(f"sample_scores: u must be contiguous fp32 [{B}], got {u.dtype} {tuple(u.shape)}")
     _same_device("sample_scores", S, u)
-    if n > 2**31 - 1 or (B > 65535 and n > 16384):
-        raise ValueError(f"sample_scores: {B} rows of {n} scores: rows of up to 2^31 - 1, at most 65535 rows longer than "
+    if n > _INT_MAX or B > _INT_MAX or (B > 65535 and n > 16384):
+        raise ValueError(f"sample_scores: {B} rows of {n} scores: up to 2^31 - 1 of each, at most 65535 rows longer than "
                          "16384")
     t, t0 = _setting("temperature", temperature, B, S, torch.float32, 0.0, math.inf)
     k, k0 = _setting("top_k", top_k, B, S, torch.int32, 0, 2**62)

@@ -256,3 +256,28 @@ def test_writes_from_two_streams_to_different_slots():
     v = t.values()
     same(v[0::2], oracle(a.double().numpy(), "fp8"))
     same(v[1::2], oracle(b.double().numpy(), "fp8"))
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The kernels count queries, claimed rows and a row's values in 32 bits: a size past that is refused, not wrapped
+    (tensors without memory: nothing but their shapes is looked at)."""
+    many = 2**31 + 5
+    t = ops.MXTable(4, 64, device="meta")
+    for f in (lambda: ops.MXTable(1, 2**32 + 64), lambda: ops.MXTable(1, 2**31),
+              lambda: ops.MXTable.from_rows(torch.empty(1, 2**32 + 64, device="meta")),
+              lambda: ops.mx_set_rows(t, torch.empty(many, dtype=torch.int32, device="meta"),
+                                      torch.empty(many, 64, device="meta")),
+              lambda: ops.mx_score(torch.empty(many, 64, dtype=torch.bfloat16, device="meta"), t)):
+        with pytest.raises(ValueError):
+            f()
+
+
+@pytest.mark.gpu
+def test_more_rows_in_order_than_32_bits_count():
+    n = 2**31 + 70
+    x = torch.zeros(n, 1, dtype=torch.bfloat16, device="cuda")
+    for r, v in ((0, 1.0), (2**31 - 1, 2.0), (2**31, 3.0), (n - 1, -4.0)):
+        x[r].fill_(v)
+    t = ops.MXTable.from_rows(x, "fp4")
+    at = torch.tensor([0, 1, 2**31 - 1, 2**31, 2**31 + 1, n - 1, n], device="cuda")
+    assert ops.mx_gather_rows(t, at).flatten().tolist() == [1.0, 0.0, 2.0, 3.0, 0.0, -4.0, 0.0]

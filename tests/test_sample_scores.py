@@ -490,3 +490,10 @@ def test_scores_apart_by_more_than_the_type_holds(dev, n):
     for T in (1e39, 3e38, 1e300, [3e38] * 4):
         for kw in (dict(), dict(top_p=0.61), dict(top_k=n // 2, top_p=0.61), dict(min_p=0.2), dict(top_p=0.61, min_p=0.2)):
             check(S, u, dev, near_ok=True, temperature=T, **kw)
+
+
+def test_row_counts_past_32_bits_are_refused():
+    """(tensors without memory: nothing but their shapes is looked at)"""
+    for B, n in ((2**31 + 5, 1), (2**32 + 3, 2), (3, 2**31)):
+        with pytest.raises(ValueError):
+            ops.sample_scores(torch.empty(B, n, device="meta"), torch.empty(B, device="meta"))
