@@ -1708,13 +1708,30 @@ int list_cap(int64_t N) { return (int)(N / 8 < 16384 ? N / 8 : 16384); }
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
+// How many rounds of passes can a row need?  (Scalars decide here, per-row settings on the device.)
+int rounds_of(int64_t N, const float* temperature, double temperature0, const int32_t* top_k, int64_t top_k0,
+              const float* top_p, double top_p0, const float* min_p, double min_p0) {
+  const bool greedy = !temperature && !(temperature0 > 0);
+  const bool can_long_k = !greedy && (top_k || (top_k0 > SHORT_K && top_k0 < N));
+  const bool can_no_k = !greedy && (top_k || top_k0 <= 0 || top_k0 >= N);
+  const bool can_p = top_p || top_p0 < 1, can_min = min_p || min_p0 > 0;
+  return can_long_k && can_p ? 2 : can_long_k || (can_no_k && (can_p || can_min)) ? 1 : 0;
+}
+
 }  // namespace
 
-// bytes of workspace for B rows of N scores
-FPS_API int64_t fps_sample_scores_ws_bytes(int64_t B, int64_t N) {
+// bytes of workspace for B rows of N scores with these settings (as below); what only the passes use is left
+// out where no row can take them
+FPS_API int64_t fps_sample_scores_ws_bytes(int64_t B, int64_t N, const float* temperature, double temperature0,
+                                           const int32_t* top_k, int64_t top_k0, const float* top_p, double top_p0,
+                                           const float* min_p, double min_p0) {
   if (B <= 0 || N <= kShortRow) return 0;
   const int64_t nseg = (N + SEG - 1) / SEG;
-  return B * (list_cap(N) * (int64_t)sizeof(Entry)) + round16(B * sizeof(RowState)) + B * BINS * 8 + B * nseg * (nseg > KEPT ? 24 : 16) + 16;
+  int64_t bytes = B * nseg * 16 + 16;
+  if (rounds_of(N, temperature, temperature0, top_k, top_k0, top_p, top_p0, min_p, min_p0))
+    bytes += B * (list_cap(N) * (int64_t)sizeof(Entry)) + round16(B * sizeof(RowState)) + B * BINS * 8 +
+             (nseg > KEPT ? B * nseg * 8 : 0);
+  return bytes;
 }
 
 // s [B, N] (row stride ld, type 0 fp32 / 1 bf16 / 2 fp16); u [B]; temperature / top_k / top_p /
@@ -1740,21 +1757,18 @@ FPS_API int fps_sample_scores(const void* s, int type, int B, int64_t N, int64_t
   int rounds = 0;
   if (N > kShortRow) {
     if (ws == nullptr || ((uintptr_t)ws & 15)) return (int)hipErrorInvalidValue;
-    a.listcap = list_cap(N);
+    rounds = rounds_of(N, temperature, temperature0, top_k, top_k0, top_p, top_p0, min_p, min_p0);
     char* p = (char*)ws;
-    a.list = (Entry*)p; p += (int64_t)B * a.listcap * sizeof(Entry);
-    a.state = (RowState*)p; p += round16(B * sizeof(RowState));
-    a.hmass = (uint64_t*)p; p += (int64_t)B * BINS * 8;
+    if (rounds) {
+      a.listcap = list_cap(N);
+      a.list = (Entry*)p; p += (int64_t)B * a.listcap * sizeof(Entry);
+      a.state = (RowState*)p; p += round16(B * sizeof(RowState));
+      a.hmass = (uint64_t*)p; p += (int64_t)B * BINS * 8;
+      if (a.nseg > KEPT) { a.listed = (uint64_t*)p; p += (int64_t)B * a.nseg * 8; }
+    }
     a.segmass = (double*)p; p += (int64_t)B * a.nseg * 8;
-    if (a.nseg > KEPT) { a.listed = (uint64_t*)p; p += (int64_t)B * a.nseg * 8; }
     a.segmax = (float*)p; p += (int64_t)B * a.nseg * 4;
     a.segtie = (int32_t*)p;
-    // which rounds of passes can a row need?  (scalars decide here, per-row settings on the device)
-    const bool greedy = !temperature && !(temperature0 > 0);
-    const bool can_long_k = !greedy && (top_k || (top_k0 > SHORT_K && top_k0 < N));
-    const bool can_no_k = !greedy && (top_k || top_k0 <= 0 || top_k0 >= N);
-    const bool can_p = top_p || top_p0 < 1, can_min = min_p || min_p0 > 0;
-    rounds = can_long_k && can_p ? 2 : can_long_k || (can_no_k && (can_p || can_min)) ? 1 : 0;
   }
   hipStream_t st = (hipStream_t)stream;
   const auto launch = [&] {

@@ -107,7 +107,7 @@ _SIGNATURES = {
     "fps_mx_set_rows": [c_vp, c_int, c_vp, c_int, c_i64, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_vp],
     "fps_mx_gather_rows": [c_vp, c_vp, c_i64, c_int, c_int, c_vp, c_int, c_i64, c_vp, c_int, c_vp],
     "fps_mx_score": [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_i64, c_int, c_vp, c_int, c_i64, c_vp],
-    "fps_sample_scores_ws_bytes": [c_i64, c_i64],
+    "fps_sample_scores_ws_bytes": [c_i64, c_i64, c_vp, c_double, c_vp, c_i64, c_vp, c_double, c_vp, c_double],
     "fps_sample_scores": [c_vp, c_int, c_int, c_i64, c_i64, c_vp, c_vp, c_double, c_vp, c_i64, c_vp, c_double, c_vp,
                           c_double, c_vp, c_vp, c_vp, c_vp],
     "fps_sgns_rows": [c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp],

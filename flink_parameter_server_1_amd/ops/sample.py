@@ -17,6 +17,7 @@ from . import reference as R
 from .mx import _INT_MAX, _TYPE, _launch, _same_device
 
 Setting = Union[float, int, torch.Tensor]
+_SHORT_ROW = 16384  # rows up to this are one workgroup's, without a workspace (the kernel library's own border)
 
 
 def _setting(name: str, v: Setting, B: int, S: torch.Tensor, dtype, lo: float, hi: float):
@@ -63,9 +64,9 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
     if u.dtype != torch.float32 or tuple(u.shape) != (B,) or not u.is_contiguous():
         raise ValueError(f"sample_scores: u must be contiguous fp32 [{B}], got {u.dtype} {tuple(u.shape)}")
     _same_device("sample_scores", S, u)
-    if n > _INT_MAX or B > _INT_MAX or (B > 65535 and n > 16384):
+    if n > _INT_MAX or B > _INT_MAX or (B > 65535 and n > _SHORT_ROW):
         raise ValueError(f"sample_scores: {B} rows of {n} scores: up to 2^31 - 1 of each, at most 65535 rows longer than "
-                         "16384")
+                         f"{_SHORT_ROW}")
     t, t0 = _setting("temperature", temperature, B, S, torch.float32, 0.0, math.inf)
     k, k0 = _setting("top_k", top_k, B, S, torch.int32, 0, 2**62)
     p, p0 = _setting("top_p", top_p, B, S, torch.float32, 0.0, 1.0)
@@ -83,9 +84,11 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
         if with_prob:
             prob.copy_(q)
     elif B:
-        size = N.require().fps_sample_scores_ws_bytes(B, n) if n > 16384 else 0
-        ws = torch.empty(size, dtype=torch.uint8, device=S.device) if size else None
+        settings = (N.ptr(t), t0, N.ptr(k), k0, N.ptr(p), p0, N.ptr(m), m0)
+        ws = None
+        if n > _SHORT_ROW:
+            size = N.require().fps_sample_scores_ws_bytes(B, n, *settings)
+            ws = torch.empty(size, dtype=torch.uint8, device=S.device)
         _launch("sample_scores", S.get_device(), S.data_ptr(), _TYPE[S.dtype], B, n, S.stride(0) if B > 1 else n,
-                u.data_ptr(), N.ptr(t), t0, N.ptr(k), k0, N.ptr(p), p0, N.ptr(m), m0, out.data_ptr(), N.ptr(prob),
-                N.ptr(ws))
+                u.data_ptr(), *settings, out.data_ptr(), N.ptr(prob), N.ptr(ws))
     return (out, prob) if with_prob else out

@@ -497,3 +497,38 @@ def test_row_counts_past_32_bits_are_refused():
     for B, n in ((2**31 + 5, 1), (2**32 + 3, 2), (3, 2**31)):
         with pytest.raises(ValueError):
             ops.sample_scores(torch.empty(B, n, device="meta"), torch.empty(B, device="meta"))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 16383, 16384, 16385])
+@pytest.mark.parametrize("case", range(len(SETTINGS)))
+def test_lengths_at_which_the_path_changes(dev, n, case):
+    """A segment per wave in registers up to 2048 scores, one launch without a workspace up to 16384."""
+    S, u = scores(2, n, seed=5000 * case + n)
+    check(S, u, dev, **SETTINGS[case])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1_048_576, 1_048_577])
+@pytest.mark.parametrize("case", [0, 4, 5, 7, 17, 18, 20])
+def test_lengths_at_which_maxima_leave_lds(n, case):
+    S, u = scores(1, n, seed=6000 * case + n)
+    check(S, u, "cuda", **SETTINGS[case])
+
+
+def test_workspace_by_length_and_settings():
+    from flink_parameter_server_1_amd.ops import _native
+    from flink_parameter_server_1_amd.ops.sample import _SHORT_ROW
+
+    if not _native.available():
+        pytest.skip("kernel library not built")
+
+    def size(B, n, T=1.0, k=0, p=1.0, q=0.0):
+        return _native.require().fps_sample_scores_ws_bytes(B, n, None, T, None, k, None, p, None, q)
+
+    assert size(5, _SHORT_ROW, p=0.5) == 0 < size(5, _SHORT_ROW + 1)
+    n, segments = 131072, 512
+    for kw in (dict(), dict(T=0.0, p=0.5, q=0.5), dict(k=100, p=0.9, q=0.1), dict(k=n), dict(T=0.0, k=5000)):
+        assert size(256, n, **kw) <= 256 * segments * 16 + 16  # a maximum, a mass, a count per segment
+    for kw in (dict(p=0.9), dict(q=0.1), dict(k=5000), dict(k=n, p=0.9)):
+        assert size(256, n, **kw) > 256 * 16384 * 16
