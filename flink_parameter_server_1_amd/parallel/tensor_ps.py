@@ -229,7 +229,8 @@ class TensorPS:
         device-bound pipeline that is plain back-pressure), host_stalls = the subset
         where nothing had been enqueued after those counts -- the device drains and
         idles while the host waits (``plan()`` back to back, or a pipeline without
-        lookahead)."""
+        lookahead).  A model load's own wait for its counts is in neither: whether they
+        had arrived says nothing about the run."""
         if self._lazy:
             for k, parts in self._lazy.items():
                 self._stats[k] += int(torch.stack(parts).sum().item())
@@ -850,7 +851,9 @@ class TensorPS:
         to their owning shards and written there (last record of an id wins).
         Collective."""
         vals = values.to(device=self.table.device, dtype=torch.float32).reshape(ids.numel(), self.table.dim)
+        waits = {k: self._stats[k] for k in ("host_waits", "host_stalls")}
         self.push_keys(ids, vals, op="set")
+        self._stats.update(waits)  # of the run, not of what was loaded before it
 
     def pull_values(self, keys: torch.Tensor) -> torch.Tensor:
         """Convenience: fp32 ``[B, D]`` values for every request (expanded)."""

@@ -461,3 +461,54 @@ def test_rank_without_worker_refuses_input():
     with pytest.raises(ValueError, match="runs no worker"):
         rt2.submit(torch.tensor([3]))
     rt2.submit(None)  # taking part without data is fine
+
+
+class _LateEvent:
+    """Counts that are never on the host yet when ``plan_end`` looks."""
+
+    def query(self):
+        return False
+
+    def synchronize(self):
+        pass
+
+
+def _late_counts(rank, world, capacity):
+    from flink_parameter_server_1_amd.parallel import tensor_ps
+
+    pending = tensor_ps.TensorPS._pending
+
+    def late(self, *args, **kw):
+        pp = pending(self, *args, **kw)
+        pp.event = _LateEvent()
+        return pp
+
+    tensor_ps.TensorPS._pending = late
+    try:
+        return _model_load(rank, world, 50, 0, None, capacity)
+    finally:
+        tensor_ps.TensorPS._pending = pending
+
+
+def test_a_model_load_is_no_host_wait_of_the_run():
+    """The load plans its keys with a count exchange and may wait for it; the run's fixed-shape plans never do, and the
+    statistics (asserted in ``_model_load``) are the run's, whenever the load's counts arrived."""
+    dump = _dump_of(run_ranks(_late_counts, 2, 7))
+    assert dump == {k: 10.0 * k + 3 for k in range(50)}
+
+
+def test_a_plan_that_waits_is_counted():
+    from flink_parameter_server_1_amd.parallel.comm import Comm
+    from flink_parameter_server_1_amd.parallel.tensor_ps import TensorPS
+
+    logic = DeviceSimplePSLogicWithClose(10, 1, op="add")
+    TensorRuntime(Comm()).execute([torch.tensor([1, 2])], _CountWorker(), logic, model=[(3, [1.0])])
+    ps = logic.ps
+    assert isinstance(ps, TensorPS)
+    before = ps.stats["host_waits"]
+    pp = ps.plan_begin(torch.tensor([1, 2, 3]), fixed=False)
+    if pp.static:
+        pytest.skip("static plans at world 1 wait for nothing")
+    pp.event = _LateEvent()
+    ps.plan_end(pp)
+    assert ps.stats["host_waits"] == before + 1 and ps.stats["host_stalls"] >= 1
