@@ -185,8 +185,8 @@ __device__ __forceinline__ uint64_t mass(float s, float M, double c, int shift, 
   const uint64_t bits = (uint64_t)__double_as_longlong(w.p);
   uint64_t m = (bits << 10 & 0x3fffffffffffffffull) | 1ull << 62;
   const int down = 63 - shift - w.n - (int)(bits >> 52 & 1);  // (p in [1, 2) or [1/2, 1))
-  m += ((uint64_t)place << 56) >> (64 - min(down, 63));
-  return down > 63 ? 0 : m >> down;
+  m += ((uint64_t)place << 56) >> (-down & 63);  // (down in 1 .. 63; past that nothing is left)
+  return down > 63 ? 0 : m >> (down & 63);
 }
 // The unit for a row whose weights sum up to `total` at most (and 1 at least): all masses together stay
 // below 2^62, and what rounding takes from N scores is about 2^-69 N of a total that is known to a factor
