@@ -3,7 +3,8 @@
 //   S[b, i] = sum_d Q[b, d] X[i, d]      X: E2M1 or E4M3 blocks of 32 with a power of two each
 //
 // Two forms.  bf16 queries: X's elements become bf16 in registers, their block's power of two
-// included (exact), and v_mfma_f32_32x32x16_bf16 sums in fp32.  Queries in E2M1 blocks
+// included (exact down to bf16's smallest subnormal, 2^-133, which only E4M3 blocks of scale bytes below 3
+// pass), and v_mfma_f32_32x32x16_bf16 sums in fp32.  Queries in E2M1 blocks
 // against an E2M1 table: v_mfma_scale_f32_32x32x64_f8f6f4 on the packed elements.  (An
 // 8-bit table takes the bf16 form too: the 8-bit matrix instructions keep only about 2^-13
 // of the sum of magnitudes on this card, the 4-bit and the bf16 ones 2^-24.)

@@ -204,8 +204,10 @@ def mx_score(Q, X: MXTable, out: Optional[torch.Tensor] = None, out_dtype=torch.
 
     ``Q``: bf16 queries ``[B, dim]`` (contiguous), or an fp4 ``MXTable`` against an fp4 ``X`` (both
     sides in 4 bits).  ``out``: fp32 / bf16 / fp16 ``[B, rows]``, its rows may be strided (a column
-    slice of a wider score matrix).  Sums are held in fp32 and rounded once.  A NaN in a query row or
-    a NaN block in a table row makes its scores NaN."""
+    slice of a wider score matrix).  Sums are held in fp32 and rounded once.  Against bf16 queries a
+    table's values take part as bf16: exact, but for elements of fp8 blocks whose largest value is below
+    2^-116, which are rounded to whole multiples of 2^-133.  A NaN in a query row or a NaN block in a
+    table row makes its scores NaN."""
     mx = isinstance(Q, MXTable)
     if not isinstance(X, MXTable):
         raise ValueError("mx_score: X must be an MXTable")

@@ -208,3 +208,21 @@ def test_replayed_scores_equal_eager_ones():
         torch.cuda.synchronize()
         assert torch.equal(out, ops.mx_score(Q, X))
     assert want.shape == out.shape
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("B,dim", [(3, 64), (70, 300), (5, 1024)])
+@pytest.mark.parametrize("e", [-126, -122, -117, -112])
+def test_rows_next_to_the_smallest_numbers(dev, form, B, dim, e):
+    """Rows of about 2^e against queries that bring their products back: against bf16 queries a value is off by half of
+    bf16's smallest subnormal, 2^-134, at most."""
+    q, x = make(B, dim, 31, 0.3) * 2.0**110, make(200, dim, 32, 0.3) * 2.0**e
+    X = ops.MXTable.from_rows(x.to(dev), form[1])
+    Q = q.to(dev).bfloat16() if form[0] == "bf16" else ops.MXTable.from_rows(q.to(dev))
+    S = ops.mx_score(Q, X).cpu().double()
+    qv, xv = floats(Q), floats(X)
+    bound = 2 * dim * 2.0**-24 * (qv.abs() @ xv.abs().t())
+    if form == ("bf16", "fp8"):
+        bound = bound + qv.abs().sum(1, keepdim=True) * 2.0**-134
+    assert bool(((S - qv @ xv.t()).abs() <= bound).all())
