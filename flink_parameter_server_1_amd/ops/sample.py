@@ -50,7 +50,8 @@ def sample_scores(S: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, 
     order, exceeds ``u`` times their total; ``u`` fp32 ``[B]`` in [0, 1) (below: the first kept index,
     above or NaN: the last).  ``temperature = 0`` takes the largest score, lowest index.  A score of
     -inf or NaN is masked; a row with nothing left answers -1.  If a row holds +inf, only its +inf
-    scores have weight.  Weights and sums are held in 64 bits.
+    scores have weight.  Weights and sums are held in 64 bits: where ``u`` times the total (or ``top_p`` times it) falls
+    within about 1e-12 of the total from a step, either side may be taken.
 
     Every setting is a number or a per-row tensor (fp32 ``[B]``; ``top_k`` int32 ``[B]``).  Per-row
     values are not checked: a temperature that is not above 0 is greedy, a ``top_k`` <= 0, a ``top_p``
