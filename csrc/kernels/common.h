@@ -18,6 +18,9 @@ namespace fps {
 
 constexpr int kWave = 64;
 
+// element types as the launchers of the microscaled-table and sampling operators get them
+enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
 // butterfly sum over groups of G lanes (G power of two <= 64)

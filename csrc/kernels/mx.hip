@@ -32,8 +32,6 @@ namespace {
 constexpr int VPL = 8;            // values per lane of a write
 constexpr int LPB = MX_BLOCK / VPL;  // lanes per block
 
-enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
-
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 

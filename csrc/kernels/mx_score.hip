@@ -37,8 +37,6 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
-
 constexpr int WAVES = 4;      // waves per workgroup
 constexpr int THREADS = WAVES * 64;
 
@@ -210,48 +208,48 @@ __device__ __forceinline__ void multiply(const uint8_t* qrow, const uint8_t* qsr
 #pragma unroll
   for (int t = 0; t < IT; ++t) sc[t] = cur.scales(t);
 #pragma unroll
-        for (int j = 0; j < CS; ++j) {
-          if (j < S) {
-            if constexpr (Q4) {
-              i32x8 qa[QT];
-              int qsc[QT];
+  for (int j = 0; j < CS; ++j) {
+    if (j < S) {
+      if constexpr (Q4) {
+        i32x8 qa[QT];
+        int qsc[QT];
 #pragma unroll
-              for (int q = 0; q < QT; ++q) {
-                const uint4 v = *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 16);
-                qa[q] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-                qsc[q] = qsrow[q * 32 * SSTRIDE + first + j];
-              }
+        for (int q = 0; q < QT; ++q) {
+          const uint4 v = *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 16);
+          qa[q] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+          qsc[q] = qsrow[q * 32 * SSTRIDE + first + j];
+        }
 #pragma unroll
-              for (int t = 0; t < IT; ++t) {
-                const uint4 v = cur.b[t][j].v;
-                const i32x8 xb = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+        for (int t = 0; t < IT; ++t) {
+          const uint4 v = cur.b[t][j].v;
+          const i32x8 xb = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
 #pragma unroll
-                for (int q = 0; q < QT; ++q)
-                  acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
-                                                                              (int)(sc[t] >> (8 * j)));
-              }
-            } else {
-              float f[IT];
+          for (int q = 0; q < QT; ++q)
+            acc[t][q] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qa[q], xb, acc[t][q], 4, 4, 0, qsc[q], 0,
+                                                                        (int)(sc[t] >> (8 * j)));
+        }
+      } else {
+        float f[IT];
 #pragma unroll
-              for (int t = 0; t < IT; ++t) {
-                const uint32_t s = (sc[t] >> (8 * j)) & 255u;
-                f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
-              }
+        for (int t = 0; t < IT; ++t) {
+          const uint32_t s = (sc[t] >> (8 * j)) & 255u;
+          f[t] = s == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(s);
+        }
 #pragma unroll
-              for (int s = 0; s < 4; ++s) {
-                bf16x8 xb[IT];
+        for (int s = 0; s < 4; ++s) {
+          bf16x8 xb[IT];
 #pragma unroll
-                for (int t = 0; t < IT; ++t) xb[t] = to_bf16(cur.b[t][j], s, f[t]);
+          for (int t = 0; t < IT; ++t) xb[t] = to_bf16(cur.b[t][j], s, f[t]);
 #pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                  const bf16x8 qa = __builtin_bit_cast(bf16x8, *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 64 + s * 16));
+          for (int q = 0; q < QT; ++q) {
+            const bf16x8 qa = __builtin_bit_cast(bf16x8, *(const uint4*)(qrow + q * 32 * STRIDE + (first + j) * 64 + s * 16));
 #pragma unroll
-                  for (int t = 0; t < IT; ++t) acc[t][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, xb[t], acc[t][q], 0, 0, 0);
-                }
-              }
-            }
+            for (int t = 0; t < IT; ++t) acc[t][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, xb[t], acc[t][q], 0, 0, 0);
           }
         }
+      }
+    }
+  }
 }
 
 // 16-byte pieces 0 .. pieces - 1 of 32 QT queries from block blk0 on to LDS, U in flight a thread

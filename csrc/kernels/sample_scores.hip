@@ -31,8 +31,6 @@ using namespace fps;
 
 namespace {
 
-enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
-
 constexpr int SEG = 256;        // scores per segment: one wave, four a lane
 constexpr int BINS = 2048;
 constexpr int THREADS = 512;    // of a finishing workgroup

@@ -532,3 +532,29 @@ def test_workspace_by_length_and_settings():
         assert size(256, n, **kw) <= 256 * segments * 16 + 16  # a maximum, a mass, a count per segment
     for kw in (dict(p=0.9), dict(q=0.1), dict(k=5000), dict(k=n, p=0.9)):
         assert size(256, n, **kw) > 256 * 16384 * 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dtype", [(1500, torch.float32), (60000, torch.float32), (60000, torch.bfloat16),
+                                     (1_200_003, torch.float32)])
+def test_draws_do_not_depend_on_the_order_of_atomics(n, dtype):
+    """The same call again and again, and captured and replayed: indices and probabilities to the last bit."""
+    S, u = (t.cuda() for t in scores(8, n, seed=n, spread=1.0, dtype=dtype))
+    k = torch.tensor([0, 40, 600, n // 2, n // 3, 0, 7, n - 1], dtype=torch.int32, device="cuda")
+    p = torch.tensor([0.9, 0.8, 1.0, 0.95, 1.0, 1.0, 0.5, 0.99], device="cuda")
+    q = torch.tensor([0.0, 0.0, 0.01, 0.001, 0.0, 0.02, 0.0, 0.0], device="cuda")
+    call = lambda: ops.sample_scores(S, u, top_k=k, top_p=p, min_p=q, with_prob=True)  # noqa: E731
+    i, r = call()
+    for _ in range(20):
+        j, s = call()
+        assert torch.equal(i, j) and torch.equal(r, s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        j, s = call()
+    for _ in range(3):
+        j.fill_(-7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(i, j) and torch.equal(r, s)
+        call()
+        torch.cuda.synchronize()
